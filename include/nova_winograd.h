@@ -187,6 +187,71 @@ int nova_weight_grad_v2(const void* d_input, const void* d_grad_output, void* d_
                         void* d_workspace, long long workspace_bytes, int batch, int C, int K,
                         int H, int W, int pad, void* stream);
 
+/* ---- UNet operators around the convolutions ------------------------------ */
+/* Element types of the UNet operators, and the mask types of the attention
+ * (a bool mask is one byte per key; an additive mask names its element type). */
+enum { NOVA_DTYPE_F16 = 0, NOVA_DTYPE_BF16 = 1, NOVA_DTYPE_F32 = 2 };
+enum { NOVA_MASK_NONE = -1, NOVA_MASK_BOOL = 3 };
+enum { NOVA_ACT_NONE = 0, NOVA_ACT_SILU = 1 };
+
+/* Group normalisation with its activation, channels last.  No reference
+ * counterpart: the reference's UNet callers leave the norm to the host framework
+ * (benchmarks/bench_sd_unet.py:38-109).
+ *   y = act(weight * (u - mean) / sqrt(var + eps) + bias),  u = x + shift[b][c]
+ * x: [batch][pixels][C] of type dtype, pixel_stride >= C and batch_stride in
+ * elements; y (same type) is dense.  weight and bias: [C] of type param_dtype,
+ * each may be NULL (1 and 0).  shift: [batch][C] of type shift_dtype, or NULL.
+ * stats: float[2][batch][groups], mean and 1/sqrt(var + eps), for the gradient;
+ * NULL where it is not wanted.  The caller passes a 256-byte aligned workspace
+ * of nova_group_norm_workspace_bytes() bytes; calls that overlap need one each.
+ * Allocates nothing, never synchronizes, runs on `stream`; returns a NOVA_*
+ * status. */
+long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups, int grad);
+int nova_group_norm_v2(const void* d_input, const void* d_weight, const void* d_bias,
+                       const void* d_shift, void* d_output, void* d_stats, void* d_workspace,
+                       long long workspace_bytes, int batch, int pixels, int C, int groups,
+                       long long batch_stride, long long pixel_stride, int dtype,
+                       int param_dtype, int shift_dtype, int activation, float eps, void* stream);
+/* Gradient.  dy has strides of its own; dx is dense.  grad_weight and grad_bias
+ * (param_dtype) and grad_shift (shift_dtype) may be NULL.  Every sum has a fixed
+ * order: results repeat bit for bit. */
+int nova_group_norm_grad_v2(const void* d_input, const void* d_grad_output, const void* d_weight,
+                            const void* d_bias, const void* d_shift, const void* d_stats,
+                            void* d_grad_input, void* d_grad_weight, void* d_grad_bias,
+                            void* d_grad_shift, void* d_workspace, long long workspace_bytes,
+                            int batch, int pixels, int C, int groups, long long batch_stride,
+                            long long pixel_stride, long long grad_batch_stride,
+                            long long grad_pixel_stride, int dtype, int param_dtype,
+                            int shift_dtype, int activation, void* stream);
+
+/* Cross attention of `queries` tokens to `keys` encoder states.  No reference
+ * counterpart (benchmarks/bench_sdxl.py:38-138 leaves it to the host framework).
+ *   o = softmax(scale * q k^T + mask) v      per batch and head
+ * q: [batch][queries][heads][head_dim], k and v: [batch][keys][heads][head_dim],
+ * FP16 or BF16, head_dim a multiple of 8 up to 160, rows 16-byte aligned.
+ * strides (host array, elements): batch, token, head of q, of k, of v, then batch
+ * and key stride of the mask; the gradient's array goes on with batch, token and
+ * head of grad_output.  Outputs are dense in the layout of q (o, grad_q) and of
+ * k (grad_k, grad_v).  mask: [batch][keys]; a key with false, or with an additive
+ * -inf, takes no part whatever k and v hold there, and a query without keys gets
+ * zeros.  lse: float[batch][heads][queries], the base-2 logarithm of the softmax's
+ * denominator, for the gradient; NULL where it is not wanted.  Workspace, stream
+ * and status as above (a workspace of 0 bytes may be NULL). */
+long long nova_cross_attention_workspace_bytes(int batch, int queries, int keys, int heads,
+                                               int head_dim, int grad);
+int nova_cross_attention_v2(const void* d_q, const void* d_k, const void* d_v, const void* d_mask,
+                            void* d_output, void* d_lse, void* d_workspace,
+                            long long workspace_bytes, int batch, int queries, int keys,
+                            int heads, int head_dim, const long long* strides, int dtype,
+                            int mask_type, float scale, void* stream);
+int nova_cross_attention_grad_v2(const void* d_q, const void* d_k, const void* d_v,
+                                 const void* d_mask, const void* d_output,
+                                 const void* d_grad_output, const void* d_lse, void* d_grad_q,
+                                 void* d_grad_k, void* d_grad_v, void* d_workspace,
+                                 long long workspace_bytes, int batch, int queries, int keys,
+                                 int heads, int head_dim, const long long* strides, int dtype,
+                                 int mask_type, float scale, void* stream);
+
 /* Library version string. */
 const char* nova_version(void);
 

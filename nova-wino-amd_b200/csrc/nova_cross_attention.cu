@@ -1,0 +1,310 @@
+// Cross attention of one set of tokens to an encoder's states of another length.
+//
+//   s = scale q k^T + bias[key],  p = softmax(s) over the keys the mask leaves,  o = p v
+//
+// and its gradient
+//
+//   dv = p^T do,  dp = do v^T,  ds = p (dp - sum(p dp)),  dq = scale ds k,  dk = scale ds^T q
+//
+// q is [B][Nq][H][D], k and v are [B][Nk][H][D] with strides of their own; the
+// outputs are dense.  A key that the mask leaves out (false, or a bias of minus
+// infinity) is never multiplied, whatever its k and v hold; a query without
+// keys gets zeros, and passes no gradient on.
+#include <string>
+
+#include "../../include/nova_winograd.h"
+#include "nova_unet_ops.h"
+
+namespace nova {
+namespace xattn {
+
+using namespace unet;
+
+constexpr int kMaskNone = -1, kMaskBool = 3;  // else the element type of an additive mask
+constexpr int kMaxD = 160;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Strides {
+  long long b, n, h;  // elements
+};
+
+struct Args {
+  const void *q, *k, *v, *dout, *mask;
+  const float* lse_in;
+  void* out;   // o
+  float* lse;  // [B][H][Nq], base 2; minus infinity for a query without keys
+  void *dq, *dk, *dv;
+  const float* delta;  // [B][H][Nq]: sum(p dp)
+  Strides qs, ks, vs, dos;
+  long long mb, mn;  // mask strides
+  int B, Nq, Nk, H, D;
+  int mask_kind;
+  float scale;
+};
+
+// Bias of key n in base 2, and whether the key takes part.  The lowest finite
+// bias stays finite after the change of base, so that a row with nothing else
+// is the uniform row that the definition gives.
+__device__ __forceinline__ bool key_bias(const Args& a, int b, int n, float* bias) {
+  *bias = 0.f;
+  if (a.mask_kind == kMaskNone) return true;
+  const long long i = b * a.mb + n * a.mn;
+  if (a.mask_kind == kMaskBool) return static_cast<const unsigned char*>(a.mask)[i] != 0;
+  const float m = load_param(a.mask, a.mask_kind, i);
+  if (m == -INFINITY) return false;
+  const float t = m * kLog2e;
+  *bias = t == -INFINITY ? -3.402823466e38f : t;
+  return true;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+constexpr int kPer = kMaxD / 32;  // elements of a row that a lane holds
+
+template <typename T>
+__device__ __forceinline__ void load_row(const void* p, long long off, int D, float (&r)[kPer]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    r[i] = lane + 32 * i < D ? to_f32(static_cast<const T*>(p)[off + lane + 32 * i]) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store_row(void* p, long long off, int D, const float (&r)[kPer]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (lane + 32 * i < D) static_cast<T*>(p)[off + lane + 32 * i] = from_f32<T>(r[i]);
+}
+__device__ __forceinline__ float dot(const float (&x)[kPer], const float (&y)[kPer]) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) t = fmaf(x[i], y[i], t);
+  return warp_sum(t);
+}
+
+// One warp for a query: one pass over the keys with the running maximum and sum.
+template <typename T>
+__global__ void __launch_bounds__(128) forward_rows(Args a) {
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (long long)a.B * a.H * a.Nq) return;
+  const int n = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H;
+  float q[kPer], k[kPer], v[kPer], o[kPer] = {};
+  load_row<T>(a.q, b * a.qs.b + n * a.qs.n + h * a.qs.h, a.D, q);
+  const float c = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  for (int j = 0; j < a.Nk; ++j) {
+    float bias;
+    if (!key_bias(a, b, j, &bias)) continue;
+    load_row<T>(a.k, b * a.ks.b + j * a.ks.n + h * a.ks.h, a.D, k);
+    load_row<T>(a.v, b * a.vs.b + j * a.vs.n + h * a.vs.h, a.D, v);
+    const float s = fmaf(dot(q, k), c, bias);
+    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
+    const float f = exp2f(m - base), e = exp2f(s - base);
+    m = top;
+    l = fmaf(l, f, e);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], f, e * v[i]);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] *= inv;
+  store_row<T>(a.out, (((long long)b * a.Nq + n) * a.H + h) * a.D, a.D, o);
+  if (a.lse && (threadIdx.x & 31) == 0) a.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+
+__device__ __forceinline__ float prob(float s, float lse) {
+  return lse == -INFINITY ? 0.f : exp2f(s - lse);
+}
+
+// dq: a warp for a query, two passes over the keys (sum(p dp), then dq).
+template <typename T>
+__global__ void __launch_bounds__(128) grad_queries(Args a, float* delta) {
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (long long)a.B * a.H * a.Nq) return;
+  const int n = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H;
+  float q[kPer], g[kPer], k[kPer], v[kPer], dq[kPer] = {};
+  load_row<T>(a.q, b * a.qs.b + n * a.qs.n + h * a.qs.h, a.D, q);
+  load_row<T>(a.dout, b * a.dos.b + n * a.dos.n + h * a.dos.h, a.D, g);
+  const float c = a.scale * kLog2e, lse = a.lse_in[row];
+  float d = 0.f;
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int j = 0; j < a.Nk; ++j) {
+      float bias;
+      if (!key_bias(a, b, j, &bias)) continue;
+      load_row<T>(a.k, b * a.ks.b + j * a.ks.n + h * a.ks.h, a.D, k);
+      load_row<T>(a.v, b * a.vs.b + j * a.vs.n + h * a.vs.h, a.D, v);
+      const float p = prob(fmaf(dot(q, k), c, bias), lse), dp = dot(g, v);
+      if (pass == 0) {
+        d = fmaf(p, dp, d);
+      } else {
+        const float ds = p * (dp - d) * a.scale;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) dq[i] = fmaf(ds, k[i], dq[i]);
+      }
+    }
+  }
+  store_row<T>(a.dq, (((long long)b * a.Nq + n) * a.H + h) * a.D, a.D, dq);
+  if ((threadIdx.x & 31) == 0) delta[row] = d;
+}
+
+// dk and dv: a warp for a key, one pass over the queries.
+template <typename T>
+__global__ void __launch_bounds__(128) grad_keys(Args a) {
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (long long)a.B * a.H * a.Nk) return;
+  const int j = row % a.Nk, h = row / a.Nk % a.H, b = row / a.Nk / a.H;
+  float k[kPer], v[kPer], q[kPer], g[kPer], dk[kPer] = {}, dv[kPer] = {};
+  float bias;
+  if (key_bias(a, b, j, &bias)) {
+    load_row<T>(a.k, b * a.ks.b + j * a.ks.n + h * a.ks.h, a.D, k);
+    load_row<T>(a.v, b * a.vs.b + j * a.vs.n + h * a.vs.h, a.D, v);
+    const float c = a.scale * kLog2e;
+    for (int n = 0; n < a.Nq; ++n) {
+      const long long r = ((long long)b * a.H + h) * a.Nq + n;
+      load_row<T>(a.q, b * a.qs.b + n * a.qs.n + h * a.qs.h, a.D, q);
+      load_row<T>(a.dout, b * a.dos.b + n * a.dos.n + h * a.dos.h, a.D, g);
+      const float p = prob(fmaf(dot(q, k), c, bias), a.lse_in[r]);
+      const float ds = p * (dot(g, v) - a.delta[r]) * a.scale;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        dk[i] = fmaf(ds, q[i], dk[i]);
+        dv[i] = fmaf(p, g[i], dv[i]);
+      }
+    }
+  }
+  const long long off = (((long long)b * a.Nk + j) * a.H + h) * a.D;
+  store_row<T>(a.dk, off, a.D, dk);
+  store_row<T>(a.dv, off, a.D, dv);
+}
+
+long long workspace_bytes(int B, int Nq, int Nk, int H, int D, bool grad) {
+  (void)Nk;
+  (void)D;
+  return grad ? (long long)B * H * Nq * 4 : 0;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int check(const char* what, const Args& a, int dtype, const void* ws, long long ws_bytes,
+          bool grad) {
+  auto bad = [&](const char* why) {
+    return record_error(NOVA_ERR_INVALID_ARGUMENT, std::string(what) + ": " + why);
+  };
+  if (a.B < 1 || a.Nq < 1 || a.Nk < 1 || a.H < 1 || a.D < 1) return bad("bad sizes");
+  if (a.D % 8 || a.D > kMaxD) return bad("head_dim must be a multiple of 8, at most 160");
+  if (dtype != kF16 && dtype != kBF16) return bad("element type must be fp16 or bf16");
+  if (a.mask_kind < kMaskNone || a.mask_kind > kMaskBool) return bad("bad mask type");
+  if (!a.q || !a.k || !a.v || (a.mask_kind != kMaskNone && !a.mask)) return bad("null pointer");
+  if (grad ? !a.dout || !a.lse_in || !a.dq || !a.dk || !a.dv : !a.out) return bad("null pointer");
+  auto fine = [](const void* p, const Strides& s) {
+    return aligned16(p) && s.b >= 0 && s.n >= 0 && s.h >= 0 && s.b % 8 == 0 && s.n % 8 == 0 &&
+           s.h % 8 == 0;
+  };
+  if (!fine(a.q, a.qs) || !fine(a.k, a.ks) || !fine(a.v, a.vs) ||
+      (grad && !fine(a.dout, a.dos)))
+    return bad("rows must start on 16 bytes and strides must not be negative");
+  if (grad ? !aligned16(a.dq) || !aligned16(a.dk) || !aligned16(a.dv) : !aligned16(a.out))
+    return bad("outputs must be 16-byte aligned");
+  if (a.mb < 0 || a.mn < 0) return bad("negative mask stride");
+  const long long rows = (long long)a.B * a.H * (a.Nq > a.Nk ? a.Nq : a.Nk);
+  if (rows > (1ll << 31) - 1) return bad("more than 2^31 rows");
+  const long long need = workspace_bytes(a.B, a.Nq, a.Nk, a.H, a.D, grad);
+  if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 256))
+    return bad("workspace missing or not 256-byte aligned");
+  if (ws_bytes < need)
+    return record_error(NOVA_ERR_WORKSPACE,
+                        std::string(what) + ": workspace needs " + std::to_string(need) + " bytes");
+  return NOVA_OK;
+}
+
+int done(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) return NOVA_OK;
+  return record_error(NOVA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+unsigned blocks4(long long rows) { return (unsigned)((rows + 3) / 4); }
+
+}  // namespace xattn
+}  // namespace nova
+
+#define NOVA_EXPORT extern "C" __attribute__((visibility("default")))
+
+NOVA_EXPORT long long nova_cross_attention_workspace_bytes(int batch, int queries, int keys,
+                                                           int heads, int head_dim, int grad) {
+  if (batch < 1 || queries < 1 || keys < 1 || heads < 1 || head_dim < 8 || head_dim % 8 ||
+      head_dim > nova::xattn::kMaxD)
+    return -1;
+  return nova::xattn::workspace_bytes(batch, queries, keys, heads, head_dim, grad != 0);
+}
+
+NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const void* d_v,
+                                        const void* d_mask, void* d_output, void* d_lse,
+                                        void* d_workspace, long long ws_bytes, int batch,
+                                        int queries, int keys, int heads, int head_dim,
+                                        const long long* strides, int dtype, int mask_type,
+                                        float scale, void* stream) try {
+  using namespace nova;
+  using namespace nova::xattn;
+  if (!strides) return record_error(NOVA_ERR_INVALID_ARGUMENT, "cross_attention: null strides");
+  Args a{};
+  a.q = d_q, a.k = d_k, a.v = d_v, a.mask = d_mask, a.out = d_output;
+  a.lse = static_cast<float*>(d_lse);
+  const long long* t = strides;
+  a.qs = {t[0], t[1], t[2]}, a.ks = {t[3], t[4], t[5]}, a.vs = {t[6], t[7], t[8]};
+  a.mb = t[9], a.mn = t[10];
+  a.B = batch, a.Nq = queries, a.Nk = keys, a.H = heads, a.D = head_dim;
+  a.mask_kind = mask_type, a.scale = scale;
+  if (const int rc = check("cross_attention", a, dtype, d_workspace, ws_bytes, false)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = blocks4((long long)batch * heads * queries);
+  if (dtype == kF16) forward_rows<__half><<<grid, 128, 0, s>>>(a);
+  else forward_rows<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
+  return done("cross_attention", cudaGetLastError());
+} catch (...) {
+  return NOVA_ERR_ALLOC;
+}
+
+NOVA_EXPORT int nova_cross_attention_grad_v2(
+    const void* d_q, const void* d_k, const void* d_v, const void* d_mask, const void* d_output,
+    const void* d_grad_output, const void* d_lse, void* d_grad_q, void* d_grad_k, void* d_grad_v,
+    void* d_workspace, long long ws_bytes, int batch, int queries, int keys, int heads,
+    int head_dim, const long long* strides, int dtype, int mask_type, float scale,
+    void* stream) try {
+  using namespace nova;
+  using namespace nova::xattn;
+  if (!strides) return record_error(NOVA_ERR_INVALID_ARGUMENT, "cross_attention_grad: null strides");
+  Args a{};
+  a.q = d_q, a.k = d_k, a.v = d_v, a.mask = d_mask, a.dout = d_grad_output;
+  a.out = const_cast<void*>(d_output);
+  a.lse_in = static_cast<const float*>(d_lse);
+  a.dq = d_grad_q, a.dk = d_grad_k, a.dv = d_grad_v;
+  const long long* t = strides;
+  a.qs = {t[0], t[1], t[2]}, a.ks = {t[3], t[4], t[5]}, a.vs = {t[6], t[7], t[8]};
+  a.mb = t[9], a.mn = t[10];
+  a.dos = {t[11], t[12], t[13]};
+  a.B = batch, a.Nq = queries, a.Nk = keys, a.H = heads, a.D = head_dim;
+  a.mask_kind = mask_type, a.scale = scale;
+  if (const int rc = check("cross_attention_grad", a, dtype, d_workspace, ws_bytes, true))
+    return rc;
+  if (!a.out || !aligned16(a.out))
+    return record_error(NOVA_ERR_INVALID_ARGUMENT, "cross_attention_grad: bad output pointer");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  float* delta = static_cast<float*>(d_workspace);
+  a.delta = delta;
+  const unsigned gq = blocks4((long long)batch * heads * queries);
+  const unsigned gk = blocks4((long long)batch * heads * keys);
+  if (dtype == kF16) {
+    grad_queries<__half><<<gq, 128, 0, s>>>(a, delta);
+    grad_keys<__half><<<gk, 128, 0, s>>>(a);
+  } else {
+    grad_queries<__nv_bfloat16><<<gq, 128, 0, s>>>(a, delta);
+    grad_keys<__nv_bfloat16><<<gk, 128, 0, s>>>(a);
+  }
+  return done("cross_attention_grad", cudaGetLastError());
+} catch (...) {
+  return NOVA_ERR_ALLOC;
+}

@@ -1,0 +1,597 @@
+// Group normalisation with its activation on channels-last activations.
+//
+//   u = x + shift[b][c]                       (shift optional)
+//   m, v = mean and variance of u over the pixels and channels of (b, group)
+//   n = (u - m) / sqrt(v + eps),  z = w n + beta,  y = act(z)
+//
+// and its gradient
+//
+//   dz = dy act'(z),  A = mean(w dz),  D = mean(w dz n)   over (b, group)
+//   dx = (w dz - A - n D) / sqrt(v + eps)
+//   dw = sum dz n,  dbeta = sum dz  (over b and pixels),  dshift = sum dx (over pixels)
+//
+// x is [B][HW][C] with a pixel stride and a batch stride of its own; y and dx
+// are dense.  No reference counterpart: the reference's UNet callers leave the
+// norm to the host framework (benchmarks/bench_sd_unet.py:38-109).
+//
+// Statistics.  Every thread keeps sums relative to the first value it sees, so
+// a mean far from zero costs no digits, and parts are joined as (count, mean,
+// sum of squared deviations), in 64 bits where whole samples meet.  Every sum
+// has a fixed order: results repeat bit for bit.
+#include <string>
+
+#include "../../include/nova_winograd.h"
+#include "nova_unet_ops.h"
+
+namespace nova {
+namespace gn {
+
+using namespace unet;
+
+enum Act : int { kNone = 0, kSilu = 1 };
+
+struct Args {
+  const void* x;
+  const void* dy;
+  const void* w;      // [C] or null
+  const void* beta;   // [C] or null
+  const void* shift;  // [B][C] or null
+  void* y;            // y, or dx in the gradient
+  long long xb, xp;   // batch and pixel stride of x, in elements
+  long long yb, yp;   // of dy (the outputs are dense)
+  int B, HW, C, G, cpg;
+  int wtype, stype;
+  float eps;
+};
+
+// How the grid walks one tensor: a block takes TX vector columns of `chunk`
+// pixels of one sample, TY pixels at a time.
+struct Walk {
+  int cv;      // vector columns of a pixel
+  int ncb;     // column blocks
+  int tx, ty;  // threads
+  int chunk;   // pixels per block
+  int nchunk;
+};
+
+constexpr int kThreads = 256;
+
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+template <int ACT>
+__device__ __forceinline__ float act(float z) {
+  return ACT == kSilu ? __fdividef(z, 1.f + __expf(-z)) : z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_grad(float z) {
+  if (ACT != kSilu) return 1.f;
+  const float s = sigmoid(z);
+  return s * fmaf(z, 1.f - s, 1.f);
+}
+
+// Joins (nb, mb, qb) into (na, ma, qa): counts, means, squared deviations.
+__device__ __forceinline__ void join(float& na, float& ma, float& qa, float nb, float mb,
+                                     float qb) {
+  if (nb == 0.f) return;
+  const float n = na + nb, d = mb - ma, f = nb / n;
+  ma = fmaf(d, f, ma);
+  qa += qb + d * d * na * f;
+  na = n;
+}
+
+struct Place {
+  int b, chunk, p0, p1, tx, ty, col;
+  bool active;
+};
+__device__ __forceinline__ Place place(const Args& a, const Walk& k) {
+  Place q;
+  unsigned id = blockIdx.x;
+  const int cb = id % k.ncb;
+  id /= k.ncb;
+  q.chunk = id % k.nchunk;
+  q.b = id / k.nchunk;
+  q.p0 = q.chunk * k.chunk;
+  q.p1 = min(a.HW, q.p0 + k.chunk);
+  q.tx = threadIdx.x % k.tx;
+  q.ty = threadIdx.x / k.tx;
+  q.col = cb * k.tx + q.tx;
+  q.active = q.ty < k.ty && q.col < k.cv;
+  return q;
+}
+
+// Per-channel mean and squared deviations of x over one chunk of pixels.
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2* part) {
+  __shared__ float2 red[kThreads * V];
+  pdl_wait();
+  const Place q = place(a, k);
+  float s1[V] = {}, s2[V] = {}, pivot[V] = {};
+  int n = 0;
+  if (q.active && q.p0 + q.ty < q.p1) {
+    n = (q.p1 - q.p0 - q.ty + k.ty - 1) / k.ty;
+    const T* p = static_cast<const T*>(a.x) + q.b * a.xb + (q.p0 + q.ty) * a.xp + q.col * V;
+    const long long step = k.ty * a.xp;
+    const Pack<T, V> first = load_pack<T, V>(p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) pivot[e] = to_f32(first.e[e]);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i, p += step) {
+      const Pack<T, V> v = load_pack<T, V>(p);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = to_f32(v.e[e]) - pivot[e];
+        s1[e] += d;
+        s2[e] = fmaf(d, d, s2[e]);
+      }
+    }
+  }
+  if (q.ty < k.ty) {
+    const float inv = n ? 1.f / n : 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float md = s1[e] * inv;
+      red[(q.ty * k.tx + q.tx) * V + e] = make_float2(pivot[e] + md, fmaxf(s2[e] - s1[e] * md, 0.f));
+    }
+  }
+  __syncthreads();
+  const int cols = k.tx * V;
+  const int c0 = (q.col - q.tx) * V;
+  for (int j = threadIdx.x; j < cols; j += kThreads) {
+    if (c0 + j >= a.C) break;
+    float cn = 0.f, cm = 0.f, cq = 0.f;
+    for (int r = 0; r < k.ty; ++r) {
+      const int rows = q.p1 - q.p0 - r;
+      if (rows <= 0) break;
+      const float2 v = red[r * cols + j];
+      join(cn, cm, cq, (float)((rows + k.ty - 1) / k.ty), v.x, v.y);
+    }
+    part[((long long)q.b * k.nchunk + q.chunk) * a.C + c0 + j] = make_float2(cm, cq);
+  }
+}
+
+template <int N>
+__device__ __forceinline__ double block_sum(double v, double* buf) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0;
+#pragma unroll
+  for (int i = 0; i < N / 32; ++i) t += buf[i];
+  return t;
+}
+
+// Mean and 1/sqrt(variance + eps) of every (b, group) from the parts.
+__global__ void __launch_bounds__(128) finish_stats(Args a, Walk k, const float2* part,
+                                                    float* stats) {
+  __shared__ double buf[4];
+  pdl_wait();
+  const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
+  const int items = k.nchunk * a.cpg;
+  const double total = (double)a.HW * a.cpg;
+  auto item = [&](int i, double* n, double* m, double* q) {
+    const int ch = i / a.cpg, c = g * a.cpg + i % a.cpg;
+    const float2 v = part[((long long)b * k.nchunk + ch) * a.C + c];
+    *n = min(k.chunk, a.HW - ch * k.chunk);
+    *m = (double)v.x + (a.shift ? load_param(a.shift, a.stype, (long long)b * a.C + c) : 0.f);
+    *q = v.y;
+  };
+  double n, m, q, s = 0;
+  for (int i = threadIdx.x; i < items; i += 128) {
+    item(i, &n, &m, &q);
+    s += n * m;
+  }
+  const double mean = block_sum<128>(s, buf) / total;
+  s = 0;
+  for (int i = threadIdx.x; i < items; i += 128) {
+    item(i, &n, &m, &q);
+    s += q + n * (m - mean) * (m - mean);
+  }
+  const double var = block_sum<128>(s, buf) / total;
+  if (threadIdx.x == 0) {
+    stats[blockIdx.x] = (float)mean;
+    stats[(long long)a.B * a.G + blockIdx.x] = (float)(1.0 / sqrt(var + (double)a.eps));
+  }
+}
+
+// A thread's channel constants: n = (x - mu) r, z = n w + beta.
+template <int V>
+struct Chan {
+  float mu[V], r[V], w[V], beta[V];
+};
+template <int V>
+__device__ __forceinline__ Chan<V> channels(const Args& a, int b, int c0, const float* stats) {
+  Chan<V> h;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const int c = c0 + e;
+    const long long bg = (long long)b * a.G + c / a.cpg;
+    h.mu[e] = stats[bg] -
+              (a.shift ? load_param(a.shift, a.stype, (long long)b * a.C + c) : 0.f);
+    h.r[e] = stats[(long long)a.B * a.G + bg];
+    h.w[e] = a.w ? load_param(a.w, a.wtype, c) : 1.f;
+    h.beta[e] = a.beta ? load_param(a.beta, a.wtype, c) : 0.f;
+  }
+  return h;
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* stats) {
+  pdl_wait();
+  const Place q = place(a, k);
+  if (!q.active) return;
+  Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+#pragma unroll
+  for (int e = 0; e < V; ++e) h.w[e] *= h.r[e];
+  const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
+  T* y = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
+#pragma unroll 4
+  for (int p = q.p0 + q.ty; p < q.p1; p += k.ty) {
+    const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
+    Pack<T, V> o;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      o.e[e] = from_f32<T>(act<ACT>(fmaf(to_f32(v.e[e]) - h.mu[e], h.w[e], h.beta[e])));
+    store_pack<T, V>(y + (long long)p * a.C, o);
+  }
+}
+
+// Gradient, first pass: per channel of one chunk, sums of dz, dz n and n.
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const float* stats,
+                                                         float* part) {
+  __shared__ float red[3][kThreads * V];
+  pdl_wait();
+  const Place q = place(a, k);
+  float s1[V] = {}, s2[V] = {}, s3[V] = {};
+  if (q.active) {
+    const Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+    const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
+    const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
+#pragma unroll 2
+    for (int p = q.p0 + q.ty; p < q.p1; p += k.ty) {
+      const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
+      const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float n = (to_f32(v.e[e]) - h.mu[e]) * h.r[e];
+        const float dz = to_f32(d.e[e]) * act_grad<ACT>(fmaf(n, h.w[e], h.beta[e]));
+        s1[e] += dz;
+        s2[e] = fmaf(dz, n, s2[e]);
+        s3[e] += n;
+      }
+    }
+  }
+  if (q.ty < k.ty) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const int i = (q.ty * k.tx + q.tx) * V + e;
+      red[0][i] = s1[e];
+      red[1][i] = s2[e];
+      red[2][i] = s3[e];
+    }
+  }
+  __syncthreads();
+  const int cols = k.tx * V;
+  const int c0 = (q.col - q.tx) * V;
+  const long long plane = (long long)a.B * k.nchunk * a.C;
+  for (int j = threadIdx.x; j < cols; j += kThreads) {
+    if (c0 + j >= a.C) break;
+    float t[3] = {};
+    for (int r = 0; r < k.ty; ++r)
+#pragma unroll
+      for (int i = 0; i < 3; ++i) t[i] += red[i][r * cols + j];
+    float* o = part + ((long long)q.b * k.nchunk + q.chunk) * a.C + c0 + j;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) o[i * plane] = t[i];
+  }
+}
+
+// Joins the chunks: sums[b][c] = (sum dz, sum dz n), means[b][g] = (A, D), and
+// the shift's gradient.  A warp per channel, lanes over the chunks.
+__global__ void __launch_bounds__(128) finish_grad(Args a, Walk k, const float* stats,
+                                                   const float* part, float2* sums,
+                                                   float2* means, void* dshift) {
+  __shared__ double buf[4];
+  extern __shared__ float s3[];  // [cpg]
+  pdl_wait();
+  const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long plane = (long long)a.B * k.nchunk * a.C;
+  double wa = 0, wd = 0;
+  for (int j = warp; j < a.cpg; j += 4) {
+    const int c = g * a.cpg + j;
+    double t[3] = {};
+    for (int ch = lane; ch < k.nchunk; ch += 32) {
+      const float* o = part + ((long long)b * k.nchunk + ch) * a.C + c;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) t[i] += o[i * plane];
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      for (int o = 16; o > 0; o >>= 1) t[i] += __shfl_xor_sync(~0u, t[i], o);
+    if (lane == 0) {
+      const float w = a.w ? load_param(a.w, a.wtype, c) : 1.f;
+      sums[(long long)b * a.C + c] = make_float2((float)t[0], (float)t[1]);
+      s3[j] = (float)t[2];
+      wa += w * t[0];
+      wd += w * t[1];
+    }
+  }
+  const double total = (double)a.HW * a.cpg;
+  const double A = block_sum<128>(wa, buf) / total;
+  const double D = block_sum<128>(wd, buf) / total;
+  if (threadIdx.x == 0) means[blockIdx.x] = make_float2((float)A, (float)D);
+  if (dshift) {
+    const double r = stats[(long long)a.B * a.G + blockIdx.x];
+    for (int j = threadIdx.x; j < a.cpg; j += 128) {
+      const int c = g * a.cpg + j;
+      const double w = a.w ? load_param(a.w, a.wtype, c) : 1.f;
+      const double t = sums[(long long)b * a.C + c].x;
+      store_param(dshift, a.stype, (long long)b * a.C + c, (float)(r * (w * t - a.HW * A - D * s3[j])));
+    }
+  }
+}
+
+// dw and dbeta: the samples' sums, in order.
+__global__ void __launch_bounds__(128) param_grad(Args a, const float2* sums, void* dw,
+                                                  void* dbeta) {
+  pdl_wait();
+  const int c = blockIdx.x * 128 + threadIdx.x;
+  if (c >= a.C) return;
+  double s = 0, t = 0;
+  for (int b = 0; b < a.B; ++b) {
+    const float2 v = sums[(long long)b * a.C + c];
+    s += v.x;
+    t += v.y;
+  }
+  if (dw) store_param(dw, a.wtype, c, (float)t);
+  if (dbeta) store_param(dbeta, a.wtype, c, (float)s);
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kThreads) apply_grad(Args a, Walk k, const float* stats,
+                                                       const float2* means) {
+  pdl_wait();
+  const Place q = place(a, k);
+  if (!q.active) return;
+  const Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+  float A[V], D[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float2 m = means[(long long)q.b * a.G + (q.col * V + e) / a.cpg];
+    A[e] = m.x;
+    D[e] = m.y;
+  }
+  const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
+  const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
+  T* dx = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
+#pragma unroll 2
+  for (int p = q.p0 + q.ty; p < q.p1; p += k.ty) {
+    const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
+    const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
+    Pack<T, V> o;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float n = (to_f32(v.e[e]) - h.mu[e]) * h.r[e];
+      const float dz = to_f32(d.e[e]) * act_grad<ACT>(fmaf(n, h.w[e], h.beta[e]));
+      o.e[e] = from_f32<T>(h.r[e] * (fmaf(h.w[e], dz, -A[e]) - n * D[e]));
+    }
+    store_pack<T, V>(dx + (long long)p * a.C, o);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+int device_sms() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return sms;
+}
+
+Walk make_walk(int B, int HW, int C, int V) {
+  Walk k;
+  k.cv = C / V;
+  k.ncb = (k.cv + kThreads - 1) / kThreads;
+  k.tx = (k.cv + k.ncb - 1) / k.ncb;
+  k.ty = kThreads / k.tx;
+  // Eight blocks for every SM, but at least four pixels for every thread.
+  const long long blocks = 8ll * device_sms();
+  long long chunks = blocks / ((long long)B * k.ncb);
+  if (chunks < 1) chunks = 1;
+  const long long most = (HW + 4ll * k.ty - 1) / (4ll * k.ty);
+  if (chunks > most) chunks = most;
+  k.chunk = (int)((HW + chunks - 1) / chunks);
+  k.nchunk = (HW + k.chunk - 1) / k.chunk;
+  return k;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+// Workspace of the larger walk (the vector width depends on the pointers).
+long long workspace_bytes(int B, int HW, int C, int G, bool grad) {
+  long long most = 0;
+  for (int V : {1, 4, 8}) {
+    if (C % V) continue;
+    const Walk k = make_walk(B, HW, C, V);
+    const long long parts = (long long)B * k.nchunk * C;
+    const long long n = grad ? (long long)(align256(parts * 12) + align256((size_t)B * C * 8) +
+                                           align256((size_t)B * G * 8))
+                             : (long long)(align256(parts * 8) + align256((size_t)B * G * 8));
+    if (n > most) most = n;
+  }
+  return most;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, int V>
+cudaError_t forward(const Args& a, int act, float* stats, unsigned char* ws, cudaStream_t s) {
+  const Walk k = make_walk(a.B, a.HW, a.C, V);
+  float2* part = reinterpret_cast<float2*>(ws);
+  const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
+  cudaError_t e = launch_pdl(kPdlInput, partial_stats<T, V>, grid, dim3(kThreads), 0, s, a, k, part);
+  if (e == cudaSuccess)
+    e = launch_pdl(kPdlInput, finish_stats, dim3(a.B * a.G), dim3(128), 0, s, a, k,
+                   (const float2*)part, stats);
+  if (e != cudaSuccess) return e;
+  return act == kSilu ? launch_pdl(kPdlInput, apply<T, V, kSilu>, grid, dim3(kThreads), 0, s, a, k,
+                                   (const float*)stats)
+                      : launch_pdl(kPdlInput, apply<T, V, kNone>, grid, dim3(kThreads), 0, s, a, k,
+                                   (const float*)stats);
+}
+
+template <typename T, int V, int ACT>
+cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, void* dshift,
+                     unsigned char* ws, cudaStream_t s) {
+  const Walk k = make_walk(a.B, a.HW, a.C, V);
+  float* part = reinterpret_cast<float*>(ws);
+  ws += align256((size_t)a.B * k.nchunk * a.C * 12);
+  float2* sums = reinterpret_cast<float2*>(ws);
+  ws += align256((size_t)a.B * a.C * 8);
+  float2* means = reinterpret_cast<float2*>(ws);
+  const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
+  cudaError_t e = launch_pdl(kPdlInput, partial_grad<T, V, ACT>, grid, dim3(kThreads), 0, s, a, k,
+                             stats, part);
+  if (e == cudaSuccess)
+    e = launch_pdl(kPdlInput, finish_grad, dim3(a.B * a.G), dim3(128), a.cpg * sizeof(float), s, a,
+                   k, stats, (const float*)part, sums, means, dshift);
+  if (e == cudaSuccess)
+    e = launch_pdl(kPdlInput, apply_grad<T, V, ACT>, grid, dim3(kThreads), 0, s, a, k, stats,
+                   (const float2*)means);
+  if (e == cudaSuccess && (dw || dbeta))
+    e = launch_pdl(kPdlInput, param_grad, dim3((a.C + 127) / 128), dim3(128), 0, s, a,
+                   (const float2*)sums, dw, dbeta);
+  return e;
+}
+
+int check(const char* what, const Args& a, int dtype, const void* ws, long long ws_bytes,
+          bool grad) {
+  auto bad = [&](const char* why) {
+    return record_error(NOVA_ERR_INVALID_ARGUMENT, std::string(what) + ": " + why);
+  };
+  if (a.B < 1 || a.HW < 1 || a.C < 1 || a.G < 1) return bad("bad sizes");
+  if (a.C % a.G) return bad("channels must divide into the groups");
+  if (a.cpg > 8192) return bad("more than 8192 channels per group");
+  if (!dtype_ok(dtype) || !dtype_ok(a.wtype) || !dtype_ok(a.stype)) return bad("bad element type");
+  if (!a.x || !a.y || !ws || (grad && !a.dy)) return bad("null pointer");
+  if (a.xp < a.C || a.xb < 0 || (grad && (a.yp < a.C || a.yb < 0)))
+    return bad("a pixel stride below the channels, or a negative batch stride");
+  if (!(a.eps >= 0.f)) return bad("eps must not be negative");
+  if (reinterpret_cast<uintptr_t>(ws) % 256) return bad("workspace not 256-byte aligned");
+  if ((long long)a.B * a.HW > (1ll << 31) - 1 - 4096 || (long long)a.B * a.G > (1ll << 31) - 1)
+    return bad("more than 2^31 pixels");
+  const long long need = workspace_bytes(a.B, a.HW, a.C, a.G, grad);
+  if (ws_bytes < need)
+    return record_error(NOVA_ERR_WORKSPACE,
+                        std::string(what) + ": workspace needs " + std::to_string(need) + " bytes");
+  return NOVA_OK;
+}
+
+// 16-byte accesses where every vector of every operand starts on 16 bytes.
+bool wide(const Args& a, int dtype, bool grad) {
+  const int V = 16 / dtype_bytes(dtype);
+  return a.C % V == 0 && a.xp % V == 0 && a.xb % V == 0 && aligned16(a.x) && aligned16(a.y) &&
+         (!grad || (a.yp % V == 0 && a.yb % V == 0 && aligned16(a.dy)));
+}
+
+int done(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) return NOVA_OK;
+  return record_error(NOVA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+}  // namespace gn
+}  // namespace nova
+
+#define NOVA_EXPORT extern "C" __attribute__((visibility("default")))
+
+NOVA_EXPORT long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups,
+                                                      int grad) {
+  if (batch < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups) return -1;
+  return nova::gn::workspace_bytes(batch, pixels, C, groups, grad != 0);
+}
+
+NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, const void* d_bias,
+                                   const void* d_shift, void* d_output, void* d_stats,
+                                   void* d_workspace, long long ws_bytes, int batch, int pixels,
+                                   int C, int groups, long long batch_stride,
+                                   long long pixel_stride, int dtype, int param_dtype,
+                                   int shift_dtype, int activation, float eps, void* stream) try {
+  using namespace nova;
+  using namespace nova::gn;
+  Args a{d_input, nullptr, d_weight, d_bias, d_shift, d_output, batch_stride, pixel_stride, 0, 0,
+         batch, pixels, C, groups, groups > 0 ? C / groups : 0, param_dtype, shift_dtype, eps};
+  if (const int rc = check("group_norm", a, dtype, d_workspace, ws_bytes, false)) return rc;
+  if (activation != kNone && activation != kSilu)
+    return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm: bad activation");
+  unsigned char* ws = static_cast<unsigned char*>(d_workspace);
+  float* stats = static_cast<float*>(d_stats);
+  if (!stats) {
+    stats = reinterpret_cast<float*>(ws);
+    ws += align256((size_t)batch * groups * 8);
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool v = wide(a, dtype, false);
+  cudaError_t e;
+  if (dtype == kF16)
+    e = v ? forward<__half, 8>(a, activation, stats, ws, s)
+          : forward<__half, 1>(a, activation, stats, ws, s);
+  else if (dtype == kBF16)
+    e = v ? forward<__nv_bfloat16, 8>(a, activation, stats, ws, s)
+          : forward<__nv_bfloat16, 1>(a, activation, stats, ws, s);
+  else
+    e = v ? forward<float, 4>(a, activation, stats, ws, s)
+          : forward<float, 1>(a, activation, stats, ws, s);
+  return done("group_norm", e);
+} catch (...) {
+  return NOVA_ERR_ALLOC;
+}
+
+namespace nova {
+namespace gn {
+template <typename T, int V>
+cudaError_t backward_act(const Args& a, int act, const float* stats, void* dw, void* dbeta,
+                         void* dshift, unsigned char* ws, cudaStream_t s) {
+  return act == kSilu ? backward<T, V, kSilu>(a, stats, dw, dbeta, dshift, ws, s)
+                      : backward<T, V, kNone>(a, stats, dw, dbeta, dshift, ws, s);
+}
+}  // namespace gn
+}  // namespace nova
+
+NOVA_EXPORT int nova_group_norm_grad_v2(
+    const void* d_input, const void* d_grad_output, const void* d_weight, const void* d_bias,
+    const void* d_shift, const void* d_stats, void* d_grad_input, void* d_grad_weight,
+    void* d_grad_bias, void* d_grad_shift, void* d_workspace, long long ws_bytes, int batch,
+    int pixels, int C, int groups, long long batch_stride, long long pixel_stride,
+    long long grad_batch_stride, long long grad_pixel_stride, int dtype, int param_dtype,
+    int shift_dtype, int activation, void* stream) try {
+  using namespace nova;
+  using namespace nova::gn;
+  Args a{d_input, d_grad_output, d_weight, d_bias, d_shift, d_grad_input, batch_stride,
+         pixel_stride, grad_batch_stride, grad_pixel_stride, batch, pixels, C, groups,
+         groups > 0 ? C / groups : 0, param_dtype, shift_dtype, 0.f};
+  if (const int rc = check("group_norm_grad", a, dtype, d_workspace, ws_bytes, true)) return rc;
+  if (!d_stats) return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm_grad: null pointer");
+  if (activation != kNone && activation != kSilu)
+    return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm_grad: bad activation");
+  unsigned char* ws = static_cast<unsigned char*>(d_workspace);
+  const float* stats = static_cast<const float*>(d_stats);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool v = wide(a, dtype, true);
+  cudaError_t e;
+#define NOVA_GN_BACKWARD(T, V) \
+  backward_act<T, V>(a, activation, stats, d_grad_weight, d_grad_bias, d_grad_shift, ws, s)
+  if (dtype == kF16)
+    e = v ? NOVA_GN_BACKWARD(__half, 8) : NOVA_GN_BACKWARD(__half, 1);
+  else if (dtype == kBF16)
+    e = v ? NOVA_GN_BACKWARD(__nv_bfloat16, 8) : NOVA_GN_BACKWARD(__nv_bfloat16, 1);
+  else
+    e = v ? NOVA_GN_BACKWARD(float, 4) : NOVA_GN_BACKWARD(float, 1);
+#undef NOVA_GN_BACKWARD
+  return done("group_norm_grad", e);
+} catch (...) {
+  return NOVA_ERR_ALLOC;
+}

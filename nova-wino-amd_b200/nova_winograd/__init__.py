@@ -10,6 +10,9 @@ Drop-in for the Python surface of Jayluci4/nova-wino-amd (``nova_winograd/__init
     model = torchvision.models.resnet50().cuda().half()
     replace_conv2d_with_nova(model)
 
+and, for the layers between a UNet's convolutions, ``nova_group_norm``,
+``NovaGroupNorm`` and ``nova_cross_attention`` (``unet_ops.py``).
+
 The arithmetic runs in ``lib/libnova_winograd.so`` (hand-written sm_100a CUDA:
 transform kernels and a tcgen05/TMEM batched GEMM fed by TMA).
 """
@@ -21,6 +24,8 @@ from nova_winograd.conv2d import (
 )
 from nova_winograd.ops import compute_tiling, nova_forward
 from nova_winograd.surgery import replace_conv2d_with_nova
+# Beyond the reference's surface, which __all__ below lists.
+from nova_winograd.unet_ops import NovaGroupNorm, nova_cross_attention, nova_group_norm  # noqa: F401
 
 __version__ = "0.1.0"
 __all__ = [

@@ -1,0 +1,356 @@
+"""The UNet operators around the 3x3 convolutions, on the GPU kernels of
+``libnova_winograd.so``:
+
+    nova_group_norm        group normalisation with its activation on channels-last
+                           activations, a per-sample channel shift added first
+    nova_cross_attention   attention of one set of tokens to an encoder's states
+    NovaGroupNorm          module form of the norm, drop-in for ``nn.GroupNorm``
+
+No reference counterpart: the reference's UNet callers leave both to the host
+framework (Jayluci4/nova-wino-amd ``benchmarks/bench_sd_unet.py:38-109``).  Both
+are differentiable once, run on the caller's current CUDA stream, allocate through
+torch's caching allocator only and never synchronize, so both can be captured
+into a CUDA graph.  Like the rest of the package they have no CPU fallback.
+"""
+
+import ctypes
+
+import torch
+import torch.nn as nn
+
+from nova_winograd.conv2d import _raw_stream
+from nova_winograd.ops import check, get_lib
+
+DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+MASK_NONE, MASK_BOOL = -1, 3
+ACTIVATIONS = {None: 0, "silu": 1}
+MAX_HEAD_DIM = 160
+
+_workspace_sizes = {}
+
+
+def _workspace(name, device, *sizes):
+    """Workspace of a call: the library says how much, the caching allocator gives it."""
+    key = (name, device.index) + sizes
+    n = _workspace_sizes.get(key)
+    if n is None:
+        n = getattr(get_lib(), name)(*sizes)
+        if n < 0:
+            raise ValueError(f"bad sizes for {name[:-len('_workspace_bytes')]}: {sizes}")
+        if len(_workspace_sizes) > 4096:
+            _workspace_sizes.clear()
+        _workspace_sizes[key] = n
+    if n == 0:
+        return None, 0
+    return torch.empty(n, dtype=torch.uint8, device=device), n
+
+
+def _call(name, device, *args):
+    """One library call on ``device`` and its current stream."""
+    fn = getattr(get_lib(), name)
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _raw_stream(device.index))
+    if status:
+        check(status, name)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------
+# Group norm
+# ---------------------------------------------------------------------------
+
+def _pixel_strides(x):
+    """(batch stride, pixel stride) of x [B, C, H, W] whose channels lie next to
+    each other and whose pixels are evenly spaced (channels-last, or channels of a
+    wider channels-last tensor); None for any other layout."""
+    B, C, H, W = x.shape
+    sb, sc, sh, sw = x.stride()
+    if C > 1 and sc != 1:
+        return None
+    pitch = sw if W > 1 else sh if H > 1 else C
+    if pitch < C or (H > 1 and W > 1 and sh != W * pitch):
+        return None
+    return (sb if B > 1 else 0), pitch
+
+
+def _norm_forward(x, num_groups, weight, bias, eps, act, shift, want_stats):
+    B, C, H, W = x.shape
+    strides = _pixel_strides(x)
+    y = torch.empty((B, C, H, W), dtype=x.dtype, device=x.device,
+                    memory_format=torch.channels_last)
+    stats = torch.empty(2, B, num_groups, device=x.device) if want_stats else None
+    if y.numel():
+        ws, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C, num_groups, 0)
+        param = weight if weight is not None else bias
+        _call("nova_group_norm_v2", x.device, x.data_ptr(), _p(weight), _p(bias), _p(shift),
+              y.data_ptr(), _p(stats), _p(ws), n, B, H * W, C, num_groups, *strides,
+              DTYPES[x.dtype], 2 if param is None else DTYPES[param.dtype],
+              2 if shift is None else DTYPES[shift.dtype], act, eps)
+    return y, stats
+
+
+class _GroupNorm(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, shift, num_groups, eps, act):
+        y, stats = _norm_forward(x, num_groups, weight, bias, eps, act, shift, True)
+        ctx.save_for_backward(x, weight, bias, shift, stats)
+        ctx.num_groups, ctx.act = num_groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, shift, stats = ctx.saved_tensors
+        B, C, H, W = x.shape
+        need = ctx.needs_input_grad
+        dx = torch.empty((B, C, H, W), dtype=x.dtype, device=x.device,
+                         memory_format=torch.channels_last)
+        dw = torch.empty_like(weight) if need[1] else None
+        db = torch.empty_like(bias) if need[2] else None
+        ds = torch.empty_like(shift) if need[3] else None
+        if not dx.numel():
+            for t in (dw, db, ds):
+                if t is not None:
+                    t.zero_()
+            return dx, dw, db, ds, None, None, None
+        strides = _pixel_strides(dy)
+        if strides is None:
+            dy = dy.contiguous(memory_format=torch.channels_last)
+            strides = _pixel_strides(dy)
+        ws, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C,
+                           ctx.num_groups, 1)
+        param = weight if weight is not None else bias
+        _call("nova_group_norm_grad_v2", x.device, x.data_ptr(), dy.data_ptr(), _p(weight),
+              _p(bias), _p(shift), stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db), _p(ds),
+              _p(ws), n, B, H * W, C, ctx.num_groups, *_pixel_strides(x), *strides,
+              DTYPES[x.dtype], 2 if param is None else DTYPES[param.dtype],
+              2 if shift is None else DTYPES[shift.dtype], ctx.act)
+        return (dx if need[0] else None), dw, db, ds, None, None, None
+
+
+def _check_param(name, t, shape, x):
+    if t.device != x.device:
+        raise ValueError(f"{name} must be on the input's device")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None, shift=None):
+    """``act(group_norm(x + shift[:, :, None, None]))`` on channels-last activations.
+
+    Args:
+        x:          [B, C, H, W] float16, bfloat16 or float32 CUDA tensor in
+                    channels-last layout, or a channel slice of one (channels next to
+                    each other, pixels evenly spaced).
+        num_groups: number of groups; divides C.
+        weight, bias: [C] float16, bfloat16 or float32, both of one type, or None.
+        eps:        added to the variance.
+        activation: None or "silu".
+        shift:      [B, C] float16, bfloat16 or float32 added to x before the norm (a
+                    residual block's time embedding), or None.
+
+    Returns a channels-last tensor of x's type.  Statistics and arithmetic are in 32
+    bits (the joining of partial sums in 64), with one rounding at the end; results
+    repeat bit for bit.  Gradients for x, weight, bias and shift.
+    """
+    if x.dim() != 4:
+        raise ValueError(f"x must be [B, C, H, W], got {list(x.shape)}")
+    if x.dtype not in DTYPES:
+        raise TypeError(f"x must be float16, bfloat16 or float32, got {x.dtype}")
+    B, C = x.shape[:2]
+    if num_groups < 1 or C < 1 or C % num_groups:
+        raise ValueError(f"{C} channels do not divide into {num_groups} groups")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be None or 'silu', got {activation!r}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if _pixel_strides(x) is None:
+        raise ValueError("x must be channels-last (torch.channels_last, or channels of one)")
+    if weight is not None:
+        weight = _check_param("weight", weight, (C,), x)
+    if bias is not None:
+        bias = _check_param("bias", bias, (C,), x)
+        if weight is not None and bias.dtype != weight.dtype:
+            raise TypeError("weight and bias must have one type")
+    if shift is not None:
+        shift = _check_param("shift", shift, (B, C), x)
+    if not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor")
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, weight, bias, shift)):
+        return _GroupNorm.apply(x, weight, bias, shift, num_groups, eps, act)
+    return _norm_forward(x, num_groups, weight, bias, eps, act, shift, False)[0]
+
+
+class NovaGroupNorm(nn.GroupNorm):
+    """``nn.GroupNorm`` with its activation fused in, on ``nova_group_norm``.
+
+    Channels-last input gives channels-last output.  Contiguous NCHW input goes
+    through an on-device copy to channels-last and back.
+    """
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None,
+                 device=None, dtype=None):
+        super().__init__(num_groups, num_channels, eps=eps, affine=affine, device=device,
+                         dtype=dtype)
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"activation must be None or 'silu', got {activation!r}")
+        self.activation = activation
+
+    def forward(self, x, shift=None):
+        back = x.dim() == 4 and _pixel_strides(x) is None
+        if back:
+            x = x.contiguous(memory_format=torch.channels_last)
+        y = nova_group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation,
+                            shift)
+        return y.contiguous() if back else y
+
+    @classmethod
+    def from_group_norm(cls, norm, activation=None):
+        """The same norm (its parameters are shared, not copied)."""
+        new = cls(norm.num_groups, norm.num_channels, eps=norm.eps, affine=False,
+                  activation=activation)
+        new.affine, new.weight, new.bias = norm.affine, norm.weight, norm.bias
+        return new.train(norm.training)
+
+    def extra_repr(self):
+        return f"{super().extra_repr()}, activation={self.activation}"
+
+
+# ---------------------------------------------------------------------------
+# Cross attention
+# ---------------------------------------------------------------------------
+
+def _rows(t):
+    """t [B, N, H, D] with its rows' elements next to each other and every row on 16
+    bytes: t itself where it lies so, else a contiguous copy."""
+    sb, sn, sh, sd = t.stride()
+    if (sd == 1 and sb % 8 == 0 and sn % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0):
+        return t
+    return t.contiguous()
+
+
+def _strides(q, k, v, mask, *more):
+    vals = [*q.stride()[:3], *k.stride()[:3], *v.stride()[:3]]
+    vals += list(mask.stride()) if mask is not None else [0, 0]
+    for t in more:
+        vals += t.stride()[:3]
+    return (ctypes.c_longlong * len(vals))(*vals)
+
+
+def _mask_type(mask):
+    if mask is None:
+        return MASK_NONE
+    return MASK_BOOL if mask.dtype == torch.bool else DTYPES[mask.dtype]
+
+
+def _cross_forward(q, k, v, mask, scale, want_lse):
+    B, Nq, H, D = q.shape
+    Nk = k.shape[1]
+    out = torch.empty((B, Nq, H, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device) if want_lse else None
+    if out.numel() and Nk:
+        ws, n = _workspace("nova_cross_attention_workspace_bytes", q.device, B, Nq, Nk, H, D, 0)
+        _call("nova_cross_attention_v2", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              _p(mask), out.data_ptr(), _p(lse), _p(ws), n, B, Nq, Nk, H, D,
+              _strides(q, k, v, mask), DTYPES[q.dtype], _mask_type(mask), scale)
+    else:
+        out.zero_()
+    return out, lse
+
+
+class _CrossAttention(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, q, k, v, mask, scale):
+        out, lse = _cross_forward(q, k, v, mask, scale, True)
+        ctx.save_for_backward(q, k, v, mask, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, mask, out, lse = ctx.saved_tensors
+        B, Nq, H, D = q.shape
+        Nk = k.shape[1]
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+        if dq.numel() and Nk:
+            do = _rows(do)
+            ws, n = _workspace("nova_cross_attention_workspace_bytes", q.device, B, Nq, Nk, H, D, 1)
+            _call("nova_cross_attention_grad_v2", q.device, q.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), _p(mask), out.data_ptr(), do.data_ptr(), lse.data_ptr(),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(ws), n, B, Nq, Nk, H, D,
+                  _strides(q, k, v, mask, do), DTYPES[q.dtype], _mask_type(mask), ctx.scale)
+        else:
+            for t in (dq, dk, dv):
+                t.zero_()
+        need = ctx.needs_input_grad
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
+                None)
+
+
+def nova_cross_attention(q, k, v, key_mask=None, scale=None):
+    """``softmax(scale * q k^T + key_mask) v`` for every sample and head.
+
+    Args:
+        q:        [B, Nq, H, D] float16 or bfloat16 CUDA tensor, D a multiple of 8 up
+                  to 160.
+        k, v:     [B, Nk, H, D], of q's type.  Any strides; a tensor whose rows are
+                  not contiguous on 16 bytes is copied first.
+        key_mask: None, a bool [B, Nk] tensor (True: the key takes part), or a float
+                  [B, Nk] tensor added to the scores (float16, bfloat16 or float32; minus
+                  infinity: the key takes no part).  Not differentiable.
+        scale:    default 1 / sqrt(D).
+
+    A key that takes no part is never multiplied, whatever k and v hold there.  A
+    query without keys gets zeros and passes no gradient on.  Returns [B, Nq, H, D],
+    contiguous.  Products are accumulated and the softmax is computed in 32 bits.
+    Gradients for q, k and v repeat bit for bit.
+    """
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [B, N, H, D], got {list(t.shape)}")
+        if t.dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+        if t.device != q.device:
+            raise ValueError("q, k and v must be on one device")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must have one type")
+    B, Nq, H, D = q.shape
+    Nk = k.shape[1]
+    if k.shape != (B, Nk, H, D) or v.shape != (B, Nk, H, D):
+        raise ValueError(f"k and v must both be [{B}, Nk, {H}, {D}], got {list(k.shape)} and "
+                         f"{list(v.shape)}")
+    if D % 8 or not 8 <= D <= MAX_HEAD_DIM:
+        raise ValueError(f"head width must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
+    if key_mask is not None:
+        if key_mask.dtype != torch.bool and key_mask.dtype not in DTYPES:
+            raise TypeError(f"key_mask must be bool, float16, bfloat16 or float32, got "
+                            f"{key_mask.dtype}")
+        if key_mask.shape != (B, Nk):
+            raise ValueError(f"key_mask must be [{B}, {Nk}], got {list(key_mask.shape)}")
+        if key_mask.device != q.device:
+            raise ValueError("key_mask must be on q's device")
+        if key_mask.requires_grad:
+            raise ValueError("key_mask is not differentiable")
+    if not q.is_cuda:
+        raise ValueError("q, k and v must be CUDA tensors")
+    scale = D ** -0.5 if scale is None else float(scale)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _CrossAttention.apply(q, k, v, key_mask, scale)
+    return _cross_forward(q, k, v, key_mask, scale, False)[0]
