@@ -1,0 +1,176 @@
+// Shared by the cross-attention kernels: arguments, the masks' meaning, and the
+// tensor-core pieces that the convolution's GEMM does not need (4-D tiles,
+// operands with the other index contiguous, operands in tensor memory).
+#pragma once
+
+#include "nova_tc_ptx.cuh"
+#include "nova_unet_ops.h"
+
+namespace nova {
+namespace xattn {
+
+using namespace unet;
+
+constexpr int kMaskNone = -1, kMaskBool = 3;  // else the element type of an additive mask
+constexpr int kMaxD = 160;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Strides {
+  long long b, n, h;  // elements
+};
+
+struct Args {
+  const void *q, *k, *v, *dout, *mask;
+  const float* lse_in;
+  void* out;   // o
+  float* lse;  // [B][H][Nq], base 2; minus infinity for a query without keys
+  void *dq, *dk, *dv;
+  const float* delta;  // [B][H][Nq]: sum(p dp)
+  Strides qs, ks, vs, dos;
+  long long mb, mn;  // mask strides
+  int B, Nq, Nk, H, D;
+  int mask_kind;
+  float scale;
+};
+
+// Bias of key n in base 2, and whether the key takes part.  The lowest finite
+// bias stays finite after the change of base, so that a row with nothing else
+// is the uniform row that the definition gives.
+__device__ __forceinline__ bool key_bias(const Args& a, int b, int n, float* bias) {
+  *bias = 0.f;
+  if (a.mask_kind == kMaskNone) return true;
+  const long long i = b * a.mb + n * a.mn;
+  if (a.mask_kind == kMaskBool) return static_cast<const unsigned char*>(a.mask)[i] != 0;
+  const float m = load_param(a.mask, a.mask_kind, i);
+  if (m == -INFINITY) return false;
+  const float t = m * kLog2e;
+  *bias = t == -INFINITY ? -3.402823466e38f : t;
+  return true;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// A tensor [batch][tokens][heads][D] as TMA sees it: (D, tokens, heads, batch),
+// tiles of 64 elements x `rows` tokens, 128-byte rows swizzled.  Elements past D
+// and tokens past the end read as zero and are not written.  A dimension that all
+// its indices share (stride 0) has size 1 there, and its coordinate is 0.
+struct Tile4 {
+  CUtensorMap map;
+};
+struct Pick {  // factors of the head and batch coordinates: 1, or 0 for a shared dimension
+  int h, b;
+};
+bool encode_tile4(CUtensorMap* map, Pick* pick, const void* p, const Strides& s, int B, int N,
+                  int H, int D, int rows, bool bf16);
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                            int c2, int c3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                             int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
+      : "memory");
+}
+
+// Descriptor of a swizzled 128-byte-row tile read with its contiguous index as
+// the operand's M or N (the rows are the contraction): 64-element column blocks
+// `block_bytes` apart, 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t block_bytes) {
+  return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(block_bytes >> 4) << 16) | (64ull << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// Instruction descriptor: FP32 accumulator, both operands of one 16-bit type;
+// a_mn / b_mn: the operand's contiguous index is its M / N.
+__device__ __forceinline__ uint32_t instr_desc(bool bf16, int M, int N, bool a_mn, bool b_mn) {
+  const uint32_t t = bf16 ? 1u : 0u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// D += A B with A in tensor memory: lane = row, a column holds two elements.
+__device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16_issue(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
+}
+
+// Byte offset of 16-byte piece `piece` of row `row` in a swizzled tile.
+__device__ __forceinline__ uint32_t sw128(int row, int piece) {
+  return (uint32_t)row * 128u + (uint32_t)((piece ^ (row & 7)) << 4);
+}
+
+int device_sms();
+
+// Forward (nova_attention_fwd.cu): workspace and launch.
+long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D);
+cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why);
+
+}  // namespace xattn
+}  // namespace nova

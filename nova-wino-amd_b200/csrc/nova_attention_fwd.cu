@@ -1,0 +1,579 @@
+// Cross-attention forward on the tensor cores.
+//
+// A block of 128 threads takes 128 queries of one head at a time and owns every
+// step of them: thread 0 starts the copies (TMA) and the products (tcgen05), all
+// threads do the softmax, one query (one tensor-memory lane) each.
+//
+//   S = Q K^T      both operands as TMA lands them (rows of 64 elements, swizzled)
+//   P = 2^(c S + bias - m)   read from and written back to tensor memory, in place
+//   O += P V       P from tensor memory; V as it lies, its head index contiguous
+//
+// The keys come in `nkt` tiles of `KT` (a multiple of 16, at most 128).  With one
+// tile (77 text tokens) K and V stay in shared memory while the block walks over
+// its share of the head's queries, and the next queries land while these are
+// worked on; with more, K and V run through two stages and O keeps its place, its
+// scale renewed only when a row's maximum has risen by more than 2^kLazy.  Few
+// queries against many keys: the keys are split over blocks, which leave partial
+// rows in the workspace for a second kernel to join.
+//
+// P is held 2^kLift times larger than the definition's, so that FP16's normal
+// range reaches 2^-24 below the row's largest; the factor cancels in O / sum.
+#include <cuda_runtime.h>
+
+#include "nova_attention.cuh"
+
+namespace nova {
+namespace xattn {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kRows = 128;
+constexpr float kLift = 10.f;
+constexpr float kLazy = 4.f;
+
+struct FwdParams {
+  Args a;
+  Pick qp, kp, vp, op;
+  int KT, nkt;       // keys per tile, tiles
+  int DB, DP;        // 64-element blocks and padded width of a head
+  int qtiles, chunk; // query tiles of a head, tiles per block
+  int nchunk;
+  int splits, per;   // key splits, tiles per split
+  int qstages, kstages;
+  uint32_t tmem_cols, o_col;
+  uint32_t q_bytes, k_bytes;  // one stage of Q, of K (= of V)
+  float* part_o;    // [splits][B][Nq][H][D]
+  float* part_lse;  // [splits][B][H][Nq]
+};
+
+__device__ int g_status;
+
+template <typename T, bool MASK>
+__global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUtensorMap mq,
+                                                    const __grid_constant__ CUtensorMap mk,
+                                                    const __grid_constant__ CUtensorMap mv,
+                                                    const __grid_constant__ CUtensorMap mo,
+                                                    const __grid_constant__ FwdParams p) {
+  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t bars[6];  // q[2], kv[2], s, o
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ float bias[kRows];
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t sq = base, sk = base + p.qstages * p.q_bytes, sv = sk + p.kstages * p.k_bytes;
+  const uint32_t bq = smem_u32(&bars[0]), bkv = smem_u32(&bars[2]), bs = smem_u32(&bars[4]),
+                 bo = smem_u32(&bars[5]);
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(p.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 32) {
+    for (int i = 0; i < 6; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    abort_flag = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  pdl_wait();
+
+  unsigned id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int ch = id % p.nchunk;
+  id /= p.nchunk;
+  const int h = id % p.a.H, b = id / p.a.H;
+  const int t0 = ch * p.chunk, t1 = min(p.qtiles, t0 + p.chunk);
+  const int k0 = split * p.per, k1 = min(p.nkt, k0 + p.per);
+  const int nk = k1 - k0;
+
+  auto load_q = [&](int t, int stage) {
+    const uint32_t bar = bq + 8u * stage, dst = sq + stage * p.q_bytes;
+    mbar_expect_tx(bar, p.q_bytes);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(dst + d * (kRows * 128), &mq, d * 64, t * kRows, h * p.qp.h, b * p.qp.b, bar);
+  };
+  auto load_kv = [&](int kt, int stage) {
+    const uint32_t bar = bkv + 8u * stage;
+    mbar_expect_tx(bar, 2 * p.k_bytes);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(sk + stage * p.k_bytes + d * (p.KT * 128), &mk, d * 64, kt * p.KT, h * p.kp.h,
+                  b * p.kp.b, bar);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(sv + stage * p.k_bytes + d * (p.KT * 128), &mv, d * 64, kt * p.KT, h * p.vp.h,
+                  b * p.vp.b, bar);
+  };
+  const bool resident = nk == 1;  // K and V stay
+  const int kv_total = resident ? 1 : nk * (t1 - t0);
+  int q_loaded = 0, kv_loaded = 0;  // thread 0's count of started copies
+  if (tid == 0) {
+    load_kv(k0, 0);
+    kv_loaded = 1;
+    load_q(t0, 0);
+    q_loaded = 1;
+    if (kv_total > 1 && p.kstages > 1) {
+      load_kv(k0 + 1 % nk, 1);
+      kv_loaded = 2;
+    }
+  }
+
+  const float c = p.a.scale * kLog2e;
+  const uint32_t idesc_s = instr_desc(kBf16, kRows, p.KT, false, false);
+  const uint32_t idesc_o = instr_desc(kBf16, kRows, p.DP, false, true);
+  const int chunks = p.KT / 16;
+  uint32_t steps = 0;  // products finished: the parity of bs and bo
+  bool ok = true;
+  int kv_seen = -1;    // stage contents that this thread has waited for
+
+  for (int t = t0; t < t1 && ok; ++t) {
+    const int qi = t - t0, qstage = qi % p.qstages;
+    const uint32_t q_at = sq + qstage * p.q_bytes;
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < nk && ok; ++j, ++steps) {
+      const int kt = k0 + j;
+      const int ki = resident ? 0 : qi * nk + j, kstage = ki % p.kstages;
+      const int keys = min(p.KT, p.a.Nk - kt * p.KT);
+      const uint32_t k_at = sk + kstage * p.k_bytes, v_at = sv + kstage * p.k_bytes;
+      if (MASK && kv_seen != ki) {
+        // The bias of this tile's keys; the rows of V behind a masked key are cleared:
+        // P is zero there, and zero times infinity is not.
+        if (tid < p.KT) {
+          float x = -INFINITY;
+          const bool in = tid < keys && key_bias(p.a, b, kt * p.KT + tid, &x);
+          bias[tid] = in ? x : -INFINITY;
+          ok = mbar_wait(bkv + 8u * kstage, (ki / p.kstages) & 1, &abort_flag, &g_status,
+                         kDevTimeoutProducer);
+          if (ok && !in && tid < keys) {
+            for (int d = 0; d < p.DB; ++d)
+              for (int i = 0; i < 8; ++i)
+                st_shared_v4(v_at + d * (p.KT * 128) + sw128(tid, i), 0, 0, 0, 0);
+            fence_async_smem();
+          }
+        }
+        kv_seen = ki;
+        if (!__syncthreads_and(ok)) {
+          ok = false;
+          break;
+        }
+      }
+      if (tid == 0) {
+        ok = mbar_wait(bq + 8u * qstage, (qi / p.qstages) & 1, &abort_flag, &g_status,
+                       kDevTimeoutProducer) &&
+             mbar_wait(bkv + 8u * kstage, (ki / p.kstages) & 1, &abort_flag, &g_status,
+                       kDevTimeoutProducer);
+        if (ok) {
+          tc_fence_after();
+          const uint64_t ad = smem_desc_sw128(q_at), bd = smem_desc_sw128(k_at);
+          for (int s = 0; s < p.DP / 16; ++s)
+            umma_f16(tmem, ad + (uint32_t)((s >> 2) * (kRows * 8) + (s & 3) * 2),
+                     bd + (uint32_t)((s >> 2) * (p.KT * 8) + (s & 3) * 2), idesc_s, s != 0);
+          umma_commit(bs);
+          if (j == 0 && t + 1 < t1 && p.qstages > 1) {
+            // The stage's last rows have left for global memory before it is filled.
+            bulk_wait_read_all();
+            load_q(t + 1, (qi + 1) % p.qstages);
+            ++q_loaded;
+          }
+        }
+      }
+      ok = ok && mbar_wait(bs, steps & 1, &abort_flag, &g_status, kDevTimeoutMma);
+      if (!__syncthreads_and(ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+
+      // The row's maximum.
+      uint32_t r[2][16];
+      float top = -INFINITY;
+      tmem_ld16_issue(lanes, r[0]);
+#pragma unroll 1
+      for (int i = 0; i < chunks; i += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (i + u < chunks) {
+            tmem_wait_ld();
+            if (i + u + 1 < chunks) tmem_ld16_issue(lanes + 16u * (i + u + 1), r[u ^ 1]);
+            const int col = 16 * (i + u);
+            if (MASK) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float add = bias[col + e];
+                const float x = fmaf(__uint_as_float(r[u][e]), c, add);
+                top = fmaxf(top, add == -INFINITY ? -INFINITY : x);
+              }
+            } else if (col + 16 <= keys) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e) top = fmaxf(top, __uint_as_float(r[u][e]) * c);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (col + e < keys) top = fmaxf(top, __uint_as_float(r[u][e]) * c);
+            }
+          }
+        }
+      }
+      // The scale that the row's sums are kept at.
+      float factor = 1.f;
+      if (j == 0) {
+        m = top;
+      } else if (top > m + kLazy || m == -INFINITY) {
+        const float up = fmaxf(top, m);
+        factor = m == -INFINITY ? 1.f : ex2(m - up);  // nothing yet: zeros stay zeros
+        m = up;
+      }
+      if (j > 0 && __any_sync(~0u, factor != 1.f)) {
+        l *= factor;
+        for (int i = 0; i < p.DP / 16; ++i) {
+          uint32_t o[16];
+          tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+          tmem_st16(lanes + p.o_col + 16u * i, o);
+        }
+      }
+      const float sub = (m == -INFINITY ? 0.f : m) - kLift;
+
+      // P, packed over the scores that have been read.
+      tmem_ld16_issue(lanes, r[0]);
+#pragma unroll 1
+      for (int i = 0; i < chunks; i += 2) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (i + u < chunks) {
+            tmem_wait_ld();
+            if (i + u + 1 < chunks) tmem_ld16_issue(lanes + 16u * (i + u + 1), r[u ^ 1]);
+            const int col = 16 * (i + u);
+            uint32_t o[8];
+            float e0[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float s = __uint_as_float(r[u][e]);
+              if (MASK) {
+                const float add = bias[col + e];
+                e0[e] = add == -INFINITY ? 0.f : ex2(fmaf(s, c, add) - sub);
+              } else {
+                e0[e] = ex2(fmaf(s, c, -sub));
+              }
+            }
+            if (!MASK && col + 16 > keys) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (col + e >= keys) e0[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              l += e0[2 * e] + e0[2 * e + 1];
+              o[e] = pack2<T>(e0[2 * e], e0[2 * e + 1]);
+            }
+            tmem_st8(lanes + 8u * (i + u), o);
+          }
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncthreads();
+      if (tid == 0) {
+        tc_fence_after();
+        const uint64_t bd = smem_desc_mn(v_at, p.KT * 128);
+        for (int s = 0; s < chunks; ++s)
+          umma_f16_ta(tmem + p.o_col, tmem + 8u * s, bd + 128ull * s, idesc_o, s != 0 || j != 0);
+        umma_commit(bo);
+      }
+      ok = mbar_wait(bo, steps & 1, &abort_flag, &g_status, kDevTimeoutEpilogue);
+      if (tid == 0 && ok && !resident && kv_loaded < kv_total) {
+        load_kv(k0 + kv_loaded % nk, kv_loaded % p.kstages);
+        ++kv_loaded;
+      }
+      if (!__syncthreads_and(ok)) {
+        ok = false;
+        ++steps;
+        break;
+      }
+      tc_fence_after();
+    }
+    if (!ok) break;
+
+    // O / sum.
+    const int row = t * kRows + tid;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float lse = l == 0.f ? -INFINITY : m - kLift + log2f(l);
+    const long long lrow = ((long long)b * p.a.H + h) * p.a.Nq + row;
+    if (p.splits > 1) {
+      float* po = p.part_o + ((((long long)split * p.a.B + b) * p.a.Nq + row) * p.a.H + h) * p.a.D;
+      for (int i = 0; i < p.DP / 16; ++i) {
+        uint32_t o[16];
+        __syncwarp();
+        tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
+        tmem_wait_ld();
+        if (row < p.a.Nq) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            if (16 * i + e < p.a.D)
+              *reinterpret_cast<float4*>(po + 16 * i + e) =
+                  make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                              __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+        }
+      }
+      if (row < p.a.Nq)
+        p.part_lse[(long long)split * p.a.B * p.a.H * p.a.Nq + lrow] = lse;
+      tc_fence_before();
+      __syncthreads();
+    } else {
+      for (int i = 0; i < p.DP / 16; ++i) {
+        uint32_t o[16];
+        tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
+        tmem_wait_ld();
+        float f[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
+        const uint32_t at = q_at + (uint32_t)(i >> 2) * (kRows * 128);
+        const int piece = (i & 3) * 2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          st_shared_v4(at + sw128(tid, piece + u), pack2<T>(f[8 * u], f[8 * u + 1]),
+                       pack2<T>(f[8 * u + 2], f[8 * u + 3]), pack2<T>(f[8 * u + 4], f[8 * u + 5]),
+                       pack2<T>(f[8 * u + 6], f[8 * u + 7]));
+      }
+      if (p.a.lse && row < p.a.Nq) p.a.lse[lrow] = lse;
+      fence_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      if (tid == 0) {
+        for (int d = 0; d < p.DB; ++d)
+          tma_store_4d(&mo, q_at + d * (kRows * 128), d * 64, t * kRows, h, b);
+        bulk_commit();
+      }
+    }
+    if (tid == 0) {
+      tc_fence_after();
+      if (t + 1 < t1 && p.qstages == 1) {
+        bulk_wait_read_all();
+        load_q(t + 1, 0);
+        ++q_loaded;
+      }
+    }
+  }
+
+  if (tid == 0) {
+    if (!ok) {
+      // Let the copies and products that were started end before their memory goes.
+      const int q = q_loaded - 1, kv = kv_loaded - 1;
+      for (int i = 0; i < p.qstages && q - i >= 0; ++i)
+        mbar_wait_drain(bq + 8u * ((q - i) % p.qstages), ((q - i) / p.qstages) & 1);
+      for (int i = 0; i < p.kstages && kv - i >= 0; ++i)
+        mbar_wait_drain(bkv + 8u * ((kv - i) % p.kstages), ((kv - i) / p.kstages) & 1);
+      const uint64_t since = globaltimer();
+      while (globaltimer() - since < kDrainLimitNs) {
+      }
+    }
+    bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(p.tmem_cols)
+                 : "memory");
+  }
+}
+
+// Joins the splits' rows: a warp for a row.
+template <typename T>
+__global__ void __launch_bounds__(128) join_splits(const __grid_constant__ FwdParams p) {
+  pdl_wait();
+  const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  const int n = row % p.a.Nq, h = row / p.a.Nq % p.a.H;
+  const long long b = row / p.a.Nq / p.a.H;
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * rows + row]);
+  const float sub = top == -INFINITY ? 0.f : top;
+  const long long off = ((b * p.a.Nq + n) * p.a.H + h) * p.a.D, plane = rows * p.a.D;
+  float acc[kMaxD / 32] = {}, sum = 0.f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float w = ex2(p.part_lse[s * rows + row] - sub);
+    sum += w;
+#pragma unroll
+    for (int i = 0; i < kMaxD / 32; ++i)
+      if (lane + 32 * i < p.a.D)
+        acc[i] = fmaf(w, p.part_o[s * plane + off + lane + 32 * i], acc[i]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < kMaxD / 32; ++i)
+    if (lane + 32 * i < p.a.D)
+      static_cast<T*>(p.a.out)[off + lane + 32 * i] = from_f32<T>(acc[i] * inv);
+  if (p.a.lse && lane == 0) p.a.lse[row] = sum == 0.f ? -INFINITY : top + log2f(sum);
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+int up(int v, int to) { return (v + to - 1) / to * to; }
+
+}  // namespace
+
+int device_sms() {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return sms;
+}
+
+bool encode_tile4(CUtensorMap* map, Pick* pick, const void* ptr, const Strides& s, int B, int N,
+                  int H, int D, int rows, bool bf16) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  pick->h = H > 1 && s.h != 0;
+  pick->b = B > 1 && s.b != 0;
+  // A dimension of size 1 is never stepped along: any legal stride does.
+  const cuuint64_t row = (cuuint64_t)D * 2;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)N, pick->h ? (cuuint64_t)H : 1,
+                        pick->b ? (cuuint64_t)B : 1};
+  cuuint64_t strides[3] = {N > 1 ? (cuuint64_t)s.n * 2 : row, pick->h ? (cuuint64_t)s.h * 2 : row,
+                           pick->b ? (cuuint64_t)s.b * 2 : row};
+  cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(ptr), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
+
+constexpr size_t kSmemMax = 227 * 1024 - 1024;  // beside the static part
+
+// The split of one call over blocks, tiles and stages.
+void plan(FwdParams* p, int sms) {
+  const Args& a = p->a;
+  p->DB = (a.D + 63) / 64;
+  // Two stages of K and V beside Q fit shared memory, and S beside O a half of
+  // tensor memory, with 128 keys a tile up to 128-wide heads and with 96 above.
+  const int most = a.Nk > 128 && p->DB > 2 ? 96 : 128;
+  p->nkt = (a.Nk + most - 1) / most;
+  p->KT = up((a.Nk + p->nkt - 1) / p->nkt, 16);
+  p->nkt = (a.Nk + p->KT - 1) / p->KT;
+  p->DP = up(a.D, 16);
+  p->qtiles = (a.Nq + kRows - 1) / kRows;
+  const long long heads = (long long)a.B * a.H;
+  p->splits = 1;
+  if (p->nkt > 1 && heads * p->qtiles < 2 * sms) {
+    long long want = (2ll * sms + heads * p->qtiles - 1) / (heads * p->qtiles);
+    if (want > p->nkt) want = p->nkt;
+    p->per = (int)((p->nkt + want - 1) / want);
+    p->splits = (p->nkt + p->per - 1) / p->per;
+  }
+  if (p->splits == 1) p->per = p->nkt;
+  p->q_bytes = (uint32_t)p->DB * kRows * 128;
+  p->k_bytes = (uint32_t)p->DB * p->KT * 128;
+  const bool one = p->per == 1;
+  // With one tile O takes the columns that P leaves of S.
+  p->o_col = (uint32_t)(one ? up(p->KT / 2, 16) : p->KT);
+  const int cols = p->KT > (int)p->o_col + p->DP ? p->KT : (int)p->o_col + p->DP;
+  p->tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
+  p->kstages = one ? 1 : 2;
+  // Blocks of the GPU at a time decide how many query tiles a block walks over.
+  p->qstages = one ? 2 : 1;
+  const size_t smem = (size_t)p->qstages * p->q_bytes + 2ull * p->kstages * p->k_bytes + 1024;
+  long long per_sm = (long long)(kSmemMax / smem);
+  if (per_sm > 512 / p->tmem_cols) per_sm = 512 / p->tmem_cols;
+  if (per_sm < 1) per_sm = 1;
+  if (per_sm > 8) per_sm = 8;
+  long long nchunk = one ? (per_sm * sms) / (heads * p->splits) : p->qtiles;
+  if (nchunk < 1) nchunk = 1;
+  if (nchunk > p->qtiles) nchunk = p->qtiles;
+  p->chunk = (int)((p->qtiles + nchunk - 1) / nchunk);
+  p->nchunk = (p->qtiles + p->chunk - 1) / p->chunk;
+  if (p->chunk == 1) p->qstages = 1;
+}
+
+size_t smem_bytes(const FwdParams& p) {
+  size_t n = (size_t)p.qstages * p.q_bytes + 2ull * p.kstages * p.k_bytes + 1024;
+  // No more blocks on an SM than its tensor memory holds.
+  const size_t least = kSmemMax / (512 / p.tmem_cols + 1) + 1;
+  return n > least ? n : least;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+template <typename T, bool MASK>
+cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
+  const size_t smem = smem_bytes(p);
+  cudaError_t e = cudaFuncSetAttribute(forward_tc<T, MASK>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = (unsigned)((long long)p.a.B * p.a.H * p.nchunk * p.splits);
+  e = launch_pdl(kPdlInput, forward_tc<T, MASK>, dim3(grid), dim3(kRows), smem, s, m[0], m[1],
+                 m[2], m[3], p);
+  if (e == cudaSuccess && p.splits > 1) {
+    const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
+    e = launch_pdl(kPdlInput, join_splits<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p);
+  }
+  return e;
+}
+
+}  // namespace
+
+long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
+  FwdParams p{};
+  p.a.B = B, p.a.Nq = Nq, p.a.Nk = Nk, p.a.H = H, p.a.D = D;
+  plan(&p, device_sms());
+  if (p.splits == 1) return 0;
+  const size_t rows = (size_t)B * H * Nq * p.splits;
+  return (long long)(align256(rows * D * 4) + align256(rows * 4));
+}
+
+cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why) {
+  FwdParams p{};
+  p.a = a;
+  plan(&p, device_sms());
+  const size_t rows = (size_t)a.B * a.H * a.Nq * p.splits;
+  p.part_o = static_cast<float*>(ws);
+  p.part_lse = p.splits > 1 ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) +
+                                                       align256(rows * a.D * 4))
+                            : nullptr;
+  CUtensorMap m[4];
+  const Strides dense{(long long)a.Nq * a.H * a.D, (long long)a.H * a.D, a.D};
+  if (!encode_tile4(&m[0], &p.qp, a.q, a.qs, a.B, a.Nq, a.H, a.D, kRows, bf16) ||
+      !encode_tile4(&m[1], &p.kp, a.k, a.ks, a.B, a.Nk, a.H, a.D, p.KT, bf16) ||
+      !encode_tile4(&m[2], &p.vp, a.v, a.vs, a.B, a.Nk, a.H, a.D, p.KT, bf16) ||
+      !encode_tile4(&m[3], &p.op, a.out, dense, a.B, a.Nq, a.H, a.D, kRows, bf16)) {
+    *why = "tensor map encode failed";
+    return cudaErrorInvalidValue;
+  }
+  const bool mask = a.mask_kind != kMaskNone;
+  if (bf16) return mask ? run<__nv_bfloat16, true>(p, m, s) : run<__nv_bfloat16, false>(p, m, s);
+  return mask ? run<__half, true>(p, m, s) : run<__half, false>(p, m, s);
+}
+
+}  // namespace xattn
+}  // namespace nova

@@ -13,49 +13,10 @@
 #include <string>
 
 #include "../../include/nova_winograd.h"
-#include "nova_unet_ops.h"
+#include "nova_attention.cuh"
 
 namespace nova {
 namespace xattn {
-
-using namespace unet;
-
-constexpr int kMaskNone = -1, kMaskBool = 3;  // else the element type of an additive mask
-constexpr int kMaxD = 160;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct Strides {
-  long long b, n, h;  // elements
-};
-
-struct Args {
-  const void *q, *k, *v, *dout, *mask;
-  const float* lse_in;
-  void* out;   // o
-  float* lse;  // [B][H][Nq], base 2; minus infinity for a query without keys
-  void *dq, *dk, *dv;
-  const float* delta;  // [B][H][Nq]: sum(p dp)
-  Strides qs, ks, vs, dos;
-  long long mb, mn;  // mask strides
-  int B, Nq, Nk, H, D;
-  int mask_kind;
-  float scale;
-};
-
-// Bias of key n in base 2, and whether the key takes part.  The lowest finite
-// bias stays finite after the change of base, so that a row with nothing else
-// is the uniform row that the definition gives.
-__device__ __forceinline__ bool key_bias(const Args& a, int b, int n, float* bias) {
-  *bias = 0.f;
-  if (a.mask_kind == kMaskNone) return true;
-  const long long i = b * a.mb + n * a.mn;
-  if (a.mask_kind == kMaskBool) return static_cast<const unsigned char*>(a.mask)[i] != 0;
-  const float m = load_param(a.mask, a.mask_kind, i);
-  if (m == -INFINITY) return false;
-  const float t = m * kLog2e;
-  *bias = t == -INFINITY ? -3.402823466e38f : t;
-  return true;
-}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -84,36 +45,6 @@ __device__ __forceinline__ float dot(const float (&x)[kPer], const float (&y)[kP
 #pragma unroll
   for (int i = 0; i < kPer; ++i) t = fmaf(x[i], y[i], t);
   return warp_sum(t);
-}
-
-// One warp for a query: one pass over the keys with the running maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(128) forward_rows(Args a) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (long long)a.B * a.H * a.Nq) return;
-  const int n = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H;
-  float q[kPer], k[kPer], v[kPer], o[kPer] = {};
-  load_row<T>(a.q, b * a.qs.b + n * a.qs.n + h * a.qs.h, a.D, q);
-  const float c = a.scale * kLog2e;
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < a.Nk; ++j) {
-    float bias;
-    if (!key_bias(a, b, j, &bias)) continue;
-    load_row<T>(a.k, b * a.ks.b + j * a.ks.n + h * a.ks.h, a.D, k);
-    load_row<T>(a.v, b * a.vs.b + j * a.vs.n + h * a.vs.h, a.D, v);
-    const float s = fmaf(dot(q, k), c, bias);
-    const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top;
-    const float f = exp2f(m - base), e = exp2f(s - base);
-    m = top;
-    l = fmaf(l, f, e);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], f, e * v[i]);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] *= inv;
-  store_row<T>(a.out, (((long long)b * a.Nq + n) * a.H + h) * a.D, a.D, o);
-  if (a.lse && (threadIdx.x & 31) == 0) a.lse[row] = l == 0.f ? -INFINITY : m + log2f(l);
 }
 
 __device__ __forceinline__ float prob(float s, float lse) {
@@ -182,9 +113,7 @@ __global__ void __launch_bounds__(128) grad_keys(Args a) {
 }
 
 long long workspace_bytes(int B, int Nq, int Nk, int H, int D, bool grad) {
-  (void)Nk;
-  (void)D;
-  return grad ? (long long)B * H * Nq * 4 : 0;
+  return grad ? (long long)B * H * Nq * 4 : forward_workspace_bytes(B, Nq, Nk, H, D);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -201,12 +130,12 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
   if (!a.q || !a.k || !a.v || (a.mask_kind != kMaskNone && !a.mask)) return bad("null pointer");
   if (grad ? !a.dout || !a.lse_in || !a.dq || !a.dk || !a.dv : !a.out) return bad("null pointer");
   auto fine = [](const void* p, const Strides& s) {
-    return aligned16(p) && s.b >= 0 && s.n >= 0 && s.h >= 0 && s.b % 8 == 0 && s.n % 8 == 0 &&
+    return aligned16(p) && s.b >= 0 && s.n > 0 && s.h >= 0 && s.b % 8 == 0 && s.n % 8 == 0 &&
            s.h % 8 == 0;
   };
   if (!fine(a.q, a.qs) || !fine(a.k, a.ks) || !fine(a.v, a.vs) ||
       (grad && !fine(a.dout, a.dos)))
-    return bad("rows must start on 16 bytes and strides must not be negative");
+    return bad("rows must start on 16 bytes and no stride may be negative, none of the tokens zero");
   if (grad ? !aligned16(a.dq) || !aligned16(a.dk) || !aligned16(a.dv) : !aligned16(a.out))
     return bad("outputs must be 16-byte aligned");
   if (a.mb < 0 || a.mn < 0) return bad("negative mask stride");
@@ -260,10 +189,10 @@ NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const 
   a.mask_kind = mask_type, a.scale = scale;
   if (const int rc = check("cross_attention", a, dtype, d_workspace, ws_bytes, false)) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = blocks4((long long)batch * heads * queries);
-  if (dtype == kF16) forward_rows<__half><<<grid, 128, 0, s>>>(a);
-  else forward_rows<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
-  return done("cross_attention", cudaGetLastError());
+  const char* why = nullptr;
+  const cudaError_t e = launch_forward(a, dtype == kBF16, d_workspace, s, &why);
+  if (why) return record_error(NOVA_ERR_CUDA, std::string("cross_attention: ") + why);
+  return done("cross_attention", e);
 } catch (...) {
   return NOVA_ERR_ALLOC;
 }

@@ -236,7 +236,8 @@ def _rows(t):
     """t [B, N, H, D] with its rows' elements next to each other and every row on 16
     bytes: t itself where it lies so, else a contiguous copy."""
     sb, sn, sh, sd = t.stride()
-    if (sd == 1 and sb % 8 == 0 and sn % 8 == 0 and sh % 8 == 0 and t.data_ptr() % 16 == 0):
+    if (sd == 1 and sb % 8 == 0 and sn % 8 == 0 and sh % 8 == 0 and sn and
+            t.data_ptr() % 16 == 0):
         return t
     return t.contiguous()
 

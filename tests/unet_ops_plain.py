@@ -112,9 +112,9 @@ def cross_attention(q, k, v, mask=None, scale=1.0, do=None, dtype=None):
         mag = torch.einsum("bqhd,bkhd->bhqk", q.abs(), kk.abs()) * abs(scale)
         mag = (mag + torch.where(kept, bias[:, None, None, :].abs().clamp(max=1e4), 0.0)).amax(-1, keepdim=True)
         p_rel = 4 * F32 * (D + 8) * (mag + 1) + SUM * F32
-        # One rounding of p to the element type for the product; below 2^-26 of the
-        # largest, fp16 has steps of 2^-37 of it.
-        p_off = p * (h + p_rel) + (2.0 ** -36 if dtype == torch.float16 else 0.0) * kept
+        # One rounding of p to the element type for the product.  fp16 holds p at least
+        # 2^10 times larger, so that its last half step, 2^-25, is 2^-35 of p's scale.
+        p_off = p * (h + p_rel) + (2.0 ** -35 if dtype == torch.float16 else 0.0) * kept
         out["o_tol"] = (rounded(dtype, out["o"]) + 1e-12
                         + torch.einsum("bhqk,bkhd->bqhd", p_off + SUM * F32 * p, vv.abs()))
     if do is None:
