@@ -172,5 +172,9 @@ int device_sms();
 long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D);
 cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why);
 
+// Gradient (nova_attention_bwd.cu).
+long long backward_workspace_bytes(int B, int Nq, int Nk, int H, int D);
+cudaError_t launch_backward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why);
+
 }  // namespace xattn
 }  // namespace nova

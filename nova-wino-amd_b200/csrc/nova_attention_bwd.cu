@@ -1,0 +1,673 @@
+// Cross-attention gradient on the tensor cores.
+//
+//   S = Q K^T, dP = dO V^T                         (tensor memory, 32 bits)
+//   P = 2^(c S + bias - lse), dS = P (dP - delta)  (registers; delta = sum_k P dP)
+//   dV += P^T dO, dK += dS^T Q, dQ = dS K
+//
+// A block of 256 threads owns one head's tile of up to 128 keys (kKeys, kBoth) and
+// walks over 128-query tiles with dK and dV in tensor memory, or owns a query tile
+// and walks over the keys with dQ there (kQueries).  A tensor-memory lane is a
+// query; two threads share it, half of the keys each.  Where all keys fit one tile
+// one walk does everything (kBoth): delta is summed from P and dP themselves and O
+// is not read.  More keys take a row-sum pass (delta = dO . O), then kKeys and
+// kQueries, which both form S and dP: seven products instead of five, and no sum
+// whose order could change.
+//
+// P and dS go through shared memory as [query][key] tiles in the swizzle that the
+// products read, with the queries as the contraction (dV, dK: the contiguous index
+// is the operand's M) or the keys (dQ).  S and dP of the next tile are started
+// behind the products of this one, where tensor memory has room for dQ beside them.
+//
+// Rounding.  P and dS are rounded to the element type once, for the products.
+// FP16's range is short for that: P is held 2^kLift times larger, and dS is scaled
+// by a power of two that follows the largest |dP| of the block's walk.
+#include <cuda_runtime.h>
+
+#include "nova_attention.cuh"
+
+namespace nova {
+namespace xattn {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kRows = 128;
+constexpr int kThreads = 256;
+constexpr float kLift = 10.f;
+constexpr int kMaxExp = 60;
+
+enum Mode : int { kBoth = 0, kKeys = 1, kQueries = 2 };
+
+struct BwdParams {
+  Args a;
+  Pick qp, kp, vp, gp;
+  int KT, nkt;        // keys per tile, tiles
+  int DB, DP;         // 64-element blocks and padded width of a head
+  int qtiles;         // query tiles of a head
+  int chunk, splits;  // query tiles per block, blocks per head and key tile
+  int stages;         // of the walked pair
+  int early;          // S and dP of the next tile before dQ of this one is read
+  uint32_t c_dv, c_dk, c_dq;  // tensor-memory columns (S at 0, dP at KT)
+  uint32_t q_bytes, k_bytes;  // one tile of Q or dO, of K or V
+  float *part_dk, *part_dv;   // [splits][B][Nk][H][D]
+};
+
+__device__ int g_status;
+
+template <typename T, bool MASK, int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+    backward_tc(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mg,
+                const __grid_constant__ CUtensorMap mdq, const __grid_constant__ BwdParams p) {
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  constexpr bool kWalkQ = MODE != kQueries;
+  extern __shared__ unsigned char raw[];
+  __shared__ uint64_t bars[5];  // fixed pair, walked pair [2], S and dP, the other products
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ float bias[2][kRows];
+  __shared__ float red[2][kRows];
+  __shared__ uint32_t peak[kThreads / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, half = tid >> 7, r = tid & (kRows - 1);
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  // Fixed pair, walked pairs, P, dS.
+  const uint32_t fixed_bytes = kWalkQ ? p.k_bytes : p.q_bytes;
+  const uint32_t walk_bytes = kWalkQ ? p.q_bytes : p.k_bytes;
+  const uint32_t s_fix = base, s_walk = base + 2 * fixed_bytes;
+  const uint32_t s_p = s_walk + 2 * p.stages * walk_bytes;
+  const uint32_t s_ds = MODE == kQueries ? s_p : s_p + 2 * kRows * 128;
+  const uint32_t bf = smem_u32(&bars[0]), bx = smem_u32(&bars[1]), bs = smem_u32(&bars[3]),
+                 bd = smem_u32(&bars[4]);
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 32) {
+    for (int i = 0; i < 5; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    abort_flag = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  pdl_wait();
+
+  unsigned id = blockIdx.x;
+  int split = 0, kt_fix = 0, t_first, steps;
+  if (kWalkQ) {
+    split = id % p.splits;
+    id /= p.splits;
+    kt_fix = id % p.nkt;
+    id /= p.nkt;
+    t_first = split * p.chunk;
+    steps = min(p.qtiles, t_first + p.chunk) - t_first;
+  } else {
+    t_first = id % p.qtiles;
+    id /= p.qtiles;
+    steps = p.nkt;
+  }
+  const int h = id % p.a.H, b = id / p.a.H;
+  const long long row0 = ((long long)b * p.a.H + h) * p.a.Nq;
+
+  // A pair of tiles: (Q, dO) of query tile t, or (K, V) of key tile t.
+  auto load_q = [&](int t, uint32_t at, uint32_t bar) {
+    mbar_expect_tx(bar, 2 * p.q_bytes);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(at + d * (kRows * 128), &mq, d * 64, t * kRows, h * p.qp.h, b * p.qp.b, bar);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(at + p.q_bytes + d * (kRows * 128), &mg, d * 64, t * kRows, h * p.gp.h,
+                  b * p.gp.b, bar);
+  };
+  auto load_k = [&](int t, uint32_t at, uint32_t bar) {
+    mbar_expect_tx(bar, 2 * p.k_bytes);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(at + d * (p.KT * 128), &mk, d * 64, t * p.KT, h * p.kp.h, b * p.kp.b, bar);
+    for (int d = 0; d < p.DB; ++d)
+      tma_load_4d(at + p.k_bytes + d * (p.KT * 128), &mv, d * 64, t * p.KT, h * p.vp.h, b * p.vp.b,
+                  bar);
+  };
+  auto load_step = [&](int i) {
+    const int st = i % p.stages;
+    const uint32_t at = s_walk + 2 * st * walk_bytes;
+    if (kWalkQ) load_q(t_first + i, at, bx + 8u * st);
+    else load_k(i, at, bx + 8u * st);
+  };
+  const uint32_t idesc_s = instr_desc(kBf16, kRows, p.KT, false, false);
+  const uint32_t idesc_d = instr_desc(kBf16, kRows, p.DP, true, true);
+  const uint32_t idesc_q = instr_desc(kBf16, kRows, p.DP, false, true);
+  const int chunks = p.KT / 16;
+  // S and dP of step i; its tiles have landed when this returns true.
+  auto start_scores = [&](int i) {
+    const int st = i % p.stages;
+    if (!mbar_wait(bx + 8u * st, (i / p.stages) & 1, &abort_flag, &g_status, kDevTimeoutProducer))
+      return false;
+    tc_fence_after();
+    const uint32_t x = s_walk + 2 * st * walk_bytes;
+    const uint32_t q_at = kWalkQ ? x : s_fix, k_at = kWalkQ ? s_fix : x;
+    for (int u = 0; u < 2; ++u) {
+      const uint64_t ad = smem_desc_sw128(q_at + u * p.q_bytes);
+      const uint64_t kd = smem_desc_sw128(k_at + u * p.k_bytes);
+      for (int s = 0; s < p.DP / 16; ++s)
+        umma_f16(tmem + u * p.KT, ad + (uint32_t)((s >> 2) * (kRows * 8) + (s & 3) * 2),
+                 kd + (uint32_t)((s >> 2) * (p.KT * 8) + (s & 3) * 2), idesc_s, s != 0);
+    }
+    umma_commit(bs);
+    return true;
+  };
+
+  int loaded = 0;  // thread 0's count of started walked pairs
+  bool ok = true;
+  if (tid == 0) {
+    if (kWalkQ) load_k(kt_fix, s_fix, bf);
+    else load_q(t_first, s_fix, bf);
+    for (; loaded < p.stages && loaded < steps; ++loaded) load_step(loaded);
+  }
+  // Bias of key tile `t` into bias[slot]; rows of K behind masked keys are cleared
+  // for dQ: dS is zero there, and zero times infinity is not.
+  auto set_bias = [&](int t, int slot) {
+    const int keys = min(p.KT, p.a.Nk - t * p.KT);
+    if (tid < p.KT) {
+      float x = -INFINITY;
+      const bool in = tid < keys && key_bias(p.a, b, t * p.KT + tid, &x);
+      bias[slot][tid] = in ? x : -INFINITY;
+    }
+  };
+  auto clear_masked = [&](uint32_t k_at, int slot) {
+    if (tid < p.KT && bias[slot][tid] == -INFINITY) {
+      for (int d = 0; d < p.DB; ++d)
+        for (int i = 0; i < 8; ++i)
+          st_shared_v4(k_at + d * (p.KT * 128) + sw128(tid, i), 0, 0, 0, 0);
+      fence_async_smem();
+    }
+  };
+  ok = mbar_wait(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
+  if (MASK && kWalkQ) {
+    set_bias(kt_fix, 0);
+    if (MODE == kBoth && ok) clear_masked(s_fix, 0);
+  }
+  if (!__syncthreads_and(ok)) ok = false;
+  if (tid == 0 && ok) ok = start_scores(0);
+
+  const float c = p.a.scale * kLog2e;
+  const int n0 = (chunks + 1) / 2;
+  const int first = half ? n0 : 0, count = half ? chunks - n0 : n0;  // this thread's 16-key chunks
+  int exp_now = 0;
+  bool exp_set = false;
+
+  // The row's lse (no contribution from rows past the end or without keys) and delta.
+  auto row_lse = [&](int t) {
+    const int row = t * kRows + r;
+    if (row >= p.a.Nq) return INFINITY;
+    const float v = p.a.lse_in[row0 + row];
+    return v == -INFINITY ? INFINITY : v;
+  };
+  auto row_delta = [&](int t) {
+    const int row = t * kRows + r;
+    return row < p.a.Nq ? p.a.delta[row0 + row] : 0.f;
+  };
+  float lse = row_lse(t_first);
+  float delta = MODE == kBoth ? 0.f : row_delta(t_first);
+
+  int i = 0;
+  for (; i < steps; ++i) {  // leaves early only where all threads do
+    const int st = i % p.stages, slot = kWalkQ ? 0 : (i & 1);
+    const uint32_t x = s_walk + 2 * st * walk_bytes;
+    const uint32_t q_at = kWalkQ ? x : s_fix, k_at = kWalkQ ? s_fix : x;
+    const int kt = kWalkQ ? kt_fix : i;
+    const int keys = min(p.KT, p.a.Nk - kt * p.KT);
+    if (MASK && !kWalkQ) {
+      set_bias(i, slot);
+      __syncthreads();
+    }
+    float lse_next = 0.f, delta_next = 0.f;
+    if (kWalkQ && i + 1 < steps) {
+      lse_next = row_lse(t_first + i + 1);
+      if (MODE == kKeys) delta_next = row_delta(t_first + i + 1);
+    }
+    ok = mbar_wait(bs, i & 1, &abort_flag, &g_status, kDevTimeoutMma);
+    __syncwarp();
+    tc_fence_after();
+
+    // P (times 2^kLift) and dP of this thread's keys.
+    uint32_t s[4][16], g[4][16];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (u < count) {
+        tmem_ld16_issue(lanes + 16u * (first + u), s[u]);
+        tmem_ld16_issue(lanes + p.KT + 16u * (first + u), g[u]);
+      }
+    tmem_wait_ld();
+    tc_fence_before();
+    float sum = 0.f, top = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (u < count) {
+        const int col = 16 * (first + u);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float dp = __uint_as_float(g[u][e]);
+          // The product is rounded before lse is taken off, as it was when lse was
+          // formed: a single key's probability is then exactly one.
+          float pr;
+          if (MASK) {
+            const float add = bias[slot][col + e];
+            const bool in = add != -INFINITY;
+            pr = in ? ex2(fmaf(__uint_as_float(s[u][e]), c, add) - lse + kLift) : 0.f;
+            if (!in) dp = 0.f;
+          } else {
+            pr = ex2(__fmul_rn(__uint_as_float(s[u][e]), c) - lse + kLift);
+          }
+          s[u][e] = __float_as_uint(pr);
+          g[u][e] = __float_as_uint(dp);
+        }
+        if (!MASK && col + 16 > keys) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (col + e >= keys) s[u][e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          if (MODE == kBoth) sum = fmaf(__uint_as_float(s[u][e]), __uint_as_float(g[u][e]), sum);
+          if (!kBf16) top = fmaxf(top, fabsf(__uint_as_float(g[u][e])));
+        }
+      }
+    if (MODE == kBoth) red[half][r] = sum;
+    if (!kBf16) {
+      // A row that is not finite has no say in the scale of the others.
+      const uint32_t bits = isfinite(top) && isfinite(sum) ? __float_as_uint(top) : 0u;
+      const uint32_t most = __reduce_max_sync(~0u, bits);
+      if ((tid & 31) == 0) peak[warp] = most;
+    }
+    // The rows of dQ staged over P and dS have left before these are written.
+    if (MODE == kBoth && tid == 0) bulk_wait_read_all();
+    if (!__syncthreads_and(ok)) {
+      ok = false;
+      break;
+    }
+    if (MODE == kBoth) delta = (red[0][r] + red[1][r]) * (1.f / 1024.f);
+    float lift = 1.f / 1024.f;  // 2^-kLift, times 2^exp_now
+    if (!kBf16) {
+      uint32_t most = 0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) most = max(most, peak[w]);
+      const int ex = (int)(most >> 23) - 127;  // |dP| < 2^(ex + 1), |dS| < 2^(ex + 2)
+      if (!exp_set || exp_now > 13 - ex) {
+        int to = 9 - ex;
+        to = to > kMaxExp ? kMaxExp : to < -kMaxExp ? -kMaxExp : to;
+        if (exp_set && i > 0 && to != exp_now) {
+          const float f = exp2f((float)(to - exp_now));
+          const uint32_t acc = MODE == kQueries ? p.c_dq : p.c_dk;
+          for (int u = half; u < p.DP / 16; u += 2) {
+            uint32_t o[16];
+            tmem_ld16_issue(lanes + acc + 16u * u, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(lanes + acc + 16u * u, o);
+          }
+          tmem_wait_st();
+        }
+        exp_now = to;
+        exp_set = true;
+      }
+      lift *= exp2f((float)exp_now);
+    }
+    if (MASK && MODE == kQueries) clear_masked(k_at, slot);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (u < count) {
+        const int ck = first + u;
+        const uint32_t at = (uint32_t)(ck >> 2) * (kRows * 128);
+        uint32_t w[8];
+        if (MODE != kQueries) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = pack2<T>(__uint_as_float(s[u][2 * e]), __uint_as_float(s[u][2 * e + 1]));
+          st_shared_v4(s_p + at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
+          st_shared_v4(s_p + at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
+        }
+        float d[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          d[e] = __uint_as_float(s[u][e]) * ((__uint_as_float(g[u][e]) - delta) * lift);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = pack2<T>(d[2 * e], d[2 * e + 1]);
+        st_shared_v4(s_ds + at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
+        st_shared_v4(s_ds + at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
+      }
+    fence_async_smem();
+    tc_fence_before();
+    __syncthreads();
+
+    if (tid == 0) {
+      tc_fence_after();
+      if (MODE != kQueries) {
+        // dV += P^T dO, dK += dS^T Q: the queries are the contraction.
+        const uint64_t pd = smem_desc_mn(s_p, kRows * 128), sd = smem_desc_mn(s_ds, kRows * 128);
+        const uint64_t gd = smem_desc_mn(q_at + p.q_bytes, kRows * 128),
+                       qd = smem_desc_mn(q_at, kRows * 128);
+        for (int u = 0; u < kRows / 16; ++u)
+          umma_f16(tmem + p.c_dv, pd + 128ull * u, gd + 128ull * u, idesc_d, u != 0 || i != 0);
+        for (int u = 0; u < kRows / 16; ++u)
+          umma_f16(tmem + p.c_dk, sd + 128ull * u, qd + 128ull * u, idesc_d, u != 0 || i != 0);
+      }
+      if (MODE != kKeys) {
+        const uint64_t sd = smem_desc_sw128(s_ds), kd = smem_desc_mn(k_at, p.KT * 128);
+        for (int u = 0; u < chunks; ++u)
+          umma_f16(tmem + p.c_dq, sd + (uint32_t)((u >> 2) * (kRows * 8) + (u & 3) * 2),
+                   kd + 128ull * u, idesc_q, u != 0 || (MODE == kQueries && i != 0));
+      }
+      umma_commit(bd);
+      if (p.early && i + 1 < steps) ok = start_scores(i + 1);
+    }
+    ok = ok && mbar_wait(bd, i & 1, &abort_flag, &g_status, kDevTimeoutEpilogue);
+    if (tid == 0 && ok && loaded < steps) {
+      load_step(loaded);
+      ++loaded;
+    }
+    __syncwarp();
+    tc_fence_after();
+    if (MODE == kBoth) {
+      // dQ of the tile, staged over P and dS.
+      const float f = p.a.scale * exp2f((float)-exp_now);
+      for (int u = half; u < p.DP / 16; u += 2) {
+        uint32_t o[16];
+        tmem_ld16_issue(lanes + p.c_dq + 16u * u, o);
+        tmem_wait_ld();
+        float d[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = __uint_as_float(o[e]) * f;
+        const uint32_t at = s_p + (uint32_t)(u >> 2) * (kRows * 128);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          st_shared_v4(at + sw128(r, (u & 3) * 2 + e), pack2<T>(d[8 * e], d[8 * e + 1]),
+                       pack2<T>(d[8 * e + 2], d[8 * e + 3]), pack2<T>(d[8 * e + 4], d[8 * e + 5]),
+                       pack2<T>(d[8 * e + 6], d[8 * e + 7]));
+      }
+      fence_async_smem();
+      tc_fence_before();
+      if (!__syncthreads_and(ok)) {
+        ok = false;
+        ++i;
+        break;
+      }
+      if (tid == 0) {
+        for (int d = 0; d < p.DB; ++d)
+          tma_store_4d(&mdq, s_p + d * (kRows * 128), d * 64, (t_first + i) * kRows, h, b);
+        bulk_commit();
+      }
+    }
+    if (tid == 0 && ok && !p.early && i + 1 < steps) {
+      tc_fence_after();
+      ok = start_scores(i + 1);
+    }
+    if (kWalkQ) {
+      lse = lse_next;
+      if (MODE == kKeys) delta = delta_next;
+    }
+  }
+  ok = __syncthreads_and(ok);
+
+  if (ok) {
+    __syncwarp();
+    tc_fence_after();
+    if (MODE != kQueries) {
+      // dK and dV: a lane is a key.
+      const int keys = min(p.KT, p.a.Nk - kt_fix * p.KT);
+      const bool in = !MASK || (r < p.KT && bias[0][r] != -INFINITY);
+      const float fv = 1.f / 1024.f, fk = p.a.scale * exp2f((float)-exp_now);
+      const long long off =
+          (((long long)b * p.a.Nk + kt_fix * p.KT + r) * p.a.H + h) * (long long)p.a.D;
+      const long long plane = (long long)p.a.B * p.a.Nk * p.a.H * p.a.D;
+      for (int w = 0; w < 2; ++w) {
+        const float f = w ? fk : fv;
+        for (int u = half; u < p.DP / 16; u += 2) {
+          uint32_t o[16];
+          __syncwarp();
+          tmem_ld16_issue(lanes + (w ? p.c_dk : p.c_dv) + 16u * u, o);
+          tmem_wait_ld();
+          float d[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) d[e] = in ? __uint_as_float(o[e]) * f : 0.f;
+          if (r < keys) {
+            if (p.splits > 1) {
+              float* to = (w ? p.part_dk : p.part_dv) + split * plane + off + 16 * u;
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                if (16 * u + e < p.a.D)
+                  *reinterpret_cast<float4*>(to + e) = make_float4(d[e], d[e + 1], d[e + 2], d[e + 3]);
+            } else {
+              T* to = static_cast<T*>(w ? p.a.dk : p.a.dv) + off + 16 * u;
+#pragma unroll
+              for (int e = 0; e < 16; e += 8)
+                if (16 * u + e < p.a.D)
+                  *reinterpret_cast<uint4*>(to + e) =
+                      make_uint4(pack2<T>(d[e], d[e + 1]), pack2<T>(d[e + 2], d[e + 3]),
+                                 pack2<T>(d[e + 4], d[e + 5]), pack2<T>(d[e + 6], d[e + 7]));
+            }
+          }
+        }
+      }
+    } else {
+      const int row = t_first * kRows + r;
+      const float f = p.a.scale * exp2f((float)-exp_now);
+      T* to = static_cast<T*>(p.a.dq) +
+              (((long long)b * p.a.Nq + row) * p.a.H + h) * (long long)p.a.D;
+      for (int u = half; u < p.DP / 16; u += 2) {
+        uint32_t o[16];
+        __syncwarp();
+        tmem_ld16_issue(lanes + p.c_dq + 16u * u, o);
+        tmem_wait_ld();
+        float d[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) d[e] = __uint_as_float(o[e]) * f;
+        if (row < p.a.Nq) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8)
+            if (16 * u + e < p.a.D)
+              *reinterpret_cast<uint4*>(to + 16 * u + e) =
+                  make_uint4(pack2<T>(d[e], d[e + 1]), pack2<T>(d[e + 2], d[e + 3]),
+                             pack2<T>(d[e + 4], d[e + 5]), pack2<T>(d[e + 6], d[e + 7]));
+        }
+      }
+    }
+  } else if (tid == 0) {
+    // Let the copies and products that were started end before their memory goes.
+    mbar_wait_drain(bf, 0);
+    for (int u = 0; u < p.stages && loaded - 1 - u >= 0; ++u)
+      mbar_wait_drain(bx + 8u * ((loaded - 1 - u) % p.stages), ((loaded - 1 - u) / p.stages) & 1);
+    const uint64_t since = globaltimer();
+    while (globaltimer() - since < kDrainLimitNs) {
+    }
+  }
+  if (tid == 0) bulk_wait_all();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512)
+                 : "memory");
+  }
+}
+
+// delta = dO . O: a warp for a query.
+template <typename T>
+__global__ void __launch_bounds__(128) row_delta(const __grid_constant__ Args a, float* delta) {
+  pdl_wait();
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= (long long)a.B * a.H * a.Nq) return;
+  const int lane = threadIdx.x & 31;
+  const int n = row % a.Nq, h = row / a.Nq % a.H;
+  const long long b = row / a.Nq / a.H;
+  const T* o = static_cast<const T*>(a.out) + ((b * a.Nq + n) * a.H + h) * a.D;
+  const T* g = static_cast<const T*>(a.dout) + b * a.dos.b + n * a.dos.n + h * a.dos.h;
+  float t = 0.f;
+  for (int i = lane * 8; i < a.D; i += 256) {
+    const Pack<T, 8> x = load_pack<T, 8>(o + i), y = load_pack<T, 8>(g + i);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t = fmaf(to_f32(x.e[e]), to_f32(y.e[e]), t);
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(~0u, t, s);
+  if (lane == 0) delta[row] = t;
+}
+
+// dK and dV from the query splits' parts, in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_parts(const float* __restrict__ dk,
+                                                  const float* __restrict__ dv, T* to_k, T* to_v,
+                                                  long long n, int splits) {
+  pdl_wait();
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const float* from = blockIdx.y ? dv : dk;
+  float4 t = *reinterpret_cast<const float4*>(from + i);
+  for (int s = 1; s < splits; ++s) {
+    const float4 u = *reinterpret_cast<const float4*>(from + s * n + i);
+    t.x += u.x, t.y += u.y, t.z += u.z, t.w += u.w;
+  }
+  *reinterpret_cast<uint2*>((blockIdx.y ? to_v : to_k) + i) =
+      make_uint2(pack2<T>(t.x, t.y), pack2<T>(t.z, t.w));
+}
+
+int up(int v, int to) { return (v + to - 1) / to * to; }
+size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
+
+constexpr size_t kSmemMax = 226 * 1024;
+
+size_t smem_of(const BwdParams& p, int mode, int stages) {
+  const size_t fix = mode == kQueries ? p.q_bytes : p.k_bytes;
+  const size_t walk = mode == kQueries ? p.k_bytes : p.q_bytes;
+  return 2 * fix + 2 * stages * walk + (mode == kQueries ? 1 : 2) * 2ull * kRows * 128 + 1024;
+}
+
+void plan(BwdParams* p, int sms) {
+  const Args& a = p->a;
+  p->DB = (a.D + 63) / 64;
+  p->DP = up(a.D, 16);
+  // Three-block heads: 80 keys a tile leave shared memory room for P and dS.
+  const int most = p->DB > 2 ? 80 : 128;
+  p->nkt = (a.Nk + most - 1) / most;
+  p->KT = up((a.Nk + p->nkt - 1) / p->nkt, 16);
+  p->nkt = (a.Nk + p->KT - 1) / p->KT;
+  p->qtiles = (a.Nq + kRows - 1) / kRows;
+  p->q_bytes = (uint32_t)p->DB * kRows * 128;
+  p->k_bytes = (uint32_t)p->DB * p->KT * 128;
+  // Query splits: the number of tiles that the busiest SM works through, and about
+  // two tiles' time for every block's start and end.
+  const long long units = (long long)a.B * a.H * p->nkt;
+  long long best = -1;
+  for (int chunk = p->qtiles; chunk >= 1; chunk = chunk > 1 ? (chunk + 1) / 2 : 0) {
+    const int splits = (p->qtiles + chunk - 1) / chunk;
+    const int even = (p->qtiles + splits - 1) / splits;
+    const long long cost = (units * splits + sms - 1) / sms * (even + 2);
+    if (best < 0 || cost < best) {
+      best = cost;
+      p->chunk = even;
+      p->splits = (p->qtiles + even - 1) / even;
+    }
+  }
+}
+
+// Tensor memory and stages of one mode.
+size_t arrange(BwdParams* p, int mode) {
+  const uint32_t two = 2u * p->KT, dp = (uint32_t)p->DP;
+  p->stages = smem_of(*p, mode, 2) <= kSmemMax ? 2 : 1;
+  if (mode == kBoth) {
+    const bool room = two + 3 * dp <= 512;
+    const uint32_t at = room ? two : (two > dp ? two : dp);
+    p->c_dv = at, p->c_dk = at + dp, p->c_dq = room ? at + 2 * dp : 0;
+    p->early = room && p->stages == 2;
+  } else {
+    p->c_dv = two, p->c_dk = two + dp, p->c_dq = two;
+    p->early = p->stages == 2;
+  }
+  return smem_of(*p, mode, p->stages);
+}
+
+template <typename T, bool MASK, int MODE>
+cudaError_t run_mode(BwdParams p, const CUtensorMap* m, cudaStream_t s) {
+  const size_t smem = arrange(&p, MODE);
+  cudaError_t e = cudaFuncSetAttribute(backward_tc<T, MASK, MODE>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const long long heads = (long long)p.a.B * p.a.H;
+  const long long grid = MODE == kQueries ? heads * p.qtiles : heads * p.nkt * p.splits;
+  return launch_pdl(kPdlInput, backward_tc<T, MASK, MODE>, dim3((unsigned)grid), dim3(kThreads),
+                    smem, s, m[0], m[1], m[2], m[3], m[4], p);
+}
+
+template <typename T, bool MASK>
+cudaError_t run(BwdParams p, const CUtensorMap* m, float* delta, cudaStream_t s) {
+  cudaError_t e;
+  if (p.nkt == 1) {
+    e = run_mode<T, MASK, kBoth>(p, m, s);
+  } else {
+    const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
+    e = launch_pdl(kPdlInput, row_delta<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p.a,
+                   delta);
+    p.a.delta = delta;
+    if (e == cudaSuccess) e = run_mode<T, MASK, kKeys>(p, m, s);
+    if (e == cudaSuccess) e = run_mode<T, MASK, kQueries>(p, m, s);
+  }
+  if (e == cudaSuccess && p.splits > 1) {
+    const long long n = (long long)p.a.B * p.a.Nk * p.a.H * p.a.D;
+    e = launch_pdl(kPdlInput, join_parts<T>, dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), 0,
+                   s, (const float*)p.part_dk, (const float*)p.part_dv, static_cast<T*>(p.a.dk),
+                   static_cast<T*>(p.a.dv), n, p.splits);
+  }
+  return e;
+}
+
+}  // namespace
+
+long long backward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
+  BwdParams p{};
+  p.a.B = B, p.a.Nq = Nq, p.a.Nk = Nk, p.a.H = H, p.a.D = D;
+  plan(&p, device_sms());
+  const size_t n = (size_t)B * Nk * H * D * 4;
+  size_t total = p.nkt > 1 ? align256((size_t)B * H * Nq * 4) : 0;
+  if (p.splits > 1) total += 2 * align256(n * p.splits);
+  return (long long)total;
+}
+
+cudaError_t launch_backward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why) {
+  BwdParams p{};
+  p.a = a;
+  plan(&p, device_sms());
+  unsigned char* at = static_cast<unsigned char*>(ws);
+  float* delta = nullptr;
+  if (p.nkt > 1) {
+    delta = reinterpret_cast<float*>(at);
+    at += align256((size_t)a.B * a.H * a.Nq * 4);
+  }
+  if (p.splits > 1) {
+    p.part_dk = reinterpret_cast<float*>(at);
+    p.part_dv = reinterpret_cast<float*>(at + align256((size_t)a.B * a.Nk * a.H * a.D * 4 * p.splits));
+  }
+  CUtensorMap m[5];
+  Pick out;
+  const Strides dense{(long long)a.Nq * a.H * a.D, (long long)a.H * a.D, a.D};
+  if (!encode_tile4(&m[0], &p.qp, a.q, a.qs, a.B, a.Nq, a.H, a.D, kRows, bf16) ||
+      !encode_tile4(&m[1], &p.kp, a.k, a.ks, a.B, a.Nk, a.H, a.D, p.KT, bf16) ||
+      !encode_tile4(&m[2], &p.vp, a.v, a.vs, a.B, a.Nk, a.H, a.D, p.KT, bf16) ||
+      !encode_tile4(&m[3], &p.gp, a.dout, a.dos, a.B, a.Nq, a.H, a.D, kRows, bf16) ||
+      !encode_tile4(&m[4], &out, a.dq, dense, a.B, a.Nq, a.H, a.D, kRows, bf16)) {
+    *why = "tensor map encode failed";
+    return cudaErrorInvalidValue;
+  }
+  const bool mask = a.mask_kind != kMaskNone;
+  if (bf16)
+    return mask ? run<__nv_bfloat16, true>(p, m, delta, s)
+                : run<__nv_bfloat16, false>(p, m, delta, s);
+  return mask ? run<__half, true>(p, m, delta, s) : run<__half, false>(p, m, delta, s);
+}
+
+}  // namespace xattn
+}  // namespace nova

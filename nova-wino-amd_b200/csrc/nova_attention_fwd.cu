@@ -6,6 +6,8 @@
 //
 //   S = Q K^T      both operands as TMA lands them (rows of 64 elements, swizzled)
 //   P = 2^(c S + bias - m)   read from and written back to tensor memory, in place
+//                            (the product is rounded before m is taken off, so that a
+//                            row's largest probability is 2^0 and a single key's is one)
 //   O += P V       P from tensor memory; V as it lies, its head index contiguous
 //
 // The keys come in `nkt` tiles of `KT` (a multiple of 16, at most 128).  With one
@@ -15,9 +17,6 @@
 // scale renewed only when a row's maximum has risen by more than 2^kLazy.  Few
 // queries against many keys: the keys are split over blocks, which leave partial
 // rows in the workspace for a second kernel to join.
-//
-// P is held 2^kLift times larger than the definition's, so that FP16's normal
-// range reaches 2^-24 below the row's largest; the factor cancels in O / sum.
 #include <cuda_runtime.h>
 
 #include "nova_attention.cuh"
@@ -30,7 +29,6 @@ using namespace tc;
 namespace {
 
 constexpr int kRows = 128;
-constexpr float kLift = 10.f;
 constexpr float kLazy = 4.f;
 
 struct FwdParams {
@@ -242,7 +240,7 @@ __global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUte
           tmem_st16(lanes + p.o_col + 16u * i, o);
         }
       }
-      const float sub = (m == -INFINITY ? 0.f : m) - kLift;
+      const float sub = m == -INFINITY ? 0.f : m;
 
       // P, packed over the scores that have been read.
       tmem_ld16_issue(lanes, r[0]);
@@ -263,7 +261,7 @@ __global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUte
                 const float add = bias[col + e];
                 e0[e] = add == -INFINITY ? 0.f : ex2(fmaf(s, c, add) - sub);
               } else {
-                e0[e] = ex2(fmaf(s, c, -sub));
+                e0[e] = ex2(__fmul_rn(s, c) - sub);
               }
             }
             if (!MASK && col + 16 > keys) {
@@ -307,7 +305,7 @@ __global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUte
     // O / sum.
     const int row = t * kRows + tid;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float lse = l == 0.f ? -INFINITY : m - kLift + log2f(l);
+    const float lse = l == 0.f ? -INFINITY : m + log2f(l);
     const long long lrow = ((long long)b * p.a.H + h) * p.a.Nq + row;
     if (p.splits > 1) {
       float* po = p.part_o + ((((long long)split * p.a.B + b) * p.a.Nq + row) * p.a.H + h) * p.a.D;

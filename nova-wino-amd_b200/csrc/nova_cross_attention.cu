@@ -18,102 +18,8 @@
 namespace nova {
 namespace xattn {
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
-}
-
-constexpr int kPer = kMaxD / 32;  // elements of a row that a lane holds
-
-template <typename T>
-__device__ __forceinline__ void load_row(const void* p, long long off, int D, float (&r)[kPer]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    r[i] = lane + 32 * i < D ? to_f32(static_cast<const T*>(p)[off + lane + 32 * i]) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void store_row(void* p, long long off, int D, const float (&r)[kPer]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (lane + 32 * i < D) static_cast<T*>(p)[off + lane + 32 * i] = from_f32<T>(r[i]);
-}
-__device__ __forceinline__ float dot(const float (&x)[kPer], const float (&y)[kPer]) {
-  float t = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) t = fmaf(x[i], y[i], t);
-  return warp_sum(t);
-}
-
-__device__ __forceinline__ float prob(float s, float lse) {
-  return lse == -INFINITY ? 0.f : exp2f(s - lse);
-}
-
-// dq: a warp for a query, two passes over the keys (sum(p dp), then dq).
-template <typename T>
-__global__ void __launch_bounds__(128) grad_queries(Args a, float* delta) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (long long)a.B * a.H * a.Nq) return;
-  const int n = row % a.Nq, h = row / a.Nq % a.H, b = row / a.Nq / a.H;
-  float q[kPer], g[kPer], k[kPer], v[kPer], dq[kPer] = {};
-  load_row<T>(a.q, b * a.qs.b + n * a.qs.n + h * a.qs.h, a.D, q);
-  load_row<T>(a.dout, b * a.dos.b + n * a.dos.n + h * a.dos.h, a.D, g);
-  const float c = a.scale * kLog2e, lse = a.lse_in[row];
-  float d = 0.f;
-  for (int pass = 0; pass < 2; ++pass) {
-    for (int j = 0; j < a.Nk; ++j) {
-      float bias;
-      if (!key_bias(a, b, j, &bias)) continue;
-      load_row<T>(a.k, b * a.ks.b + j * a.ks.n + h * a.ks.h, a.D, k);
-      load_row<T>(a.v, b * a.vs.b + j * a.vs.n + h * a.vs.h, a.D, v);
-      const float p = prob(fmaf(dot(q, k), c, bias), lse), dp = dot(g, v);
-      if (pass == 0) {
-        d = fmaf(p, dp, d);
-      } else {
-        const float ds = p * (dp - d) * a.scale;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) dq[i] = fmaf(ds, k[i], dq[i]);
-      }
-    }
-  }
-  store_row<T>(a.dq, (((long long)b * a.Nq + n) * a.H + h) * a.D, a.D, dq);
-  if ((threadIdx.x & 31) == 0) delta[row] = d;
-}
-
-// dk and dv: a warp for a key, one pass over the queries.
-template <typename T>
-__global__ void __launch_bounds__(128) grad_keys(Args a) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (long long)a.B * a.H * a.Nk) return;
-  const int j = row % a.Nk, h = row / a.Nk % a.H, b = row / a.Nk / a.H;
-  float k[kPer], v[kPer], q[kPer], g[kPer], dk[kPer] = {}, dv[kPer] = {};
-  float bias;
-  if (key_bias(a, b, j, &bias)) {
-    load_row<T>(a.k, b * a.ks.b + j * a.ks.n + h * a.ks.h, a.D, k);
-    load_row<T>(a.v, b * a.vs.b + j * a.vs.n + h * a.vs.h, a.D, v);
-    const float c = a.scale * kLog2e;
-    for (int n = 0; n < a.Nq; ++n) {
-      const long long r = ((long long)b * a.H + h) * a.Nq + n;
-      load_row<T>(a.q, b * a.qs.b + n * a.qs.n + h * a.qs.h, a.D, q);
-      load_row<T>(a.dout, b * a.dos.b + n * a.dos.n + h * a.dos.h, a.D, g);
-      const float p = prob(fmaf(dot(q, k), c, bias), a.lse_in[r]);
-      const float ds = p * (dot(g, v) - a.delta[r]) * a.scale;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        dk[i] = fmaf(ds, q[i], dk[i]);
-        dv[i] = fmaf(p, g[i], dv[i]);
-      }
-    }
-  }
-  const long long off = (((long long)b * a.Nk + j) * a.H + h) * a.D;
-  store_row<T>(a.dk, off, a.D, dk);
-  store_row<T>(a.dv, off, a.D, dv);
-}
-
 long long workspace_bytes(int B, int Nq, int Nk, int H, int D, bool grad) {
-  return grad ? (long long)B * H * Nq * 4 : forward_workspace_bytes(B, Nq, Nk, H, D);
+  return grad ? backward_workspace_bytes(B, Nq, Nk, H, D) : forward_workspace_bytes(B, Nq, Nk, H, D);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -155,8 +61,6 @@ int done(const char* what, cudaError_t e) {
   return record_error(NOVA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
-unsigned blocks4(long long rows) { return (unsigned)((rows + 3) / 4); }
-
 }  // namespace xattn
 }  // namespace nova
 
@@ -188,6 +92,8 @@ NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const 
   a.B = batch, a.Nq = queries, a.Nk = keys, a.H = heads, a.D = head_dim;
   a.mask_kind = mask_type, a.scale = scale;
   if (const int rc = check("cross_attention", a, dtype, d_workspace, ws_bytes, false)) return rc;
+  const OnDeviceOf device(d_q);
+  if (device.status() != cudaSuccess) return done("cross_attention: q", device.status());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const char* why = nullptr;
   const cudaError_t e = launch_forward(a, dtype == kBF16, d_workspace, s, &why);
@@ -221,19 +127,13 @@ NOVA_EXPORT int nova_cross_attention_grad_v2(
     return rc;
   if (!a.out || !aligned16(a.out))
     return record_error(NOVA_ERR_INVALID_ARGUMENT, "cross_attention_grad: bad output pointer");
+  const OnDeviceOf device(d_q);
+  if (device.status() != cudaSuccess) return done("cross_attention_grad: q", device.status());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float* delta = static_cast<float*>(d_workspace);
-  a.delta = delta;
-  const unsigned gq = blocks4((long long)batch * heads * queries);
-  const unsigned gk = blocks4((long long)batch * heads * keys);
-  if (dtype == kF16) {
-    grad_queries<__half><<<gq, 128, 0, s>>>(a, delta);
-    grad_keys<__half><<<gk, 128, 0, s>>>(a);
-  } else {
-    grad_queries<__nv_bfloat16><<<gq, 128, 0, s>>>(a, delta);
-    grad_keys<__nv_bfloat16><<<gk, 128, 0, s>>>(a);
-  }
-  return done("cross_attention_grad", cudaGetLastError());
+  const char* why = nullptr;
+  const cudaError_t e = launch_backward(a, dtype == kBF16, d_workspace, s, &why);
+  if (why) return record_error(NOVA_ERR_CUDA, std::string("cross_attention_grad: ") + why);
+  return done("cross_attention_grad", e);
 } catch (...) {
   return NOVA_ERR_ALLOC;
 }

@@ -527,6 +527,8 @@ NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, co
   if (const int rc = check("group_norm", a, dtype, d_workspace, ws_bytes, false)) return rc;
   if (activation != kNone && activation != kSilu)
     return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm: bad activation");
+  const OnDeviceOf device(d_input);
+  if (device.status() != cudaSuccess) return done("group_norm: input", device.status());
   unsigned char* ws = static_cast<unsigned char*>(d_workspace);
   float* stats = static_cast<float*>(d_stats);
   if (!stats) {
@@ -577,6 +579,8 @@ NOVA_EXPORT int nova_group_norm_grad_v2(
   if (!d_stats) return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm_grad: null pointer");
   if (activation != kNone && activation != kSilu)
     return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm_grad: bad activation");
+  const OnDeviceOf device(d_input);
+  if (device.status() != cudaSuccess) return done("group_norm_grad: input", device.status());
   unsigned char* ws = static_cast<unsigned char*>(d_workspace);
   const float* stats = static_cast<const float*>(d_stats);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

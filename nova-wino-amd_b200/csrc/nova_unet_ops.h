@@ -16,6 +16,33 @@ enum DType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
 inline bool dtype_ok(int t) { return t == kF16 || t == kBF16 || t == kF32; }
 inline int dtype_bytes(int t) { return t == kF32 ? 4 : 2; }
 
+// Makes the device that `p` lives on, and its context, current for a call: the
+// threads that run a backward pass may come without a context, and a tensor may
+// live on another device than the caller's current one.
+class OnDeviceOf {
+ public:
+  explicit OnDeviceOf(const void* p) {
+    cudaPointerAttributes at{};
+    status_ = cudaPointerGetAttributes(&at, p);
+    if (status_ == cudaSuccess && at.type != cudaMemoryTypeDevice &&
+        at.type != cudaMemoryTypeManaged)
+      status_ = cudaErrorInvalidValue;
+    if (status_ == cudaSuccess) status_ = cudaGetDevice(&before_);
+    if (status_ == cudaSuccess) status_ = cudaSetDevice(at.device);
+    device_ = at.device;
+  }
+  ~OnDeviceOf() {
+    if (before_ >= 0 && before_ != device_) cudaSetDevice(before_);
+  }
+  OnDeviceOf(const OnDeviceOf&) = delete;
+  OnDeviceOf& operator=(const OnDeviceOf&) = delete;
+  cudaError_t status() const { return status_; }
+
+ private:
+  cudaError_t status_ = cudaSuccess;
+  int before_ = -1, device_ = -1;
+};
+
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>

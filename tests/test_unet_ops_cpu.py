@@ -181,8 +181,12 @@ def test_cross_attention_grad_entry_validates(lib):
     for kw in ({"o": None}, {"do": None}, {"lse": None}, {"dq": None}, {"dk": None}, {"dv": None},
                {"do": 8}, {"dk": 8}, {"st": cross_strides(1, 4, 4, 2, 16, i12=20)}):
         assert call(**kw) == 1, kw
-    assert call(n=0) == 3
-    assert call(ws=None) == 1
+    # More keys than one tile: a workspace is needed.
+    long = {"Nk": 300, "st": cross_strides(1, 4, 300, 2, 16)}
+    assert lib.nova_cross_attention_workspace_bytes(1, 4, 300, 2, 16, 1) > 0
+    assert call(n=0, **long) == 3
+    assert call(ws=None, **long) == 1
+    assert call(ws=128, **long) == 1
     assert lib.nova_cross_attention_workspace_bytes(1, 4, 4, 2, 12, 0) == -1
 
 

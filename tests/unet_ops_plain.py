@@ -112,11 +112,13 @@ def cross_attention(q, k, v, mask=None, scale=1.0, do=None, dtype=None):
         mag = torch.einsum("bqhd,bkhd->bhqk", q.abs(), kk.abs()) * abs(scale)
         mag = (mag + torch.where(kept, bias[:, None, None, :].abs().clamp(max=1e4), 0.0)).amax(-1, keepdim=True)
         p_rel = 4 * F32 * (D + 8) * (mag + 1) + SUM * F32
-        # One rounding of p to the element type for the product.  fp16 holds p at least
-        # 2^10 times larger, so that its last half step, 2^-25, is 2^-35 of p's scale.
-        p_off = p * (h + p_rel) + (2.0 ** -35 if dtype == torch.float16 else 0.0) * kept
-        out["o_tol"] = (rounded(dtype, out["o"]) + 1e-12
-                        + torch.einsum("bhqk,bkhd->bqhd", p_off + SUM * F32 * p, vv.abs()))
+        # One rounding of p to the element type for the product.  Below fp16's normal
+        # range that is half a subnormal step, 2^-25, of what the kernels hold: e^(s -
+        # max), at least p, in the forward pass; 2^10 p in the gradient.
+        p_off = p * (h + p_rel)
+        tail = (2.0 ** -25 if dtype == torch.float16 else 0.0) * kept
+        out["o_tol"] = (rounded(dtype, out["o"]) + 1e-12 + torch.einsum(
+            "bhqk,bkhd->bqhd", p_off + tail + SUM * F32 * p, vv.abs()))
     if do is None:
         return out
     out["dv"] = torch.einsum("bhqk,bqhd->bkhd", p, do)
@@ -127,7 +129,8 @@ def cross_attention(q, k, v, mask=None, scale=1.0, do=None, dtype=None):
     out["dk"] = torch.einsum("bhqk,bqhd->bkhd", ds, q)
     if dtype:
         out["dv_tol"] = (rounded(dtype, out["dv"]) + 1e-12
-                         + torch.einsum("bhqk,bqhd->bkhd", p_off + SUM * F32 * p, do.abs()))
+                         + torch.einsum("bhqk,bqhd->bkhd", p_off + tail / 1024 + SUM * F32 * p,
+                                        do.abs()))
         dp_mag = torch.einsum("bqhd,bkhd->bhqk", do.abs(), vv.abs())
         dp_off = F32 * (D + 8) * dp_mag
         # sum(p dp) from the probabilities, or from the rounded o: one rounding of each
@@ -135,11 +138,14 @@ def cross_attention(q, k, v, mask=None, scale=1.0, do=None, dtype=None):
         o_mag = torch.einsum("bqhd,bqhd->bhq", do.abs(), out["o_tol"])[..., None]
         delta_off = ((p * dp_off).sum(-1, keepdim=True) + o_mag
                      + ((p * p_rel + SUM * F32 * p) * dp.abs()).sum(-1, keepdim=True))
-        # One rounding of ds to the element type for the products, and fp16's last
-        # step beside the tile's largest (kept near 2^8 and never below 2^-8).
+        # One rounding of ds to the element type for the products.  fp16 holds ds scaled
+        # so that twice the largest |dp| of some earlier tile of the head, or of this
+        # one, came to 2^10 or more: half a subnormal step, 2^-25, is then at most
+        # 2^-25 * 2 / 2^10 = 2^-34 of the head's largest |dp|.
         ds_off = abs(scale) * p * ((h + p_rel) * (dp - delta).abs() + dp_off + delta_off)
         if dtype == torch.float16:
-            ds_off = ds_off + 2.0 ** -16 * h * ds.abs().amax((-1, -2), keepdim=True)
+            biggest = (dp * kept).abs().amax((-1, -2), keepdim=True)
+            ds_off = ds_off + abs(scale) * 2.0 ** -34 * biggest * kept
         out["dq_tol"] = (rounded(dtype, out["dq"]) + 1e-12 + torch.einsum(
             "bhqk,bkhd->bqhd", ds_off + SUM * F32 * ds.abs(), kk.abs()))
         out["dk_tol"] = (rounded(dtype, out["dk"]) + 1e-12 + torch.einsum(
