@@ -387,6 +387,170 @@ __global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUte
   }
 }
 
+// Up to four queries against many keys: nothing to multiply on the tensor cores,
+// K and V are read once.  A warp takes 8 x (32 / LPK) keys at a time; LPK lanes
+// share a key, 8 elements of its row each, so that a warp's load is whole rows.
+// All K loads of a step are in flight together, then all V loads.  Rows of keys that
+// take no part are not read.  The keys are split over blocks (`per` keys each) and
+// over a block's warps; the warps join in shared memory, the blocks through the
+// workspace.
+constexpr int kTokenWarps = 4, kTokenUnroll = 8, kTokenQueries = 4;
+
+template <typename T, int LPK, int NQ, bool MASK>
+__global__ void __launch_bounds__(kTokenWarps * 32)
+    forward_token(const __grid_constant__ FwdParams p) {
+  constexpr int G = 32 / LPK, U = kTokenUnroll;
+  __shared__ float po[kTokenWarps][NQ][LPK * 8];
+  __shared__ float pm[kTokenWarps][NQ], pl[kTokenWarps][NQ];
+  pdl_wait();
+  const Args& a = p.a;
+  unsigned id = blockIdx.x;
+  const int split = id % p.splits;
+  id /= p.splits;
+  const int h = id % a.H, b = id / a.H;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPK, grp = lane / LPK;
+  const bool in = sub * 8 < a.D;
+  const int first = split * p.per, last = min(a.Nk, first + p.per);
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h + sub * 8;
+  const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h + sub * 8;
+  const float c = a.scale * kLog2e;
+
+  float2 q[NQ][4], o[NQ][4] = {};
+  float m[NQ], l[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    Pack<T, 8> r{};
+    if (in && i < a.Nq)
+      r = load_pack<T, 8>(static_cast<const T*>(a.q) + b * a.qs.b + i * a.qs.n + h * a.qs.h + sub * 8);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[i][e] = make_float2(to_f32(r.e[2 * e]), to_f32(r.e[2 * e + 1]));
+  }
+  for (int k0 = first + warp * (U * G); k0 < last; k0 += kTokenWarps * U * G) {
+    Pack<T, 8> r[U];
+    float bias[U];
+    bool on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = k0 + u * G + grp;
+      on[u] = key < last;
+      bias[u] = 0.f;
+      if (MASK && on[u]) on[u] = key_bias(a, b, key, &bias[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = Pack<T, 8>{};
+      if (on[u] && in) r[u] = load_pack<T, 8>(kp + (long long)(k0 + u * G + grp) * a.ks.n);
+    }
+    float s[NQ][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float2 x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(r[u].e[2 * e]), to_f32(r[u].e[2 * e + 1]));
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        float2 t = __fmul2_rn(x[0], q[i][0]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) t = __ffma2_rn(x[e], q[i][e], t);
+        s[i][u] = t.x + t.y;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = Pack<T, 8>{};
+      if (on[u] && in) r[u] = load_pack<T, 8>(vp + (long long)(k0 + u * G + grp) * a.vs.n);
+    }
+#pragma unroll
+    for (int i = 0; i < NQ; ++i) {
+      float top = m[i];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int w = LPK / 2; w > 0; w >>= 1) s[i][u] += __shfl_xor_sync(~0u, s[i][u], w);
+        s[i][u] = on[u] ? fmaf(s[i][u], c, bias[u]) : -INFINITY;
+        top = fmaxf(top, s[i][u]);
+      }
+      // One maximum for the warp, so that its lanes can add up their sums at the end.
+#pragma unroll
+      for (int w = LPK; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
+      const float base = top == -INFINITY ? 0.f : top;
+      const float f = ex2(m[i] - base);
+      m[i] = top;
+      l[i] *= f;
+      const float2 f2 = make_float2(f, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = __fmul2_rn(o[i][e], f2);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // A key that takes no part has zeros for V and minus infinity for its score.
+        s[i][u] = on[u] ? ex2(s[i][u] - base) : 0.f;
+        l[i] += s[i][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float2 x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(r[u].e[2 * e]), to_f32(r[u].e[2 * e + 1]));
+#pragma unroll
+      for (int i = 0; i < NQ; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = __ffma2_rn(make_float2(s[i][u], s[i][u]), x[e], o[i][e]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NQ; ++i) {
+#pragma unroll
+    for (int w = LPK; w < 32; w <<= 1) {
+      l[i] += __shfl_xor_sync(~0u, l[i], w);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[i][e].x += __shfl_xor_sync(~0u, o[i][e].x, w);
+        o[i][e].y += __shfl_xor_sync(~0u, o[i][e].y, w);
+      }
+    }
+    if (grp == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        po[warp][i][sub * 8 + 2 * e] = o[i][e].x;
+        po[warp][i][sub * 8 + 2 * e + 1] = o[i][e].y;
+      }
+    }
+    if (lane == 0) {
+      pm[warp][i] = m[i];
+      pl[warp][i] = l[i];
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < NQ * LPK * 8; t += kTokenWarps * 32) {
+    const int i = t / (LPK * 8), d = t % (LPK * 8);
+    if (i >= a.Nq || d >= a.D) continue;
+    float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTokenWarps; ++w) top = fmaxf(top, pm[w][i]);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < kTokenWarps; ++w) {
+      const float f = ex2(pm[w][i] - base);
+      sum = fmaf(f, pl[w][i], sum);
+      acc = fmaf(f, po[w][i][d], acc);
+    }
+    const float v = sum == 0.f ? 0.f : acc / sum;
+    const long long row = ((long long)b * a.H + h) * a.Nq + i;
+    const long long off = (((long long)b * a.Nq + i) * a.H + h) * a.D + d;
+    const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+    if (p.splits > 1) {
+      p.part_o[(long long)split * a.B * a.Nq * a.H * a.D + off] = v;
+      if (d == 0) p.part_lse[(long long)split * a.B * a.H * a.Nq + row] = lse;
+    } else {
+      static_cast<T*>(a.out)[off] = from_f32<T>(v);
+      if (d == 0 && a.lse) a.lse[row] = lse;
+    }
+  }
+}
+
 // Joins the splits' rows: a warp for a row.
 template <typename T>
 __global__ void __launch_bounds__(128) join_splits(const __grid_constant__ FwdParams p) {
@@ -470,6 +634,48 @@ namespace {
 
 constexpr size_t kSmemMax = 227 * 1024 - 1024;  // beside the static part
 
+// Few queries, more keys than one tile: the form without tensor cores.
+bool is_token(const Args& a) { return a.Nq <= kTokenQueries && a.Nk > 128; }
+
+// Its split: blocks for four times the SMs, of at least one step of every warp.
+void plan_token(FwdParams* p, int sms) {
+  const Args& a = p->a;
+  const int lanes = a.D <= 64 ? 8 : a.D <= 128 ? 16 : 32;
+  const int step = kTokenWarps * kTokenUnroll * (32 / lanes);
+  const long long heads = (long long)a.B * a.H;
+  long long want = (4ll * sms + heads - 1) / heads;
+  const int steps = (a.Nk + step - 1) / step;
+  if (want > steps) want = steps;
+  if (want > 64) want = 64;  // what the joining pass reads for a row
+  p->per = (int)((steps + want - 1) / want) * step;
+  p->splits = (a.Nk + p->per - 1) / p->per;
+}
+
+template <typename T, int LPK, int NQ>
+cudaError_t run_token_n(const FwdParams& p, cudaStream_t s) {
+  const dim3 grid((unsigned)((long long)p.a.B * p.a.H * p.splits)), block(kTokenWarps * 32);
+  return p.a.mask_kind == kMaskNone
+             ? launch_pdl(kPdlInput, forward_token<T, LPK, NQ, false>, grid, block, 0, s, p)
+             : launch_pdl(kPdlInput, forward_token<T, LPK, NQ, true>, grid, block, 0, s, p);
+}
+template <typename T, int LPK>
+cudaError_t run_token_l(const FwdParams& p, cudaStream_t s) {
+  if (p.a.Nq == 1) return run_token_n<T, LPK, 1>(p, s);
+  if (p.a.Nq == 2) return run_token_n<T, LPK, 2>(p, s);
+  return run_token_n<T, LPK, kTokenQueries>(p, s);
+}
+template <typename T>
+cudaError_t run_token(const FwdParams& p, cudaStream_t s) {
+  cudaError_t e = p.a.D <= 64    ? run_token_l<T, 8>(p, s)
+                  : p.a.D <= 128 ? run_token_l<T, 16>(p, s)
+                                 : run_token_l<T, 32>(p, s);
+  if (e == cudaSuccess && p.splits > 1) {
+    const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
+    e = launch_pdl(kPdlInput, join_splits<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p);
+  }
+  return e;
+}
+
 // The split of one call over blocks, tiles and stages.
 void plan(FwdParams* p, int sms) {
   const Args& a = p->a;
@@ -544,7 +750,8 @@ cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
 long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
   FwdParams p{};
   p.a.B = B, p.a.Nq = Nq, p.a.Nk = Nk, p.a.H = H, p.a.D = D;
-  plan(&p, device_sms());
+  if (is_token(p.a)) plan_token(&p, device_sms());
+  else plan(&p, device_sms());
   if (p.splits == 1) return 0;
   const size_t rows = (size_t)B * H * Nq * p.splits;
   return (long long)(align256(rows * D * 4) + align256(rows * 4));
@@ -553,12 +760,15 @@ long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
 cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why) {
   FwdParams p{};
   p.a = a;
-  plan(&p, device_sms());
+  const bool token = is_token(a);
+  if (token) plan_token(&p, device_sms());
+  else plan(&p, device_sms());
   const size_t rows = (size_t)a.B * a.H * a.Nq * p.splits;
   p.part_o = static_cast<float*>(ws);
   p.part_lse = p.splits > 1 ? reinterpret_cast<float*>(static_cast<unsigned char*>(ws) +
                                                        align256(rows * a.D * 4))
                             : nullptr;
+  if (token) return bf16 ? run_token<__nv_bfloat16>(p, s) : run_token<__half>(p, s);
   CUtensorMap m[4];
   const Strides dense{(long long)a.Nq * a.H * a.D, (long long)a.H * a.D, a.D};
   if (!encode_tile4(&m[0], &p.qp, a.q, a.qs, a.B, a.Nq, a.H, a.D, kRows, bf16) ||

@@ -56,17 +56,81 @@ struct Walk {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-template <int ACT>
-__device__ __forceinline__ float act(float z) {
-  return ACT == kSilu ? __fdividef(z, 1.f + __expf(-z)) : z;
+// Channels are worked on in pairs (the paired 32-bit instructions halve the count),
+// or singly where a thread holds one.
+__device__ __forceinline__ float2 add(float2 x, float2 y) { return __fadd2_rn(x, y); }
+__device__ __forceinline__ float2 mul(float2 x, float2 y) { return __fmul2_rn(x, y); }
+__device__ __forceinline__ float2 fma(float2 x, float2 y, float2 z) { return __ffma2_rn(x, y, z); }
+__device__ __forceinline__ float add(float x, float y) { return x + y; }
+__device__ __forceinline__ float mul(float x, float y) { return x * y; }
+__device__ __forceinline__ float fma(float x, float y, float z) { return fmaf(x, y, z); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-template <int ACT>
-__device__ __forceinline__ float act_grad(float z) {
-  if (ACT != kSilu) return 1.f;
-  const float s = sigmoid(z);
-  return s * fmaf(z, 1.f - s, 1.f);
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
+__device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
+template <typename F>
+__device__ __forceinline__ F splat(float x);
+template <>
+__device__ __forceinline__ float splat<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float2 splat<float2>(float x) { return make_float2(x, x); }
+
+template <typename F>
+__device__ __forceinline__ F sigmoid(F z) {
+  return rcp(add(ex2(mul(z, splat<F>(-1.4426950408889634f))), splat<F>(1.f)));
+}
+template <int ACT, typename F>
+__device__ __forceinline__ F act(F z) {
+  return ACT == kSilu ? mul(z, sigmoid(z)) : z;
+}
+// dy act'(z); silu: s (1 + z (1 - s)) = s + (z s) (1 - s).
+template <int ACT, typename F>
+__device__ __forceinline__ F act_grad(F dy, F z) {
+  if (ACT != kSilu) return dy;
+  const F s = sigmoid(z), zs = mul(z, s);
+  return mul(dy, fma(zs, fma(s, splat<F>(-1.f), splat<F>(1.f)), s));
+}
+
+// Channels j W .. j W + W - 1 of a vector, and of an array in shared memory or
+// registers.
+template <typename T, int V>
+struct Lanes {
+  static constexpr int W = 2;
+  using F = float2;
+  static __device__ __forceinline__ float2 get(const Pack<T, V>& p, int j) {
+    return make_float2(to_f32(p.e[2 * j]), to_f32(p.e[2 * j + 1]));
+  }
+  static __device__ __forceinline__ void set(Pack<T, V>& p, int j, float2 f) {
+    p.e[2 * j] = from_f32<T>(f.x);
+    p.e[2 * j + 1] = from_f32<T>(f.y);
+  }
+  static __device__ __forceinline__ float2 at(const float* a, int j) {
+    return make_float2(a[2 * j], a[2 * j + 1]);
+  }
+  static __device__ __forceinline__ void put(float* a, int j, float2 f) {
+    a[2 * j] = f.x;
+    a[2 * j + 1] = f.y;
+  }
+};
+template <typename T>
+struct Lanes<T, 1> {
+  static constexpr int W = 1;
+  using F = float;
+  static __device__ __forceinline__ float get(const Pack<T, 1>& p, int) { return to_f32(p.e[0]); }
+  static __device__ __forceinline__ void set(Pack<T, 1>& p, int, float f) {
+    p.e[0] = from_f32<T>(f);
+  }
+  static __device__ __forceinline__ float at(const float* a, int) { return a[0]; }
+  static __device__ __forceinline__ void put(float* a, int, float f) { a[0] = f; }
+};
 
 // Joins (nb, mb, qb) into (na, ma, qa): counts, means, squared deviations.
 __device__ __forceinline__ void join(float& na, float& ma, float& qa, float nb, float mb,
@@ -104,6 +168,8 @@ __global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2
   __shared__ float2 red[kThreads * V];
   pdl_wait();
   const Place q = place(a, k);
+  using L = Lanes<T, V>;
+  using F = typename L::F;
   float s1[V] = {}, s2[V] = {}, pivot[V] = {};
   int n = 0;
   if (q.active && q.p0 + q.ty < q.p1) {
@@ -117,10 +183,10 @@ __global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2
     for (int i = 0; i < n; ++i, p += step) {
       const Pack<T, V> v = load_pack<T, V>(p);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = to_f32(v.e[e]) - pivot[e];
-        s1[e] += d;
-        s2[e] = fmaf(d, d, s2[e]);
+      for (int j = 0; j < V / L::W; ++j) {
+        const F d = fma(L::at(pivot, j), splat<F>(-1.f), L::get(v, j));
+        L::put(s1, j, add(L::at(s1, j), d));
+        L::put(s2, j, fma(d, d, L::at(s2, j)));
       }
     }
   }
@@ -220,9 +286,10 @@ __global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* s
   pdl_wait();
   const Place q = place(a, k);
   if (!q.active) return;
+  using L = Lanes<T, V>;
   Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
 #pragma unroll
-  for (int e = 0; e < V; ++e) h.w[e] *= h.r[e];
+  for (int e = 0; e < V; ++e) h.w[e] *= h.r[e], h.mu[e] = -h.mu[e];
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   T* y = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
 #pragma unroll 4
@@ -230,8 +297,8 @@ __global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* s
     const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
     Pack<T, V> o;
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      o.e[e] = from_f32<T>(act<ACT>(fmaf(to_f32(v.e[e]) - h.mu[e], h.w[e], h.beta[e])));
+    for (int j = 0; j < V / L::W; ++j)
+      L::set(o, j, act<ACT>(fma(add(L::get(v, j), L::at(h.mu, j)), L::at(h.w, j), L::at(h.beta, j))));
     store_pack<T, V>(y + (long long)p * a.C, o);
   }
 }
@@ -243,9 +310,13 @@ __global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const f
   __shared__ float red[3][kThreads * V];
   pdl_wait();
   const Place q = place(a, k);
+  using L = Lanes<T, V>;
+  using F = typename L::F;
   float s1[V] = {}, s2[V] = {}, s3[V] = {};
   if (q.active) {
-    const Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+    Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+#pragma unroll
+    for (int e = 0; e < V; ++e) h.mu[e] = -h.mu[e];
     const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
     const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
 #pragma unroll 2
@@ -253,12 +324,12 @@ __global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const f
       const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
       const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float n = (to_f32(v.e[e]) - h.mu[e]) * h.r[e];
-        const float dz = to_f32(d.e[e]) * act_grad<ACT>(fmaf(n, h.w[e], h.beta[e]));
-        s1[e] += dz;
-        s2[e] = fmaf(dz, n, s2[e]);
-        s3[e] += n;
+      for (int j = 0; j < V / L::W; ++j) {
+        const F n = mul(add(L::get(v, j), L::at(h.mu, j)), L::at(h.r, j));
+        const F dz = act_grad<ACT>(L::get(d, j), fma(n, L::at(h.w, j), L::at(h.beta, j)));
+        L::put(s1, j, add(L::at(s1, j), dz));
+        L::put(s2, j, fma(dz, n, L::at(s2, j)));
+        L::put(s3, j, add(L::at(s3, j), n));
       }
     }
   }
@@ -355,13 +426,16 @@ __global__ void __launch_bounds__(kThreads) apply_grad(Args a, Walk k, const flo
   pdl_wait();
   const Place q = place(a, k);
   if (!q.active) return;
-  const Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+  using L = Lanes<T, V>;
+  using F = typename L::F;
+  Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
   float A[V], D[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
+    h.mu[e] = -h.mu[e];
     const float2 m = means[(long long)q.b * a.G + (q.col * V + e) / a.cpg];
-    A[e] = m.x;
-    D[e] = m.y;
+    A[e] = -m.x;
+    D[e] = -m.y;
   }
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
@@ -372,13 +446,384 @@ __global__ void __launch_bounds__(kThreads) apply_grad(Args a, Walk k, const flo
     const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
     Pack<T, V> o;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float n = (to_f32(v.e[e]) - h.mu[e]) * h.r[e];
-      const float dz = to_f32(d.e[e]) * act_grad<ACT>(fmaf(n, h.w[e], h.beta[e]));
-      o.e[e] = from_f32<T>(h.r[e] * (fmaf(h.w[e], dz, -A[e]) - n * D[e]));
+    for (int j = 0; j < V / L::W; ++j) {
+      const F r = L::at(h.r, j), w = L::at(h.w, j);
+      const F n = mul(add(L::get(v, j), L::at(h.mu, j)), r);
+      const F dz = act_grad<ACT>(L::get(d, j), fma(n, w, L::at(h.beta, j)));
+      L::set(o, j, mul(r, fma(n, L::at(D, j), fma(w, dz, L::at(A, j)))));
     }
     store_pack<T, V>(dx + (long long)p * a.C, o);
   }
+}
+
+// ---------------------------------------------------------------------------
+// Resident form: a cluster of blocks keeps a sample's channel block in registers
+// ---------------------------------------------------------------------------
+//
+// x is read once and y written once.  A cluster of `cs` blocks owns `gb` whole
+// groups of one sample, each block a range of the pixels, every thread up to NV
+// vectors of it.  The blocks form (mean, squared deviations) of their range in two
+// passes over their registers and exchange them through distributed shared memory.
+
+struct Slab {
+  int gb, nblk;  // groups per channel block, channel blocks
+  int cs;        // blocks of a cluster
+  int ppc;       // pixels per block
+  int tx, ty;    // threads: vector columns x pixels
+  int nv;        // vectors per thread
+  int threads;
+};
+
+constexpr int kSlabThreads = 512;
+
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// A float of the same shared variable in the cluster's block `rank`.
+__device__ __forceinline__ float peer_float(const float* p, int rank) {
+  uint32_t at;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;"
+      : "=r"(at)
+      : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// Keeps a vector packed: without this the compiler holds the 32-bit forms of all
+// vectors from one pass over them to the next, which spills.
+template <typename T, int V, int NV>
+__device__ __forceinline__ void stay_packed(Pack<T, V> (&d)[NV]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      uint4& q = reinterpret_cast<uint4&>(d[v]);
+      asm volatile("" : "+r"(q.x), "+r"(q.y), "+r"(q.z), "+r"(q.w));
+    }
+  }
+}
+
+__device__ __forceinline__ float warp_total(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+struct Spot {
+  int b, rank, c0, nch, ng, g0, p0, p1, tx, ty, nv;
+  bool active;
+};
+__device__ __forceinline__ Spot spot(const Args& a, const Slab& k, int V) {
+  Spot q;
+  unsigned id = blockIdx.x;
+  q.rank = id % k.cs;
+  id /= k.cs;
+  const int blk = id % k.nblk;
+  q.b = id / k.nblk;
+  q.g0 = blk * k.gb;
+  q.ng = min(k.gb, a.G - q.g0);
+  q.c0 = q.g0 * a.cpg;
+  q.nch = q.ng * a.cpg;
+  q.p0 = min(a.HW, q.rank * k.ppc);
+  q.p1 = min(a.HW, q.p0 + k.ppc);
+  q.tx = threadIdx.x % k.tx;
+  q.ty = threadIdx.x / k.tx;
+  q.active = q.ty < k.ty && q.tx * V < q.nch;
+  const int left = q.p1 - q.p0 - q.ty;
+  q.nv = q.active && left > 0 ? (left + k.ty - 1) / k.ty : 0;
+  return q;
+}
+
+template <typename T, int V, int NV, int ACT>
+__global__ void __launch_bounds__(kSlabThreads, 1)
+    resident_forward(Args a, Slab k, float* stats) {
+  using L = Lanes<T, V>;
+  using F = typename L::F;
+  constexpr int W = L::W;
+  extern __shared__ float sm[];
+  const int width = k.tx * V;  // channels of the block, padded to vectors
+  float* red = sm;                      // [ty][width]
+  float* mu = red + k.ty * width;       // [width] what is added to x: shift - mean
+  float* sh = mu + width;               // [width] shift
+  float* wt = sh + width;               // [width] weight, later weight / sigma
+  float* bt = wt + width;               // [width] bias, later the whole offset
+  float* part = bt + width;             // [2][gb] the block's mean and deviations
+  pdl_wait();
+  const Spot q = spot(a, k, V);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+
+  Pack<T, V> d[NV];
+  {
+    const T* x = static_cast<const T*>(a.x) + q.b * a.xb + (q.p0 + q.ty) * a.xp + q.c0 + q.tx * V;
+    const long long step = k.ty * a.xp;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (v < q.nv) d[v] = load_pack<T, V>(x + v * step);
+  }
+  for (int c = threadIdx.x; c < q.nch; c += blockDim.x) {
+    sh[c] = a.shift ? load_param(a.shift, a.stype, (long long)q.b * a.C + q.c0 + c) : 0.f;
+    wt[c] = a.w ? load_param(a.w, a.wtype, q.c0 + c) : 1.f;
+    bt[c] = a.beta ? load_param(a.beta, a.wtype, q.c0 + c) : 0.f;
+  }
+  float* mine = red + q.ty * width + q.tx * V;
+  // Most threads hold NV vectors and need no test for each: every pass comes twice.
+  const auto pass = [&](auto&& body) {
+    if (!q.active) return;
+    if (q.nv == NV) body([](int) { return true; });
+    else body([&](int v) { return v < q.nv; });
+  };
+  pass([&](auto has) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) {
+      F t = splat<F>(0.f);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (has(v)) t = add(t, L::get(d[v], j));
+      L::put(mine, j, t);
+    }
+  });
+  __syncthreads();
+  stay_packed(d);
+  // `segs` threads for every channel add up their rows; a warp then takes a group's
+  // segs x cpg sums.
+  const int segs = max(1, min(k.ty, (int)blockDim.x / width));
+  auto fold_rows = [&] {
+    for (int i = threadIdx.x; i < width * segs; i += blockDim.x) {
+      const int sg = i / width, c = i - sg * width;
+      float t = 0.f;
+      for (int r = sg; r < k.ty; r += segs) t += red[r * width + c];
+      red[sg * width + c] = t;  // no other thread reads this row's channel
+    }
+    __syncthreads();
+  };
+  auto group_sum = [&](int g) {
+    float t = 0.f;
+    for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32)
+      for (int r = 0; r < segs; ++r) t += red[r * width + c];
+    return t;
+  };
+  fold_rows();
+  const float pixels = (float)(q.p1 - q.p0);
+  for (int g = warp; g < q.ng; g += warps) {
+    float t = group_sum(g);
+    for (int c = lane; c < a.cpg; c += 32) t = fmaf(pixels, sh[g * a.cpg + c], t);
+    const float m = pixels > 0.f ? warp_total(t) / (pixels * a.cpg) : 0.f;
+    for (int c = lane; c < a.cpg; c += 32) mu[g * a.cpg + c] = sh[g * a.cpg + c] - m;
+    if (lane == 0) part[g] = m;
+  }
+  __syncthreads();
+  pass([&](auto has) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) {
+      const F m = L::at(mu + q.tx * V, j);
+      F t = splat<F>(0.f);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (has(v)) {
+          const F u = add(L::get(d[v], j), m);
+          t = fma(u, u, t);
+        }
+      L::put(mine, j, t);
+    }
+  });
+  __syncthreads();
+  stay_packed(d);
+  fold_rows();
+  for (int g = warp; g < q.ng; g += warps) {
+    const float t = warp_total(group_sum(g));
+    if (lane == 0) part[k.gb + g] = t;
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int g = warp; g < q.ng; g += warps) {
+    // Every block joins the cluster's parts in the same order.
+    float pm = 0.f, pq = 0.f;
+    if (lane < k.cs) {
+      pm = peer_float(part + g, lane);
+      pq = peer_float(part + k.gb + g, lane);
+    }
+    float n = 0.f, m = 0.f, s = 0.f;
+    for (int r = 0; r < k.cs; ++r) {
+      const float np = (float)max(0, min(k.ppc, a.HW - r * k.ppc)) * a.cpg;
+      join(n, m, s, np, __shfl_sync(~0u, pm, r), __shfl_sync(~0u, pq, r));
+    }
+    const float rstd = 1.f / sqrtf(s / n + a.eps);
+    if (stats && q.rank == 0 && lane == 0) {
+      const long long bg = (long long)q.b * a.G + q.g0 + g;
+      stats[bg] = m;
+      stats[(long long)a.B * a.G + bg] = rstd;
+    }
+    for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32) {
+      mu[c] = sh[c] - m;
+      wt[c] *= rstd;
+    }
+  }
+  cluster_arrive();  // this block has read its peers' parts
+  __syncthreads();
+  pass([&](auto has) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) {
+      const F m = L::at(mu + q.tx * V, j), w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (has(v)) L::set(d[v], j, act<ACT>(fma(add(L::get(d[v], j), m), w, b)));
+    }
+    T* y = static_cast<T*>(a.y) + ((long long)q.b * a.HW + q.p0 + q.ty) * a.C + q.c0 + q.tx * V;
+    const long long step = (long long)k.ty * a.C;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (has(v)) store_pack<T, V>(y + v * step, d[v]);
+  });
+  cluster_wait();
+}
+
+// The gradient of a slab: x and dy in registers, the channels' sums exchanged.
+template <typename T, int V, int NV, int ACT>
+__global__ void __launch_bounds__(kSlabThreads, 1)
+    resident_grad(Args a, Slab k, const float* stats, float2* sums, void* dshift) {
+  using L = Lanes<T, V>;
+  using F = typename L::F;
+  constexpr int W = L::W;
+  extern __shared__ float sm[];
+  const int width = k.tx * V;
+  const int rows = k.ty * width;
+  float* red = sm;                 // [3][ty][width]
+  float* mu = red + 3 * rows;      // [width] each
+  float* rs = mu + width;
+  float* wt = rs + width;
+  float* bt = wt + width;
+  float* own = bt + width;         // [3][width] the block's sums
+  float* all = own + 3 * width;    // [3][width] the sample's sums
+  float* ga = all + 3 * width;     // [width] -A
+  float* gd = ga + width;          // [width] -D
+  pdl_wait();
+  const Spot q = spot(a, k, V);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+
+  Pack<T, V> d[NV], e[NV];
+  {
+    const T* x = static_cast<const T*>(a.x) + q.b * a.xb + (q.p0 + q.ty) * a.xp + q.c0 + q.tx * V;
+    const T* y = static_cast<const T*>(a.dy) + q.b * a.yb + (q.p0 + q.ty) * a.yp + q.c0 + q.tx * V;
+    const long long sx = k.ty * a.xp, sy = k.ty * a.yp;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (v < q.nv) {
+        d[v] = load_pack<T, V>(x + v * sx);
+        e[v] = load_pack<T, V>(y + v * sy);
+      }
+  }
+  for (int c = threadIdx.x; c < q.nch; c += blockDim.x) {
+    const long long bg = (long long)q.b * a.G + q.g0 + c / a.cpg;
+    mu[c] = (a.shift ? load_param(a.shift, a.stype, (long long)q.b * a.C + q.c0 + c) : 0.f) -
+            stats[bg];
+    rs[c] = stats[(long long)a.B * a.G + bg];
+    wt[c] = a.w ? load_param(a.w, a.wtype, q.c0 + c) : 1.f;
+    bt[c] = a.beta ? load_param(a.beta, a.wtype, q.c0 + c) : 0.f;
+  }
+  __syncthreads();
+  const auto pass = [&](auto&& body) {
+    if (!q.active) return;
+    if (q.nv == NV) body([](int) { return true; });
+    else body([&](int v) { return v < q.nv; });
+  };
+  pass([&](auto has) {
+    float* mine = red + q.ty * width + q.tx * V;
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) {
+      const F m = L::at(mu + q.tx * V, j), r = L::at(rs + q.tx * V, j);
+      const F w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
+      F s1 = splat<F>(0.f), s2 = s1, s3 = s1;
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (has(v)) {
+          const F n = mul(add(L::get(d[v], j), m), r);
+          const F dz = act_grad<ACT>(L::get(e[v], j), fma(n, w, b));
+          s1 = add(s1, dz);
+          s2 = fma(dz, n, s2);
+          s3 = add(s3, n);
+        }
+      L::put(mine, j, s1);
+      L::put(mine + rows, j, s2);
+      L::put(mine + 2 * rows, j, s3);
+    }
+  });
+  __syncthreads();
+  stay_packed(d);
+  stay_packed(e);
+  // A few threads for every channel, then one.
+  const int segs = max(1, min(k.ty, (int)blockDim.x / (3 * width)));
+  for (int i = threadIdx.x; i < 3 * width * segs; i += blockDim.x) {
+    const int sg = i / (3 * width), s = i / width % 3, c = i % width;
+    float t = 0.f;
+    if (c < q.nch)
+      for (int r = sg; r < k.ty; r += segs) t += red[s * rows + r * width + c];
+    // The first row that this thread alone has read takes its sum.
+    red[s * rows + sg * width + c] = t;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 3 * width; i += blockDim.x) {
+    const int s = i / width, c = i % width;
+    float t = 0.f;
+    for (int r = 0; r < segs; ++r) t += red[s * rows + r * width + c];
+    own[i] = t;
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int i = threadIdx.x; i < 3 * width; i += blockDim.x) {
+    float t = 0.f;
+    for (int r = 0; r < k.cs; ++r) t += peer_float(own + i, r);
+    all[i] = t;
+  }
+  cluster_arrive();
+  __syncthreads();
+  const float inv = 1.f / ((float)a.HW * a.cpg);
+  for (int g = warp; g < q.ng; g += warps) {
+    float wa = 0.f, wd = 0.f;
+    for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32) {
+      wa = fmaf(wt[c], all[c], wa);
+      wd = fmaf(wt[c], all[width + c], wd);
+    }
+    wa = warp_total(wa) * inv;
+    wd = warp_total(wd) * inv;
+    for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32) {
+      ga[c] = -wa;
+      gd[c] = -wd;
+      if (q.rank == 0) {
+        const long long bc = (long long)q.b * a.C + q.c0 + c;
+        sums[bc] = make_float2(all[c], all[width + c]);
+        if (dshift)
+          store_param(dshift, a.stype, bc,
+                      rs[c] * (wt[c] * all[c] - a.HW * wa - wd * all[2 * width + c]));
+      }
+    }
+  }
+  __syncthreads();
+  pass([&](auto has) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) {
+      const F m = L::at(mu + q.tx * V, j), r = L::at(rs + q.tx * V, j);
+      const F w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
+      const F A = L::at(ga + q.tx * V, j), D = L::at(gd + q.tx * V, j);
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+        if (has(v)) {
+          const F n = mul(add(L::get(d[v], j), m), r);
+          const F dz = act_grad<ACT>(L::get(e[v], j), fma(n, w, b));
+          L::set(d[v], j, mul(r, fma(n, D, fma(w, dz, A))));
+        }
+    }
+    T* y = static_cast<T*>(a.y) + ((long long)q.b * a.HW + q.p0 + q.ty) * a.C + q.c0 + q.tx * V;
+    const long long step = (long long)k.ty * a.C;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (has(v)) store_pack<T, V>(y + v * step, d[v]);
+  });
+  cluster_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -428,8 +873,113 @@ long long workspace_bytes(int B, int HW, int C, int G, bool grad) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// The resident form of a call, where its slabs fit.  `most` vectors a thread.
+bool make_slab(int B, int HW, int C, int G, int V, int most, int sms, Slab* best) {
+  const int cpg = C / G;
+  const int unit = V / gcd(cpg, V);  // groups whose channels fill whole vectors
+  bool found = false;
+  double best_cost = 0;
+  for (int gb = unit;; gb *= 2) {
+    if (gb > G) gb = G;
+    const int tx = gb * cpg / V;
+    if (tx > kSlabThreads) break;
+    for (int cs = 1; cs <= 8; cs *= 2)
+      for (int nv = 2; nv <= most; nv *= 2) {
+        Slab k;
+        k.gb = gb;
+        k.nblk = (G + gb - 1) / gb;
+        k.cs = cs;
+        k.ppc = (HW + cs - 1) / cs;
+        k.tx = tx;
+        k.nv = nv;
+        k.ty = (k.ppc + nv - 1) / nv;
+        k.threads = (tx * k.ty + 31) / 32 * 32;
+        if (k.threads > kSlabThreads) continue;
+        const long long blocks = (long long)B * k.nblk * cs;
+        const int regs = nv * 4 * (most < 16 ? 2 : 1) + 64;
+        int per_sm = 65536 / (regs * k.threads);
+        if (per_sm > 32) per_sm = 32;
+        const long long waves = (blocks + (long long)sms * per_sm - 1) / ((long long)sms * per_sm);
+        const double row = (double)tx * 16;
+        const double bytes = (double)k.ppc * (row + 16);
+        const double busy = blocks < (long long)sms * per_sm ? (double)blocks / sms : per_sm;
+        const double cost = waves * ((busy < 1 ? 1 : busy) * bytes / 22.0 + 3500.0) + 200.0 * cs;
+        if (!found || cost < best_cost) {
+          found = true;
+          best_cost = cost;
+          *best = k;
+        }
+      }
+    if (gb >= G) break;
+  }
+  return found;
+}
+
+size_t slab_smem(const Slab& k, int V, bool grad) {
+  const size_t width = (size_t)k.tx * V;
+  return 4 * (grad ? 3 * k.ty * width + 12 * width : k.ty * width + 4 * width + 2 * k.gb);
+}
+
+template <typename... KArgs, typename... Args2>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int cs,
+                           size_t smem, cudaStream_t s, Args2&&... args) {
+  cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(kPdlInput) ? 1 : 0;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args2>(args)...);
+}
+
+constexpr int kMostForward = 16, kMostGrad = 8;  // vectors a thread can hold
+
+template <typename T, int V, int ACT>
+cudaError_t forward_resident(const Args& a, const Slab& k, float* stats, cudaStream_t s) {
+  const unsigned grid = (unsigned)((long long)a.B * k.nblk * k.cs);
+  const size_t smem = slab_smem(k, V, false);
+#define NOVA_GN_SLAB(NV) \
+  launch_cluster(resident_forward<T, V, NV, ACT>, grid, k.threads, k.cs, smem, s, a, k, stats)
+  if (k.nv <= 2) return NOVA_GN_SLAB(2);
+  if (k.nv <= 4) return NOVA_GN_SLAB(4);
+  if (k.nv <= 8) return NOVA_GN_SLAB(8);
+  return NOVA_GN_SLAB(16);
+#undef NOVA_GN_SLAB
+}
+
+template <typename T, int V, int ACT>
+cudaError_t grad_resident(const Args& a, const Slab& k, const float* stats, float2* sums,
+                          void* dshift, cudaStream_t s) {
+  const unsigned grid = (unsigned)((long long)a.B * k.nblk * k.cs);
+  const size_t smem = slab_smem(k, V, true);
+#define NOVA_GN_SLAB(NV)                                                                     \
+  launch_cluster(resident_grad<T, V, NV, ACT>, grid, k.threads, k.cs, smem, s, a, k, stats, \
+                 sums, dshift)
+  if (k.nv <= 2) return NOVA_GN_SLAB(2);
+  if (k.nv <= 4) return NOVA_GN_SLAB(4);
+  return NOVA_GN_SLAB(8);
+#undef NOVA_GN_SLAB
+}
+
 template <typename T, int V>
-cudaError_t forward(const Args& a, int act, float* stats, unsigned char* ws, cudaStream_t s) {
+cudaError_t forward(const Args& a, int act, float* stats, bool want_stats, unsigned char* ws,
+                    cudaStream_t s) {
+  Slab slab;
+  if (make_slab(a.B, a.HW, a.C, a.G, V, kMostForward, device_sms(), &slab))
+    return act == kSilu ? forward_resident<T, V, kSilu>(a, slab, want_stats ? stats : nullptr, s)
+                        : forward_resident<T, V, kNone>(a, slab, want_stats ? stats : nullptr, s);
   const Walk k = make_walk(a.B, a.HW, a.C, V);
   float2* part = reinterpret_cast<float2*>(ws);
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
@@ -454,7 +1004,16 @@ cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, v
   ws += align256((size_t)a.B * a.C * 8);
   float2* means = reinterpret_cast<float2*>(ws);
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
-  cudaError_t e = launch_pdl(kPdlInput, partial_grad<T, V, ACT>, grid, dim3(kThreads), 0, s, a, k,
+  cudaError_t e;
+  Slab slab;
+  if (make_slab(a.B, a.HW, a.C, a.G, V, kMostGrad, device_sms(), &slab)) {
+    e = grad_resident<T, V, ACT>(a, slab, stats, sums, dshift, s);
+    if (e == cudaSuccess && (dw || dbeta))
+      e = launch_pdl(kPdlInput, param_grad, dim3((a.C + 127) / 128), dim3(128), 0, s, a,
+                     (const float2*)sums, dw, dbeta);
+    return e;
+  }
+  e = launch_pdl(kPdlInput, partial_grad<T, V, ACT>, grid, dim3(kThreads), 0, s, a, k,
                              stats, part);
   if (e == cudaSuccess)
     e = launch_pdl(kPdlInput, finish_grad, dim3(a.B * a.G), dim3(128), a.cpg * sizeof(float), s, a,
@@ -539,14 +1098,14 @@ NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, co
   const bool v = wide(a, dtype, false);
   cudaError_t e;
   if (dtype == kF16)
-    e = v ? forward<__half, 8>(a, activation, stats, ws, s)
-          : forward<__half, 1>(a, activation, stats, ws, s);
+    e = v ? forward<__half, 8>(a, activation, stats, d_stats != nullptr, ws, s)
+          : forward<__half, 1>(a, activation, stats, d_stats != nullptr, ws, s);
   else if (dtype == kBF16)
-    e = v ? forward<__nv_bfloat16, 8>(a, activation, stats, ws, s)
-          : forward<__nv_bfloat16, 1>(a, activation, stats, ws, s);
+    e = v ? forward<__nv_bfloat16, 8>(a, activation, stats, d_stats != nullptr, ws, s)
+          : forward<__nv_bfloat16, 1>(a, activation, stats, d_stats != nullptr, ws, s);
   else
-    e = v ? forward<float, 4>(a, activation, stats, ws, s)
-          : forward<float, 1>(a, activation, stats, ws, s);
+    e = v ? forward<float, 4>(a, activation, stats, d_stats != nullptr, ws, s)
+          : forward<float, 1>(a, activation, stats, d_stats != nullptr, ws, s);
   return done("group_norm", e);
 } catch (...) {
   return NOVA_ERR_ALLOC;
