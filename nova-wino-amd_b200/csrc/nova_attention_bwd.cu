@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // S and dP of step i; its tiles have landed when this returns true.
   auto start_scores = [&](int i) {
     const int st = i % p.stages;
-    if (!mbar_wait(bx + 8u * st, (i / p.stages) & 1, &abort_flag, &g_status, kDevTimeoutProducer))
+    if (!wait_phase(bx + 8u * st, (i / p.stages) & 1, &abort_flag, &g_status, kDevTimeoutProducer))
       return false;
     tc_fence_after();
     const uint32_t x = s_walk + 2 * st * walk_bytes;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_smem();
     }
   };
-  ok = mbar_wait(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
+  ok = wait_phase(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
   if (MASK && kWalkQ) {
     set_bias(kt_fix, 0);
     if (MODE == kBoth && ok) clear_masked(s_fix, 0);
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       lse_next = row_lse(t_first + i + 1);
       if (MODE == kKeys) delta_next = row_delta(t_first + i + 1);
     }
-    ok = mbar_wait(bs, i & 1, &abort_flag, &g_status, kDevTimeoutMma);
+    ok = wait_phase(bs, i & 1, &abort_flag, &g_status, kDevTimeoutMma);
     __syncwarp();
     tc_fence_after();
 
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit(bd);
       if (p.early && i + 1 < steps) ok = start_scores(i + 1);
     }
-    ok = ok && mbar_wait(bd, i & 1, &abort_flag, &g_status, kDevTimeoutEpilogue);
+    ok = ok && wait_phase(bd, i & 1, &abort_flag, &g_status, kDevTimeoutEpilogue);
     if (tid == 0 && ok && loaded < steps) {
       load_step(loaded);
       ++loaded;

@@ -1,8 +1,8 @@
 // Cross-attention forward on the tensor cores.
 //
-// A block of 128 threads takes 128 queries of one head at a time and owns every
-// step of them: thread 0 starts the copies (TMA) and the products (tcgen05), all
-// threads do the softmax, one query (one tensor-memory lane) each.
+// A block takes 128 queries of one head at a time.  One warp starts the copies (TMA)
+// and the products (tcgen05); four do the softmax, one query (one tensor-memory lane)
+// a thread.  They wait for one another at mbarriers only.
 //
 //   S = Q K^T      both operands as TMA lands them (rows of 64 elements, swizzled)
 //   P = 2^(c S + bias - m)   read from and written back to tensor memory, in place
@@ -12,8 +12,8 @@
 //
 // The keys come in `nkt` tiles of `KT` (a multiple of 16, at most 128).  With one
 // tile (77 text tokens) K and V stay in shared memory while the block walks over
-// its share of the head's queries, and the next queries land while these are
-// worked on; with more, K and V run through two stages and O keeps its place, its
+// its share of the head's queries: the next queries land as soon as S has been formed,
+// and the next S is formed while finished rows leave; with more, K and V run through two stages and O keeps its place, its
 // scale renewed only when a row's maximum has risen by more than 2^kLazy.  Few
 // queries against many keys: the keys are split over blocks, which leave partial
 // rows in the workspace for a second kernel to join.
@@ -29,6 +29,7 @@ using namespace tc;
 namespace {
 
 constexpr int kRows = 128;
+constexpr int kThreads = kRows + 32;  // a thread for a row, and a warp that starts the work
 constexpr float kLazy = 4.f;
 
 struct FwdParams {
@@ -39,7 +40,7 @@ struct FwdParams {
   int qtiles, chunk; // query tiles of a head, tiles per block
   int nchunk;
   int splits, per;   // key splits, tiles per split
-  int qstages, kstages;
+  int kstages;           // of K and V
   uint32_t tmem_cols, o_col;
   uint32_t q_bytes, k_bytes;  // one stage of Q, of K (= of V)
   float* part_o;    // [splits][B][Nq][H][D]
@@ -49,22 +50,26 @@ struct FwdParams {
 __device__ int g_status;
 
 template <typename T, bool MASK>
-__global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUtensorMap mq,
-                                                    const __grid_constant__ CUtensorMap mk,
-                                                    const __grid_constant__ CUtensorMap mv,
-                                                    const __grid_constant__ CUtensorMap mo,
-                                                    const __grid_constant__ FwdParams p) {
-  constexpr bool kBf16 = sizeof(T) == 2 && !std::is_same<T, __half>::value;
+__global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant__ CUtensorMap mq,
+                                                       const __grid_constant__ CUtensorMap mk,
+                                                       const __grid_constant__ CUtensorMap mv,
+                                                       const __grid_constant__ CUtensorMap mo,
+                                                       const __grid_constant__ FwdParams p) {
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
   extern __shared__ unsigned char raw[];
-  __shared__ uint64_t bars[6];  // q[2], kv[2], s, o
+  // Landed: Q, K and V [2].  Formed: S, O.  Left by the rows' warps: the mask, P, rows.
+  __shared__ uint64_t bars[8];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ float bias[kRows];
-  const int tid = threadIdx.x, warp = tid >> 5;
+  __shared__ alignas(8) float bias[kRows];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(~0u, tid >> 5, 0);  // the same for the warp, and known to be
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t sq = base, sk = base + p.qstages * p.q_bytes, sv = sk + p.kstages * p.k_bytes;
-  const uint32_t bq = smem_u32(&bars[0]), bkv = smem_u32(&bars[2]), bs = smem_u32(&bars[4]),
-                 bo = smem_u32(&bars[5]);
+  // Q, the finished rows (over Q where a block has one query tile), K, V.
+  const uint32_t sq = base, so = p.chunk > 1 ? sq + p.q_bytes : sq;
+  const uint32_t sk = so + p.q_bytes, sv = sk + p.kstages * p.k_bytes;
+  const uint32_t bq = smem_u32(&bars[0]), bkv = bq + 8, bs = bq + 24, bo = bq + 32, bm = bq + 40,
+                 bp = bq + 48, br = bq + 56;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&tmem_slot)),
@@ -73,15 +78,14 @@ __global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUte
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (tid == 32) {
-    for (int i = 0; i < 6; ++i) mbar_init(smem_u32(&bars[i]), 1);
+    for (int i = 0; i < 8; ++i) mbar_init(bq + 8u * i, i < 5 ? 1 : kRows / 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     abort_flag = 0;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+  const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
   pdl_wait();
 
   unsigned id = blockIdx.x;
@@ -90,292 +94,328 @@ __global__ void __launch_bounds__(kRows) forward_tc(const __grid_constant__ CUte
   const int ch = id % p.nchunk;
   id /= p.nchunk;
   const int h = id % p.a.H, b = id / p.a.H;
-  const int t0 = ch * p.chunk, t1 = min(p.qtiles, t0 + p.chunk);
-  const int k0 = split * p.per, k1 = min(p.nkt, k0 + p.per);
-  const int nk = k1 - k0;
-
-  auto load_q = [&](int t, int stage) {
-    const uint32_t bar = bq + 8u * stage, dst = sq + stage * p.q_bytes;
-    mbar_expect_tx(bar, p.q_bytes);
-    for (int d = 0; d < p.DB; ++d)
-      tma_load_4d(dst + d * (kRows * 128), &mq, d * 64, t * kRows, h * p.qp.h, b * p.qp.b, bar);
-  };
-  auto load_kv = [&](int kt, int stage) {
-    const uint32_t bar = bkv + 8u * stage;
-    mbar_expect_tx(bar, 2 * p.k_bytes);
-    for (int d = 0; d < p.DB; ++d)
-      tma_load_4d(sk + stage * p.k_bytes + d * (p.KT * 128), &mk, d * 64, kt * p.KT, h * p.kp.h,
-                  b * p.kp.b, bar);
-    for (int d = 0; d < p.DB; ++d)
-      tma_load_4d(sv + stage * p.k_bytes + d * (p.KT * 128), &mv, d * 64, kt * p.KT, h * p.vp.h,
-                  b * p.vp.b, bar);
-  };
+  const int t0 = ch * p.chunk, tiles = min(p.qtiles, t0 + p.chunk) - t0;
+  const int k0 = split * p.per, nk = min(p.nkt, k0 + p.per) - k0;
   const bool resident = nk == 1;  // K and V stay
-  const int kv_total = resident ? 1 : nk * (t1 - t0);
-  int q_loaded = 0, kv_loaded = 0;  // thread 0's count of started copies
-  if (tid == 0) {
-    load_kv(k0, 0);
-    kv_loaded = 1;
-    load_q(t0, 0);
-    q_loaded = 1;
-    if (kv_total > 1 && p.kstages > 1) {
-      load_kv(k0 + 1 % nk, 1);
-      kv_loaded = 2;
-    }
-  }
+  const auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+    return wait_phase(bar, parity & 1, &abort_flag, &g_status, code);
+  };
 
-  const float c = p.a.scale * kLog2e;
-  const uint32_t idesc_s = instr_desc(kBf16, kRows, p.KT, false, false);
-  const uint32_t idesc_o = instr_desc(kBf16, kRows, p.DP, false, true);
-  const int chunks = p.KT / 16;
-  uint32_t steps = 0;  // products finished: the parity of bs and bo
-  bool ok = true;
-  int kv_seen = -1;    // stage contents that this thread has waited for
-
-  for (int t = t0; t < t1 && ok; ++t) {
-    const int qi = t - t0, qstage = qi % p.qstages;
-    const uint32_t q_at = sq + qstage * p.q_bytes;
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < nk && ok; ++j, ++steps) {
-      const int kt = k0 + j;
-      const int ki = resident ? 0 : qi * nk + j, kstage = ki % p.kstages;
-      const int keys = min(p.KT, p.a.Nk - kt * p.KT);
-      const uint32_t k_at = sk + kstage * p.k_bytes, v_at = sv + kstage * p.k_bytes;
-      if (MASK && kv_seen != ki) {
-        // The bias of this tile's keys; the rows of V behind a masked key are cleared:
-        // P is zero there, and zero times infinity is not.
-        if (tid < p.KT) {
-          float x = -INFINITY;
-          const bool in = tid < keys && key_bias(p.a, b, kt * p.KT + tid, &x);
-          bias[tid] = in ? x : -INFINITY;
-          ok = mbar_wait(bkv + 8u * kstage, (ki / p.kstages) & 1, &abort_flag, &g_status,
-                         kDevTimeoutProducer);
-          if (ok && !in && tid < keys) {
-            for (int d = 0; d < p.DB; ++d)
-              for (int i = 0; i < 8; ++i)
-                st_shared_v4(v_at + d * (p.KT * 128) + sw128(tid, i), 0, 0, 0, 0);
-            fence_async_smem();
-          }
-        }
-        kv_seen = ki;
-        if (!__syncthreads_and(ok)) {
-          ok = false;
-          break;
-        }
-      }
-      if (tid == 0) {
-        ok = mbar_wait(bq + 8u * qstage, (qi / p.qstages) & 1, &abort_flag, &g_status,
-                       kDevTimeoutProducer) &&
-             mbar_wait(bkv + 8u * kstage, (ki / p.kstages) & 1, &abort_flag, &g_status,
-                       kDevTimeoutProducer);
-        if (ok) {
-          tc_fence_after();
-          const uint64_t ad = smem_desc_sw128(q_at), bd = smem_desc_sw128(k_at);
-          for (int s = 0; s < p.DP / 16; ++s)
-            umma_f16(tmem, ad + (uint32_t)((s >> 2) * (kRows * 8) + (s & 3) * 2),
-                     bd + (uint32_t)((s >> 2) * (p.KT * 8) + (s & 3) * 2), idesc_s, s != 0);
-          umma_commit(bs);
-          if (j == 0 && t + 1 < t1 && p.qstages > 1) {
-            // The stage's last rows have left for global memory before it is filled.
-            bulk_wait_read_all();
-            load_q(t + 1, (qi + 1) % p.qstages);
-            ++q_loaded;
-          }
-        }
-      }
-      ok = ok && mbar_wait(bs, steps & 1, &abort_flag, &g_status, kDevTimeoutMma);
-      if (!__syncthreads_and(ok)) {
-        ok = false;
-        break;
-      }
+  if (warp == kRows / 32) {
+    // ---- The warp that starts copies and products ----
+    const bool one = elect_one();
+    const auto load_q = [&](int t) {
+      if (!one) return;
+      mbar_expect_tx(bq, p.q_bytes);
+      for (int d = 0; d < p.DB; ++d)
+        tma_load_4d(sq + d * (kRows * 128), &mq, d * 64, (t0 + t) * kRows, h * p.qp.h, b * p.qp.b,
+                    bq);
+    };
+    const auto load_kv = [&](int j) {
+      if (!one) return;
+      const int stage = j % p.kstages;
+      const uint32_t bar = bkv + 8u * stage, at = stage * p.k_bytes;
+      mbar_expect_tx(bar, 2 * p.k_bytes);
+      for (int d = 0; d < p.DB; ++d)
+        tma_load_4d(sk + at + d * (p.KT * 128), &mk, d * 64, (k0 + j) * p.KT, h * p.kp.h,
+                    b * p.kp.b, bar);
+      for (int d = 0; d < p.DB; ++d)
+        tma_load_4d(sv + at + d * (p.KT * 128), &mv, d * 64, (k0 + j) * p.KT, h * p.vp.h,
+                    b * p.vp.b, bar);
+    };
+    const uint32_t idesc_s = instr_desc(kBf16, kRows, p.KT, false, false);
+    const uint32_t idesc_o = instr_desc(kBf16, kRows, p.DP, false, true);
+    const int nd = p.DP / 16, nc = p.KT / 16;
+    const uint64_t qd = smem_desc_sw128(sq);
+    // S of the tile in Q and key tile j.
+    const auto scores = [&](int j) {
+      const uint64_t kd = smem_desc_sw128(sk + (j % p.kstages) * p.k_bytes);
       tc_fence_after();
-
-      // The row's maximum.
-      uint32_t r[2][16];
-      float top = -INFINITY;
-      tmem_ld16_issue(lanes, r[0]);
-#pragma unroll 1
-      for (int i = 0; i < chunks; i += 2) {
+      if (one) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (i + u < chunks) {
-            tmem_wait_ld();
-            if (i + u + 1 < chunks) tmem_ld16_issue(lanes + 16u * (i + u + 1), r[u ^ 1]);
-            const int col = 16 * (i + u);
-            if (MASK) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float add = bias[col + e];
-                const float x = fmaf(__uint_as_float(r[u][e]), c, add);
-                top = fmaxf(top, add == -INFINITY ? -INFINITY : x);
-              }
-            } else if (col + 16 <= keys) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e) top = fmaxf(top, __uint_as_float(r[u][e]) * c);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (col + e < keys) top = fmaxf(top, __uint_as_float(r[u][e]) * c);
-            }
-          }
-        }
+        for (int s = 0; s < kMaxD / 16; ++s)
+          if (s < nd) umma_f16(tmem, qd + (uint32_t)((s >> 2) * (kRows * 8) + (s & 3) * 2),
+                   kd + (uint32_t)((s >> 2) * (p.KT * 8) + (s & 3) * 2), idesc_s, s != 0);
+        umma_commit(bs);
       }
-      // The scale that the row's sums are kept at.
-      float factor = 1.f;
-      if (j == 0) {
-        m = top;
-      } else if (top > m + kLazy || m == -INFINITY) {
-        const float up = fmaxf(top, m);
-        factor = m == -INFINITY ? 1.f : ex2(m - up);  // nothing yet: zeros stay zeros
-        m = up;
-      }
-      if (j > 0 && __any_sync(~0u, factor != 1.f)) {
-        l *= factor;
-        for (int i = 0; i < p.DP / 16; ++i) {
-          uint32_t o[16];
-          tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
-          tmem_wait_ld();
+    };
+    const auto products = [&](int j) {
+      const uint64_t vd = smem_desc_mn(sv + (j % p.kstages) * p.k_bytes, p.KT * 128);
+      tc_fence_after();
+      if (one) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-          tmem_st16(lanes + p.o_col + 16u * i, o);
-        }
-      }
-      const float sub = m == -INFINITY ? 0.f : m;
-
-      // P, packed over the scores that have been read.
-      tmem_ld16_issue(lanes, r[0]);
-#pragma unroll 1
-      for (int i = 0; i < chunks; i += 2) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (i + u < chunks) {
-            tmem_wait_ld();
-            if (i + u + 1 < chunks) tmem_ld16_issue(lanes + 16u * (i + u + 1), r[u ^ 1]);
-            const int col = 16 * (i + u);
-            uint32_t o[8];
-            float e0[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float s = __uint_as_float(r[u][e]);
-              if (MASK) {
-                const float add = bias[col + e];
-                e0[e] = add == -INFINITY ? 0.f : ex2(fmaf(s, c, add) - sub);
-              } else {
-                e0[e] = ex2(__fmul_rn(s, c) - sub);
-              }
-            }
-            if (!MASK && col + 16 > keys) {
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (col + e >= keys) e0[e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              l += e0[2 * e] + e0[2 * e + 1];
-              o[e] = pack2<T>(e0[2 * e], e0[2 * e + 1]);
-            }
-            tmem_st8(lanes + 8u * (i + u), o);
-          }
-        }
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
-        tc_fence_after();
-        const uint64_t bd = smem_desc_mn(v_at, p.KT * 128);
-        for (int s = 0; s < chunks; ++s)
-          umma_f16_ta(tmem + p.o_col, tmem + 8u * s, bd + 128ull * s, idesc_o, s != 0 || j != 0);
+        for (int s = 0; s < 8; ++s)
+          if (s < nc)
+            umma_f16_ta(tmem + p.o_col, tmem + 8u * s, vd + 128ull * s, idesc_o, s != 0 || j != 0);
         umma_commit(bo);
       }
-      ok = mbar_wait(bo, steps & 1, &abort_flag, &g_status, kDevTimeoutEpilogue);
-      if (tid == 0 && ok && !resident && kv_loaded < kv_total) {
-        load_kv(k0 + kv_loaded % nk, kv_loaded % p.kstages);
-        ++kv_loaded;
-      }
-      if (!__syncthreads_and(ok)) {
-        ok = false;
-        ++steps;
-        break;
-      }
-      tc_fence_after();
-    }
-    if (!ok) break;
-
-    // O / sum.
-    const int row = t * kRows + tid;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float lse = l == 0.f ? -INFINITY : m + log2f(l);
-    const long long lrow = ((long long)b * p.a.H + h) * p.a.Nq + row;
-    if (p.splits > 1) {
-      float* po = p.part_o + ((((long long)split * p.a.B + b) * p.a.Nq + row) * p.a.H + h) * p.a.D;
-      for (int i = 0; i < p.DP / 16; ++i) {
-        uint32_t o[16];
-        __syncwarp();
-        tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
-        tmem_wait_ld();
-        if (row < p.a.Nq) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4)
-            if (16 * i + e < p.a.D)
-              *reinterpret_cast<float4*>(po + 16 * i + e) =
-                  make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                              __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+    };
+    int qn = 1, kn = min(nk, p.kstages);  // copies started
+    load_q(0);
+    for (int j = 0; j < kn; ++j) load_kv(j);
+    bool ok = wait(bq, 0, kDevTimeoutProducer) && wait(bkv, 0, kDevTimeoutProducer);
+    ok = __all_sync(~0u, ok);
+    if (ok) scores(0);
+    int step = 0;
+    for (int t = 0; t < tiles && ok; ++t) {
+      for (int j = 0; j < nk && ok; ++j, ++step) {
+        if (j == nk - 1 && t + 1 < tiles) {
+          // Nothing reads Q any more once the last scores are there.
+          ok = wait(bs, step, kDevTimeoutMma);
+          if (ok) load_q(t + 1);
+          ++qn;
+        }
+        ok = ok && wait(bp, step, kDevTimeoutMma);
+        // The rows of the last tile have left their place before new ones are written
+        // there, which happens behind this product.
+        if (one) bulk_wait_read_all();
+        if (!(ok = __all_sync(~0u, ok))) break;
+        products(j);
+        if (j + 1 < nk) {
+          // Behind the product that reads P, in the same order.
+          ok = __all_sync(~0u, wait(bkv + 8u * ((j + 1) % p.kstages), (j + 1) / p.kstages,
+                                    kDevTimeoutProducer));
+          if (!ok) break;
+          scores(j + 1);
+          if (kn < nk) {
+            ok = __all_sync(~0u, wait(bo, step, kDevTimeoutMma));
+            if (!ok) break;
+            load_kv(kn++);
+          }
         }
       }
-      if (row < p.a.Nq)
-        p.part_lse[(long long)split * p.a.B * p.a.H * p.a.Nq + lrow] = lse;
-      tc_fence_before();
-      __syncthreads();
-    } else {
-      for (int i = 0; i < p.DP / 16; ++i) {
-        uint32_t o[16];
-        tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
-        tmem_wait_ld();
-        float f[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
-        const uint32_t at = q_at + (uint32_t)(i >> 2) * (kRows * 128);
-        const int piece = (i & 3) * 2;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          st_shared_v4(at + sw128(tid, piece + u), pack2<T>(f[8 * u], f[8 * u + 1]),
-                       pack2<T>(f[8 * u + 2], f[8 * u + 3]), pack2<T>(f[8 * u + 4], f[8 * u + 5]),
-                       pack2<T>(f[8 * u + 6], f[8 * u + 7]));
+      ok = ok && wait(br, t, kDevTimeoutEpilogue);
+      if (!(ok = __all_sync(~0u, ok))) break;
+      if (t + 1 < tiles) {
+        ok = __all_sync(~0u, wait(bq, t + 1, kDevTimeoutProducer));
+        if (!ok) break;
+        scores(0);
       }
-      if (p.a.lse && row < p.a.Nq) p.a.lse[lrow] = lse;
-      fence_async_smem();
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
+      if (one && p.splits == 1) {
         for (int d = 0; d < p.DB; ++d)
-          tma_store_4d(&mo, q_at + d * (kRows * 128), d * 64, t * kRows, h, b);
+          tma_store_4d(&mo, so + d * (kRows * 128), d * 64, (t0 + t) * kRows, h, b);
         bulk_commit();
       }
     }
-    if (tid == 0) {
-      tc_fence_after();
-      if (t + 1 < t1 && p.qstages == 1) {
-        bulk_wait_read_all();
-        load_q(t + 1, 0);
-        ++q_loaded;
+    if (one) {
+      if (!ok) {
+        // Let the copies and products that were started end before their memory goes.
+        mbar_wait_drain(bq, (qn - 1) & 1);
+        for (int i = 0; i < p.kstages && kn - 1 - i >= 0; ++i)
+          mbar_wait_drain(bkv + 8u * ((kn - 1 - i) % p.kstages), ((kn - 1 - i) / p.kstages) & 1);
+        const uint64_t since = globaltimer();
+        while (globaltimer() - since < kDrainLimitNs) {
+        }
       }
+      bulk_wait_all();
     }
-  }
+  } else {
+    // ---- The rows' warps: one query a thread ----
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const float c = p.a.scale * kLog2e;
+    const int pieces = (p.KT + 31) / 32;
+    int step = 0;
+    bool ok = true;
+    for (int t = 0; t < tiles && ok; ++t) {
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nk; ++j, ++step) {
+        const int key0 = (k0 + j) * p.KT, keys = min(p.KT, p.a.Nk - key0);
+        if (MASK && (t == 0 || !resident)) {
+          // The bias of this tile's keys; the rows of V behind a masked key are cleared:
+          // P is zero there, and zero times infinity is not.
+          float x = -INFINITY;
+          const bool in = tid < keys && key_bias(p.a, b, key0 + tid, &x);
+          // The scores before have been read by everyone who reads the old bias.
+          if (j > 0) ok = wait(bo, step - 1, kDevTimeoutMma);
+          bias[tid] = in ? x : -INFINITY;  // past the tile too: scores are read in 32s
+          const int stage = j % p.kstages;
+          ok = ok && wait(bkv + 8u * stage, j / p.kstages, kDevTimeoutProducer);
+          if (ok && !in && tid < keys) {
+            for (int d = 0; d < p.DB; ++d)
+              for (int i = 0; i < 8; ++i)
+                st_shared_v4(sv + stage * p.k_bytes + d * (p.KT * 128) + sw128(tid, i), 0, 0, 0, 0);
+            fence_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bm);
+          ok = ok && wait(bm, step, kDevTimeoutEpilogue);
+        }
+        ok = ok && wait(bs, step, kDevTimeoutMma);
+        __syncwarp();
+        if (!__all_sync(~0u, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
 
-  if (tid == 0) {
-    if (!ok) {
-      // Let the copies and products that were started end before their memory goes.
-      const int q = q_loaded - 1, kv = kv_loaded - 1;
-      for (int i = 0; i < p.qstages && q - i >= 0; ++i)
-        mbar_wait_drain(bq + 8u * ((q - i) % p.qstages), ((q - i) / p.qstages) & 1);
-      for (int i = 0; i < p.kstages && kv - i >= 0; ++i)
-        mbar_wait_drain(bkv + 8u * ((kv - i) % p.kstages), ((kv - i) / p.kstages) & 1);
-      const uint64_t since = globaltimer();
-      while (globaltimer() - since < kDrainLimitNs) {
+        // The row's scores, 32 at a time with the next 32 on their way, twice: the
+        // maximum, then P.
+        uint32_t r[2][32];
+        float top = -INFINITY;
+        // Scores e and e + 1 of a piece, in base 2; minus infinity where the key is out.
+        const auto score2 = [&](const uint32_t(&x)[32], int col, int e) {
+          float2 v = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+          if (MASK) {
+            const float2 add = *reinterpret_cast<const float2*>(&bias[col + e]);
+            v = __ffma2_rn(v, make_float2(c, c), add);
+            if (add.x == -INFINITY) v.x = -INFINITY;
+            if (add.y == -INFINITY) v.y = -INFINITY;
+          } else {
+            v = __fmul2_rn(v, make_float2(c, c));
+          }
+          return v;
+        };
+        const auto take_top = [&](const uint32_t(&x)[32], int col) {
+          if (MASK || col + 32 <= keys) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = score2(x, col, e);
+              top = fmaxf(top, fmaxf(v.x, v.y));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const float2 v = score2(x, col, e);
+              if (col + e < keys) top = fmaxf(top, v.x);
+              if (col + e + 1 < keys) top = fmaxf(top, v.y);
+            }
+          }
+        };
+        tmem_ld32_issue(lanes, r[0]);
+#pragma unroll 1
+        for (int i = 0; i < pieces; i += 2) {
+          tmem_wait_ld();
+          if (i + 1 < pieces) tmem_ld32_issue(lanes + 32u * (i + 1), r[1]);
+          take_top(r[0], 32 * i);
+          if (i + 1 < pieces) {
+            tmem_wait_ld();
+            if (i + 2 < pieces) tmem_ld32_issue(lanes + 32u * (i + 2), r[0]);
+            take_top(r[1], 32 * (i + 1));
+          }
+        }
+        // The scale that the row's sums are kept at.
+        float factor = 1.f;
+        if (j == 0) {
+          m = top;
+        } else if (top > m + kLazy || m == -INFINITY) {
+          const float to = fmaxf(top, m);
+          factor = m == -INFINITY ? 1.f : ex2(m - to);  // nothing yet: zeros stay zeros
+          m = to;
+        }
+        if (j > 0) {
+          ok = wait(bo, step - 1, kDevTimeoutMma);
+          __syncwarp();
+          tc_fence_after();
+          if (__any_sync(~0u, factor != 1.f)) {
+            l *= factor;
+#pragma unroll 1
+            for (int i = 0; i < p.DP / 16; ++i) {
+              uint32_t o[16];
+              tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+              tmem_st16(lanes + p.o_col + 16u * i, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : m;
+
+        // P, packed over the scores that have been read.
+        const auto put_p = [&](const uint32_t(&x)[32], int col) {
+          const bool whole = MASK || col + 32 <= keys;
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            if (col + 16 * half < p.KT) {
+              uint32_t o[8];
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int at = 16 * half + 2 * e;
+                float2 v = __fadd2_rn(score2(x, col, at), make_float2(-sub, -sub));
+                v = make_float2(ex2(v.x), ex2(v.y));
+                if (!whole) {
+                  if (col + at >= keys) v.x = 0.f;
+                  if (col + at + 1 >= keys) v.y = 0.f;
+                }
+                sum = __fadd2_rn(sum, v);
+                o[e] = pack2<T>(v.x, v.y);
+              }
+              l += sum.x + sum.y;
+              tmem_st8(lanes + (uint32_t)(col / 2 + 8 * half), o);
+            }
+        };
+        tmem_ld32_issue(lanes, r[0]);
+#pragma unroll 1
+        for (int i = 0; i < pieces; i += 2) {
+          tmem_wait_ld();
+          if (i + 1 < pieces) tmem_ld32_issue(lanes + 32u * (i + 1), r[1]);
+          put_p(r[0], 32 * i);
+          if (i + 1 < pieces) {
+            tmem_wait_ld();
+            if (i + 2 < pieces) tmem_ld32_issue(lanes + 32u * (i + 2), r[0]);
+            put_p(r[1], 32 * (i + 1));
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bp);
       }
+      ok = ok && wait(bo, step - 1, kDevTimeoutEpilogue);
+      __syncwarp();
+      if (!(ok = __all_sync(~0u, ok))) break;
+      tc_fence_after();
+
+      // O / sum.
+      const int row = (t0 + t) * kRows + tid;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float lse = l == 0.f ? -INFINITY : m + log2f(l);
+      const long long lrow = ((long long)b * p.a.H + h) * p.a.Nq + row;
+      if (p.splits > 1) {
+        float* po = p.part_o + ((((long long)split * p.a.B + b) * p.a.Nq + row) * p.a.H + h) * p.a.D;
+#pragma unroll 1
+        for (int i = 0; i < p.DP / 16; ++i) {
+          uint32_t o[16];
+          __syncwarp();
+          tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
+          tmem_wait_ld();
+          if (row < p.a.Nq) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              if (16 * i + e < p.a.D)
+                *reinterpret_cast<float4*>(po + 16 * i + e) =
+                    make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+          }
+        }
+        if (row < p.a.Nq) p.part_lse[(long long)split * p.a.B * p.a.H * p.a.Nq + lrow] = lse;
+      } else {
+        const auto put_rows = [&](const uint32_t(&o)[16], int i) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          const uint32_t at = so + (uint32_t)(i >> 2) * (kRows * 128);
+          st_shared_v4(at + sw128(tid, (i & 3) * 2), w[0], w[1], w[2], w[3]);
+          st_shared_v4(at + sw128(tid, (i & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
+        };
+#pragma unroll 1
+        for (int i = 0; i < p.DP / 16; i += 2) {
+          uint32_t o[2][16];
+          tmem_ld16_issue(lanes + p.o_col + 16u * i, o[0]);
+          if (i + 1 < p.DP / 16) tmem_ld16_issue(lanes + p.o_col + 16u * (i + 1), o[1]);
+          tmem_wait_ld();
+          put_rows(o[0], i);
+          if (i + 1 < p.DP / 16) put_rows(o[1], i + 1);
+        }
+        if (p.a.lse && row < p.a.Nq) p.a.lse[lrow] = lse;
+        fence_async_smem();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(br);
     }
-    bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -702,26 +742,25 @@ void plan(FwdParams* p, int sms) {
   const bool one = p->per == 1;
   // With one tile O takes the columns that P leaves of S.
   p->o_col = (uint32_t)(one ? up(p->KT / 2, 16) : p->KT);
-  const int cols = p->KT > (int)p->o_col + p->DP ? p->KT : (int)p->o_col + p->DP;
+  // Scores are read 32 columns at a time.
+  const int cols = up(p->KT, 32) > (int)p->o_col + p->DP ? up(p->KT, 32) : (int)p->o_col + p->DP;
   p->tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
   p->kstages = one ? 1 : 2;
   // Blocks of the GPU at a time decide how many query tiles a block walks over.
-  p->qstages = one ? 2 : 1;
-  const size_t smem = (size_t)p->qstages * p->q_bytes + 2ull * p->kstages * p->k_bytes + 1024;
+  const size_t smem = (one ? 2ull : 1ull) * p->q_bytes + 2ull * p->kstages * p->k_bytes + 1024;
   long long per_sm = (long long)(kSmemMax / smem);
   if (per_sm > 512 / p->tmem_cols) per_sm = 512 / p->tmem_cols;
   if (per_sm < 1) per_sm = 1;
-  if (per_sm > 8) per_sm = 8;
+  if (per_sm > 3) per_sm = 3;  // by its registers
   long long nchunk = one ? (per_sm * sms) / (heads * p->splits) : p->qtiles;
   if (nchunk < 1) nchunk = 1;
   if (nchunk > p->qtiles) nchunk = p->qtiles;
   p->chunk = (int)((p->qtiles + nchunk - 1) / nchunk);
   p->nchunk = (p->qtiles + p->chunk - 1) / p->chunk;
-  if (p->chunk == 1) p->qstages = 1;
 }
 
 size_t smem_bytes(const FwdParams& p) {
-  size_t n = (size_t)p.qstages * p.q_bytes + 2ull * p.kstages * p.k_bytes + 1024;
+  size_t n = (p.chunk > 1 ? 2ull : 1ull) * p.q_bytes + 2ull * p.kstages * p.k_bytes + 1024;
   // No more blocks on an SM than its tensor memory holds.
   const size_t least = kSmemMax / (512 / p.tmem_cols + 1) + 1;
   return n > least ? n : least;
@@ -736,7 +775,7 @@ cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)((long long)p.a.B * p.a.H * p.nchunk * p.splits);
-  e = launch_pdl(kPdlInput, forward_tc<T, MASK>, dim3(grid), dim3(kRows), smem, s, m[0], m[1],
+  e = launch_pdl(kPdlInput, forward_tc<T, MASK>, dim3(grid), dim3(kThreads), smem, s, m[0], m[1],
                  m[2], m[3], p);
   if (e == cudaSuccess && p.splits > 1) {
     const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
