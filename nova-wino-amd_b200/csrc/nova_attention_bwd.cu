@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ float bias[2][kRows];
   __shared__ float red[2][kRows];
   __shared__ uint32_t peak[kThreads / 32];
-  const int tid = threadIdx.x, warp = tid >> 5, half = tid >> 7, r = tid & (kRows - 1);
+  const int tid = threadIdx.x, half = tid >> 7, r = tid & (kRows - 1);
+  const int warp = __shfl_sync(~0u, tid >> 5, 0);
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   // Fixed pair, walked pairs, P, dS.
   const uint32_t fixed_bytes = kWalkQ ? p.k_bytes : p.q_bytes;
@@ -94,8 +95,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
   const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  pdl_trigger();
   pdl_wait();
 
   unsigned id = blockIdx.x;
@@ -499,6 +501,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // delta = dO . O: a warp for a query.
 template <typename T>
 __global__ void __launch_bounds__(128) row_delta(const __grid_constant__ Args a, float* delta) {
+  pdl_trigger();
   pdl_wait();
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= (long long)a.B * a.H * a.Nq) return;
@@ -523,6 +526,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) join_parts(const float* __restrict__ dk,
                                                   const float* __restrict__ dv, T* to_k, T* to_v,
                                                   long long n, int splits) {
+  pdl_trigger();
   pdl_wait();
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;

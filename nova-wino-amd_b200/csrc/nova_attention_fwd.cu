@@ -31,6 +31,7 @@ namespace {
 constexpr int kRows = 128;
 constexpr int kThreads = kRows + 32;  // a thread for a row, and a warp that starts the work
 constexpr float kLazy = 4.f;
+constexpr int kHeld = 80;  // scores that a thread can hold with three blocks on an SM
 
 struct FwdParams {
   Args a;
@@ -49,7 +50,7 @@ struct FwdParams {
 
 __device__ int g_status;
 
-template <typename T, bool MASK>
+template <typename T, bool MASK, bool ONE>
 __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant__ CUtensorMap mq,
                                                        const __grid_constant__ CUtensorMap mk,
                                                        const __grid_constant__ CUtensorMap mv,
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
+  pdl_trigger();
   pdl_wait();
 
   unsigned id = blockIdx.x;
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
     // ---- The rows' warps: one query a thread ----
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const float c = p.a.scale * kLog2e;
-    const int pieces = (p.KT + 31) / 32;
+    const int chunks = p.KT / 16;
     int step = 0;
     bool ok = true;
     for (int t = 0; t < tiles && ok; ++t) {
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
           const bool in = tid < keys && key_bias(p.a, b, key0 + tid, &x);
           // The scores before have been read by everyone who reads the old bias.
           if (j > 0) ok = wait(bo, step - 1, kDevTimeoutMma);
-          bias[tid] = in ? x : -INFINITY;  // past the tile too: scores are read in 32s
+          bias[tid] = in ? x : -INFINITY;
           const int stage = j % p.kstages;
           ok = ok && wait(bkv + 8u * stage, j / p.kstages, kDevTimeoutProducer);
           if (ok && !in && tid < keys) {
@@ -248,12 +250,12 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
         }
         tc_fence_after();
 
-        // The row's scores, 32 at a time with the next 32 on their way, twice: the
-        // maximum, then P.
-        uint32_t r[2][32];
+        // The row's scores twice: the maximum, then P.
+        // Tiles of up to kHeld keys stay in registers from one to the other.
+        uint32_t r[ONE ? kHeld / 16 : 4][16];
         float top = -INFINITY;
         // Scores e and e + 1 of a piece, in base 2; minus infinity where the key is out.
-        const auto score2 = [&](const uint32_t(&x)[32], int col, int e) {
+        const auto score2 = [&](const uint32_t(&x)[16], int col, int e) {
           float2 v = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1]));
           if (MASK) {
             const float2 add = *reinterpret_cast<const float2*>(&bias[col + e]);
@@ -265,33 +267,52 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
           }
           return v;
         };
-        const auto take_top = [&](const uint32_t(&x)[32], int col) {
-          if (MASK || col + 32 <= keys) {
+        const auto take_top = [&](const uint32_t(&x)[16], int col) {
+          if (MASK || col + 16 <= keys) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
+            for (int e = 0; e < 16; e += 2) {
               const float2 v = score2(x, col, e);
               top = fmaxf(top, fmaxf(v.x, v.y));
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
+            for (int e = 0; e < 16; e += 2) {
               const float2 v = score2(x, col, e);
               if (col + e < keys) top = fmaxf(top, v.x);
               if (col + e + 1 < keys) top = fmaxf(top, v.y);
             }
           }
         };
-        tmem_ld32_issue(lanes, r[0]);
+        // Chunks of 16 two by two, the next two on their way; `use` once for each.
+        const auto each_chunk = [&](auto&& use) {
+          tmem_ld16_issue(lanes, r[0]);
+          if (1 < chunks) tmem_ld16_issue(lanes + 16u, r[1]);
 #pragma unroll 1
-        for (int i = 0; i < pieces; i += 2) {
-          tmem_wait_ld();
-          if (i + 1 < pieces) tmem_ld32_issue(lanes + 32u * (i + 1), r[1]);
-          take_top(r[0], 32 * i);
-          if (i + 1 < pieces) {
+          for (int i = 0; i < chunks; i += 4) {
             tmem_wait_ld();
-            if (i + 2 < pieces) tmem_ld32_issue(lanes + 32u * (i + 2), r[0]);
-            take_top(r[1], 32 * (i + 1));
+            if (i + 2 < chunks) tmem_ld16_issue(lanes + 16u * (i + 2), r[2]);
+            if (i + 3 < chunks) tmem_ld16_issue(lanes + 16u * (i + 3), r[3]);
+            use(r[0], 16 * i);
+            if (i + 1 < chunks) use(r[1], 16 * (i + 1));
+            if (i + 2 < chunks) {
+              tmem_wait_ld();
+              if (i + 4 < chunks) tmem_ld16_issue(lanes + 16u * (i + 4), r[0]);
+              if (i + 5 < chunks) tmem_ld16_issue(lanes + 16u * (i + 5), r[1]);
+              use(r[2], 16 * (i + 2));
+              if (i + 3 < chunks) use(r[3], 16 * (i + 3));
+            }
           }
+        };
+        if constexpr (ONE) {
+#pragma unroll
+          for (int i = 0; i < kHeld / 16; ++i)
+            if (i < chunks) tmem_ld16_issue(lanes + 16u * i, r[i]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < kHeld / 16; ++i)
+            if (i < chunks) take_top(r[i], 16 * i);
+        } else {
+          each_chunk(take_top);
         }
         // The scale that the row's sums are kept at.
         float factor = 1.f;
@@ -322,40 +343,30 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
         const float sub = m == -INFINITY ? 0.f : m;
 
         // P, packed over the scores that have been read.
-        const auto put_p = [&](const uint32_t(&x)[32], int col) {
-          const bool whole = MASK || col + 32 <= keys;
+        const auto put_p = [&](const uint32_t(&x)[16], int col) {
+          const bool whole = MASK || col + 16 <= keys;
+          uint32_t o[8];
+          float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            if (col + 16 * half < p.KT) {
-              uint32_t o[8];
-              float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int at = 16 * half + 2 * e;
-                float2 v = __fadd2_rn(score2(x, col, at), make_float2(-sub, -sub));
-                v = make_float2(ex2(v.x), ex2(v.y));
-                if (!whole) {
-                  if (col + at >= keys) v.x = 0.f;
-                  if (col + at + 1 >= keys) v.y = 0.f;
-                }
-                sum = __fadd2_rn(sum, v);
-                o[e] = pack2<T>(v.x, v.y);
-              }
-              l += sum.x + sum.y;
-              tmem_st8(lanes + (uint32_t)(col / 2 + 8 * half), o);
+          for (int e = 0; e < 8; ++e) {
+            float2 v = __fadd2_rn(score2(x, col, 2 * e), make_float2(-sub, -sub));
+            v = make_float2(ex2(v.x), ex2(v.y));
+            if (!whole) {
+              if (col + 2 * e >= keys) v.x = 0.f;
+              if (col + 2 * e + 1 >= keys) v.y = 0.f;
             }
-        };
-        tmem_ld32_issue(lanes, r[0]);
-#pragma unroll 1
-        for (int i = 0; i < pieces; i += 2) {
-          tmem_wait_ld();
-          if (i + 1 < pieces) tmem_ld32_issue(lanes + 32u * (i + 1), r[1]);
-          put_p(r[0], 32 * i);
-          if (i + 1 < pieces) {
-            tmem_wait_ld();
-            if (i + 2 < pieces) tmem_ld32_issue(lanes + 32u * (i + 2), r[0]);
-            put_p(r[1], 32 * (i + 1));
+            sum = __fadd2_rn(sum, v);
+            o[e] = pack2<T>(v.x, v.y);
           }
+          l += sum.x + sum.y;
+          tmem_st8(lanes + (uint32_t)(col / 2), o);
+        };
+        if constexpr (ONE) {
+#pragma unroll
+          for (int i = 0; i < kHeld / 16; ++i)
+            if (i < chunks) put_p(r[i], 16 * i);
+        } else {
+          each_chunk(put_p);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -442,6 +453,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
   constexpr int G = 32 / LPK, U = kTokenUnroll;
   __shared__ float po[kTokenWarps][NQ][LPK * 8];
   __shared__ float pm[kTokenWarps][NQ], pl[kTokenWarps][NQ];
+  pdl_trigger();
   pdl_wait();
   const Args& a = p.a;
   unsigned id = blockIdx.x;
@@ -594,6 +606,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
 // Joins the splits' rows: a warp for a row.
 template <typename T>
 __global__ void __launch_bounds__(128) join_splits(const __grid_constant__ FwdParams p) {
+  pdl_trigger();
   pdl_wait();
   const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
   const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -742,8 +755,7 @@ void plan(FwdParams* p, int sms) {
   const bool one = p->per == 1;
   // With one tile O takes the columns that P leaves of S.
   p->o_col = (uint32_t)(one ? up(p->KT / 2, 16) : p->KT);
-  // Scores are read 32 columns at a time.
-  const int cols = up(p->KT, 32) > (int)p->o_col + p->DP ? up(p->KT, 32) : (int)p->o_col + p->DP;
+  const int cols = p->KT > (int)p->o_col + p->DP ? p->KT : (int)p->o_col + p->DP;
   p->tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
   p->kstages = one ? 1 : 2;
   // Blocks of the GPU at a time decide how many query tiles a block walks over.
@@ -768,14 +780,14 @@ size_t smem_bytes(const FwdParams& p) {
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-template <typename T, bool MASK>
+template <typename T, bool MASK, bool ONE>
 cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
   const size_t smem = smem_bytes(p);
-  cudaError_t e = cudaFuncSetAttribute(forward_tc<T, MASK>,
+  cudaError_t e = cudaFuncSetAttribute(forward_tc<T, MASK, ONE>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   const unsigned grid = (unsigned)((long long)p.a.B * p.a.H * p.nchunk * p.splits);
-  e = launch_pdl(kPdlInput, forward_tc<T, MASK>, dim3(grid), dim3(kThreads), smem, s, m[0], m[1],
+  e = launch_pdl(kPdlInput, forward_tc<T, MASK, ONE>, dim3(grid), dim3(kThreads), smem, s, m[0], m[1],
                  m[2], m[3], p);
   if (e == cudaSuccess && p.splits > 1) {
     const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
@@ -817,9 +829,12 @@ cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, c
     *why = "tensor map encode failed";
     return cudaErrorInvalidValue;
   }
-  const bool mask = a.mask_kind != kMaskNone;
-  if (bf16) return mask ? run<__nv_bfloat16, true>(p, m, s) : run<__nv_bfloat16, false>(p, m, s);
-  return mask ? run<__half, true>(p, m, s) : run<__half, false>(p, m, s);
+  const bool mask = a.mask_kind != kMaskNone, one = p.KT <= kHeld;
+#define NOVA_XATTN_RUN(T)                                                    \
+  (mask ? (one ? run<T, true, true>(p, m, s) : run<T, true, false>(p, m, s)) \
+        : (one ? run<T, false, true>(p, m, s) : run<T, false, false>(p, m, s)))
+  return bf16 ? NOVA_XATTN_RUN(__nv_bfloat16) : NOVA_XATTN_RUN(__half);
+#undef NOVA_XATTN_RUN
 }
 
 }  // namespace xattn

@@ -52,9 +52,11 @@ struct Walk {
   int tx, ty;  // threads
   int chunk;   // pixels per block
   int nchunk;
+  int cell;    // channels that share a part of the statistics: a group's, or one
 };
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 4;  // pixels that a streaming thread has on their way
 
 // Channels are worked on in pairs (the paired 32-bit instructions halve the count),
 // or singly where a thread holds one.
@@ -166,6 +168,7 @@ __device__ __forceinline__ Place place(const Args& a, const Walk& k) {
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2* part) {
   __shared__ float2 red[kThreads * V];
+  pdl_trigger();
   pdl_wait();
   const Place q = place(a, k);
   using L = Lanes<T, V>;
@@ -199,107 +202,113 @@ __global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2
     }
   }
   __syncthreads();
-  const int cols = k.tx * V;
-  const int c0 = (q.col - q.tx) * V;
+  const int c0 = (q.col - q.tx) * V, cols = min(k.tx * V, a.C - c0), width = k.tx * V;
   for (int j = threadIdx.x; j < cols; j += kThreads) {
-    if (c0 + j >= a.C) break;
     float cn = 0.f, cm = 0.f, cq = 0.f;
     for (int r = 0; r < k.ty; ++r) {
       const int rows = q.p1 - q.p0 - r;
       if (rows <= 0) break;
-      const float2 v = red[r * cols + j];
+      const float2 v = red[r * width + j];
       join(cn, cm, cq, (float)((rows + k.ty - 1) / k.ty), v.x, v.y);
     }
-    part[((long long)q.b * k.nchunk + q.chunk) * a.C + c0 + j] = make_float2(cm, cq);
+    if (a.shift) cm += load_param(a.shift, a.stype, (long long)q.b * a.C + c0 + j);
+    red[j] = make_float2(cm, cq);  // row 0 of this channel has been read
+  }
+  __syncthreads();
+  const float pixels = (float)(q.p1 - q.p0);
+  float2* out = part + ((long long)q.b * k.nchunk + q.chunk) * (a.C / k.cell) + c0 / k.cell;
+  for (int j = threadIdx.x; j < cols / k.cell; j += kThreads) {
+    float cn = 0.f, cm = 0.f, cq = 0.f;
+    for (int c = 0; c < k.cell; ++c) {
+      const float2 v = red[j * k.cell + c];
+      join(cn, cm, cq, pixels, v.x, v.y);
+    }
+    out[j] = make_float2(cm, cq);
   }
 }
 
-template <int N>
-__device__ __forceinline__ double block_sum(double v, double* buf) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double t = 0;
-#pragma unroll
-  for (int i = 0; i < N / 32; ++i) t += buf[i];
-  return t;
-}
-
-// Mean and 1/sqrt(variance + eps) of every (b, group) from the parts.
+// Mean and 1/sqrt(variance + eps) of every (b, group) from the parts: a warp each.
 __global__ void __launch_bounds__(128) finish_stats(Args a, Walk k, const float2* part,
                                                     float* stats) {
-  __shared__ double buf[4];
+  pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
-  const int items = k.nchunk * a.cpg;
-  const double total = (double)a.HW * a.cpg;
-  auto item = [&](int i, double* n, double* m, double* q) {
-    const int ch = i / a.cpg, c = g * a.cpg + i % a.cpg;
-    const float2 v = part[((long long)b * k.nchunk + ch) * a.C + c];
-    *n = min(k.chunk, a.HW - ch * k.chunk);
-    *m = (double)v.x + (a.shift ? load_param(a.shift, a.stype, (long long)b * a.C + c) : 0.f);
-    *q = v.y;
-  };
-  double n, m, q, s = 0;
-  for (int i = threadIdx.x; i < items; i += 128) {
-    item(i, &n, &m, &q);
-    s += n * m;
+  const int bg = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (bg >= a.B * a.G) return;
+  const int b = bg / a.G, g = bg % a.G, cells = a.cpg / k.cell, items = k.nchunk * cells;
+  float n = 0.f, m = 0.f, s = 0.f;
+  for (int i = lane; i < items; i += 32) {
+    const int ch = i / cells;
+    const float2 v = part[((long long)b * k.nchunk + ch) * (a.C / k.cell) + g * cells + (i - ch * cells)];
+    join(n, m, s, (float)(min(k.chunk, a.HW - ch * k.chunk) * k.cell), v.x, v.y);
   }
-  const double mean = block_sum<128>(s, buf) / total;
-  s = 0;
-  for (int i = threadIdx.x; i < items; i += 128) {
-    item(i, &n, &m, &q);
-    s += q + n * (m - mean) * (m - mean);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    // The lower lane's part first, in both lanes of a pair.
+    const float on = __shfl_xor_sync(~0u, n, o), om = __shfl_xor_sync(~0u, m, o),
+                os = __shfl_xor_sync(~0u, s, o);
+    float x = lane & o ? on : n, y = lane & o ? om : m, z = lane & o ? os : s;
+    join(x, y, z, lane & o ? n : on, lane & o ? m : om, lane & o ? s : os);
+    n = x, m = y, s = z;
   }
-  const double var = block_sum<128>(s, buf) / total;
-  if (threadIdx.x == 0) {
-    stats[blockIdx.x] = (float)mean;
-    stats[(long long)a.B * a.G + blockIdx.x] = (float)(1.0 / sqrt(var + (double)a.eps));
+  if (lane == 0) {
+    stats[bg] = m;
+    stats[(long long)a.B * a.G + bg] = 1.f / sqrtf(s / n + a.eps);
   }
 }
 
-// A thread's channel constants: n = (x - mu) r, z = n w + beta.
+// A block's channel constants, in shared memory: n = (x + mu) r, z = n w + beta.
 template <int V>
 struct Chan {
-  float mu[V], r[V], w[V], beta[V];
+  float mu[kThreads * V], r[kThreads * V], w[kThreads * V], beta[kThreads * V];
 };
 template <int V>
-__device__ __forceinline__ Chan<V> channels(const Args& a, int b, int c0, const float* stats) {
-  Chan<V> h;
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int c = c0 + e;
-    const long long bg = (long long)b * a.G + c / a.cpg;
-    h.mu[e] = stats[bg] -
-              (a.shift ? load_param(a.shift, a.stype, (long long)b * a.C + c) : 0.f);
-    h.r[e] = stats[(long long)a.B * a.G + bg];
-    h.w[e] = a.w ? load_param(a.w, a.wtype, c) : 1.f;
-    h.beta[e] = a.beta ? load_param(a.beta, a.wtype, c) : 0.f;
+__device__ __forceinline__ void channels(Chan<V>& h, const Args& a, const Walk& k, const Place& q,
+                                         const float* stats) {
+  const int c0 = (q.col - q.tx) * V, cols = min(k.tx * V, a.C - c0);
+  for (int j = threadIdx.x; j < cols; j += kThreads) {
+    const int c = c0 + j;
+    const long long bg = (long long)q.b * a.G + c / a.cpg;
+    h.mu[j] = (a.shift ? load_param(a.shift, a.stype, (long long)q.b * a.C + c) : 0.f) - stats[bg];
+    h.r[j] = stats[(long long)a.B * a.G + bg];
+    h.w[j] = a.w ? load_param(a.w, a.wtype, c) : 1.f;
+    h.beta[j] = a.beta ? load_param(a.beta, a.wtype, c) : 0.f;
   }
-  return h;
 }
 
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* stats) {
+  using L = Lanes<T, V>;
+  using F = typename L::F;
+  constexpr int J = V / L::W;
+  __shared__ Chan<V> h;
+  pdl_trigger();
   pdl_wait();
   const Place q = place(a, k);
+  channels<V>(h, a, k, q, stats);
+  __syncthreads();
   if (!q.active) return;
-  using L = Lanes<T, V>;
-  Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+  F mu[J], w[J], beta[J];
 #pragma unroll
-  for (int e = 0; e < V; ++e) h.w[e] *= h.r[e], h.mu[e] = -h.mu[e];
+  for (int j = 0; j < J; ++j) {
+    mu[j] = L::at(h.mu + q.tx * V, j);
+    w[j] = mul(L::at(h.w + q.tx * V, j), L::at(h.r + q.tx * V, j));
+    beta[j] = L::at(h.beta + q.tx * V, j);
+  }
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   T* y = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
-#pragma unroll 4
-  for (int p = q.p0 + q.ty; p < q.p1; p += k.ty) {
-    const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
-    Pack<T, V> o;
+  for (int p = q.p0 + q.ty; p < q.p1; p += kAhead * k.ty) {
+    Pack<T, V> v[kAhead];
 #pragma unroll
-    for (int j = 0; j < V / L::W; ++j)
-      L::set(o, j, act<ACT>(fma(add(L::get(v, j), L::at(h.mu, j)), L::at(h.w, j), L::at(h.beta, j))));
-    store_pack<T, V>(y + (long long)p * a.C, o);
+    for (int u = 0; u < kAhead; ++u)
+      if (p + u * k.ty < q.p1) v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (p + u * k.ty < q.p1) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          L::set(v[u], j, act<ACT>(fma(add(L::get(v[u], j), mu[j]), w[j], beta[j])));
+        store_pack<T, V>(y + (long long)(p + u * k.ty) * a.C, v[u]);
+      }
   }
 }
 
@@ -307,16 +316,27 @@ __global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* s
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const float* stats,
                                                          float* part) {
-  __shared__ float red[3][kThreads * V];
-  pdl_wait();
-  const Place q = place(a, k);
   using L = Lanes<T, V>;
   using F = typename L::F;
-  float s1[V] = {}, s2[V] = {}, s3[V] = {};
-  if (q.active) {
-    Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
+  constexpr int J = V / L::W;
+  __shared__ union {
+    Chan<V> h;
+    float red[3][kThreads * V];
+  } sm;
+  pdl_trigger();
+  pdl_wait();
+  const Place q = place(a, k);
+  channels<V>(sm.h, a, k, q, stats);
+  __syncthreads();
+  F s1[J], s2[J], s3[J], mu[J], r[J], w[J], beta[J];
 #pragma unroll
-    for (int e = 0; e < V; ++e) h.mu[e] = -h.mu[e];
+  for (int j = 0; j < J; ++j) {
+    s1[j] = s2[j] = s3[j] = splat<F>(0.f);
+    mu[j] = L::at(sm.h.mu + q.tx * V, j), r[j] = L::at(sm.h.r + q.tx * V, j);
+    w[j] = L::at(sm.h.w + q.tx * V, j), beta[j] = L::at(sm.h.beta + q.tx * V, j);
+  }
+  __syncthreads();
+  if (q.active) {
     const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
     const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
 #pragma unroll 2
@@ -324,135 +344,149 @@ __global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const f
       const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
       const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
 #pragma unroll
-      for (int j = 0; j < V / L::W; ++j) {
-        const F n = mul(add(L::get(v, j), L::at(h.mu, j)), L::at(h.r, j));
-        const F dz = act_grad<ACT>(L::get(d, j), fma(n, L::at(h.w, j), L::at(h.beta, j)));
-        L::put(s1, j, add(L::at(s1, j), dz));
-        L::put(s2, j, fma(dz, n, L::at(s2, j)));
-        L::put(s3, j, add(L::at(s3, j), n));
+      for (int j = 0; j < J; ++j) {
+        const F n = mul(add(L::get(v, j), mu[j]), r[j]);
+        const F dz = act_grad<ACT>(L::get(d, j), fma(n, w[j], beta[j]));
+        s1[j] = add(s1[j], dz);
+        s2[j] = fma(dz, n, s2[j]);
+        s3[j] = add(s3[j], n);
       }
     }
   }
+  const int width = k.tx * V;
   if (q.ty < k.ty) {
+    const int i = q.ty * width + q.tx * V;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int i = (q.ty * k.tx + q.tx) * V + e;
-      red[0][i] = s1[e];
-      red[1][i] = s2[e];
-      red[2][i] = s3[e];
+    for (int j = 0; j < J; ++j) {
+      L::put(sm.red[0] + i, j, s1[j]);
+      L::put(sm.red[1] + i, j, s2[j]);
+      L::put(sm.red[2] + i, j, s3[j]);
     }
   }
   __syncthreads();
-  const int cols = k.tx * V;
-  const int c0 = (q.col - q.tx) * V;
+  const int c0 = (q.col - q.tx) * V, cols = min(width, a.C - c0);
   const long long plane = (long long)a.B * k.nchunk * a.C;
-  for (int j = threadIdx.x; j < cols; j += kThreads) {
-    if (c0 + j >= a.C) break;
-    float t[3] = {};
-    for (int r = 0; r < k.ty; ++r)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) t[i] += red[i][r * cols + j];
-    float* o = part + ((long long)q.b * k.nchunk + q.chunk) * a.C + c0 + j;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) o[i * plane] = t[i];
+  for (int j = threadIdx.x; j < 3 * cols; j += kThreads) {
+    const int i = j / cols, c = j - i * cols;
+    float t = 0.f;
+    for (int r = 0; r < k.ty; ++r) t += sm.red[i][r * width + c];
+    part[i * plane + ((long long)q.b * k.nchunk + q.chunk) * a.C + c0 + c] = t;
   }
 }
 
-// Joins the chunks: sums[b][c] = (sum dz, sum dz n), means[b][g] = (A, D), and
-// the shift's gradient.  A warp per channel, lanes over the chunks.
-__global__ void __launch_bounds__(128) finish_grad(Args a, Walk k, const float* stats,
-                                                   const float* part, float2* sums,
-                                                   float2* means, void* dshift) {
-  __shared__ double buf[4];
-  extern __shared__ float s3[];  // [cpg]
+// The chunks' sums of every (b, channel), in order: sums[3][B][C].
+__global__ void __launch_bounds__(256) join_grad(Args a, Walk k, const float* part, float* sums) {
+  __shared__ double buf[8][32];
+  pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / a.G, g = blockIdx.x % a.G;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long plane = (long long)a.B * k.nchunk * a.C;
-  double wa = 0, wd = 0;
-  for (int j = warp; j < a.cpg; j += 4) {
-    const int c = g * a.cpg + j;
-    double t[3] = {};
-    for (int ch = lane; ch < k.nchunk; ch += 32) {
-      const float* o = part + ((long long)b * k.nchunk + ch) * a.C + c;
-#pragma unroll
-      for (int i = 0; i < 3; ++i) t[i] += o[i * plane];
-    }
-#pragma unroll
-    for (int i = 0; i < 3; ++i)
-      for (int o = 16; o > 0; o >>= 1) t[i] += __shfl_xor_sync(~0u, t[i], o);
-    if (lane == 0) {
-      const float w = a.w ? load_param(a.w, a.wtype, c) : 1.f;
-      sums[(long long)b * a.C + c] = make_float2((float)t[0], (float)t[1]);
-      s3[j] = (float)t[2];
-      wa += w * t[0];
-      wd += w * t[1];
-    }
+  const int cblocks = (a.C + 31) / 32, lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int b = blockIdx.x / cblocks, c = blockIdx.x % cblocks * 32 + lane;
+  double t = 0;
+  if (c < a.C) {
+    const float* from = part + ((long long)blockIdx.y * a.B + b) * k.nchunk * a.C + c;
+    for (int ch = row; ch < k.nchunk; ch += 8) t += from[(long long)ch * a.C];
   }
-  const double total = (double)a.HW * a.cpg;
-  const double A = block_sum<128>(wa, buf) / total;
-  const double D = block_sum<128>(wd, buf) / total;
-  if (threadIdx.x == 0) means[blockIdx.x] = make_float2((float)A, (float)D);
-  if (dshift) {
-    const double r = stats[(long long)a.B * a.G + blockIdx.x];
-    for (int j = threadIdx.x; j < a.cpg; j += 128) {
-      const int c = g * a.cpg + j;
-      const double w = a.w ? load_param(a.w, a.wtype, c) : 1.f;
-      const double t = sums[(long long)b * a.C + c].x;
-      store_param(dshift, a.stype, (long long)b * a.C + c, (float)(r * (w * t - a.HW * A - D * s3[j])));
-    }
+  buf[row][lane] = t;
+  __syncthreads();
+  if (row == 0 && c < a.C) {
+#pragma unroll
+    for (int r = 1; r < 8; ++r) t += buf[r][lane];
+    sums[((long long)blockIdx.y * a.B + b) * a.C + c] = (float)t;
   }
 }
 
 // dw and dbeta: the samples' sums, in order.
-__global__ void __launch_bounds__(128) param_grad(Args a, const float2* sums, void* dw,
+__global__ void __launch_bounds__(128) param_grad(Args a, const float* sums, void* dw,
                                                   void* dbeta) {
+  pdl_trigger();
   pdl_wait();
   const int c = blockIdx.x * 128 + threadIdx.x;
   if (c >= a.C) return;
+  const long long plane = (long long)a.B * a.C;
   double s = 0, t = 0;
   for (int b = 0; b < a.B; ++b) {
-    const float2 v = sums[(long long)b * a.C + c];
-    s += v.x;
-    t += v.y;
+    s += sums[(long long)b * a.C + c];
+    t += sums[plane + (long long)b * a.C + c];
   }
   if (dw) store_param(dw, a.wtype, c, (float)t);
   if (dbeta) store_param(dbeta, a.wtype, c, (float)s);
 }
 
+__device__ __forceinline__ float warp_total(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// Second pass: dx, and from the first chunk's blocks the shift's gradient.
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kThreads) apply_grad(Args a, Walk k, const float* stats,
-                                                       const float2* means) {
-  pdl_wait();
-  const Place q = place(a, k);
-  if (!q.active) return;
+                                                       const float* sums, void* dshift) {
   using L = Lanes<T, V>;
   using F = typename L::F;
-  Chan<V> h = channels<V>(a, q.b, q.col * V, stats);
-  float A[V], D[V];
+  constexpr int J = V / L::W;
+  __shared__ Chan<V> h;
+  __shared__ float A[kThreads * V], D[kThreads * V];  // minus the means, by channel
+  pdl_trigger();
+  pdl_wait();
+  const Place q = place(a, k);
+  channels<V>(h, a, k, q, stats);
+  __syncthreads();
+  const int c0 = (q.col - q.tx) * V, cols = min(k.tx * V, a.C - c0);
+  const long long plane = (long long)a.B * a.C, bc = (long long)q.b * a.C;
+  const float inv = 1.f / ((float)a.HW * a.cpg);
+  for (int g = c0 / a.cpg + (threadIdx.x >> 5); g <= (c0 + cols - 1) / a.cpg; g += kThreads / 32) {
+    // The whole group's, also where the block has a part of its channels.
+    const int lane = threadIdx.x & 31;
+    float wa = 0.f, wd = 0.f;
+    for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32) {
+      const float w = a.w ? load_param(a.w, a.wtype, c) : 1.f;
+      wa = fmaf(w, sums[bc + c], wa);
+      wd = fmaf(w, sums[plane + bc + c], wd);
+    }
+    wa = warp_total(wa) * inv;
+    wd = warp_total(wd) * inv;
+    for (int c = max(c0, g * a.cpg) + lane; c < min(c0 + cols, (g + 1) * a.cpg); c += 32) {
+      A[c - c0] = -wa;
+      D[c - c0] = -wd;
+      if (dshift && q.chunk == 0)
+        store_param(dshift, a.stype, bc + c,
+                    h.r[c - c0] * (h.w[c - c0] * sums[bc + c] - a.HW * wa -
+                                   wd * sums[2 * plane + bc + c]));
+    }
+  }
+  __syncthreads();
+  if (!q.active) return;
+  F mu[J], r[J], w[J], beta[J], mA[J], mD[J];
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    h.mu[e] = -h.mu[e];
-    const float2 m = means[(long long)q.b * a.G + (q.col * V + e) / a.cpg];
-    A[e] = -m.x;
-    D[e] = -m.y;
+  for (int j = 0; j < J; ++j) {
+    mu[j] = L::at(h.mu + q.tx * V, j), r[j] = L::at(h.r + q.tx * V, j);
+    w[j] = L::at(h.w + q.tx * V, j), beta[j] = L::at(h.beta + q.tx * V, j);
+    mA[j] = L::at(A + q.tx * V, j), mD[j] = L::at(D + q.tx * V, j);
   }
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
   T* dx = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
-#pragma unroll 2
-  for (int p = q.p0 + q.ty; p < q.p1; p += k.ty) {
-    const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
-    const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
-    Pack<T, V> o;
+  constexpr int U = kAhead / 2;
+  for (int p = q.p0 + q.ty; p < q.p1; p += U * k.ty) {
+    Pack<T, V> v[U], d[U];
 #pragma unroll
-    for (int j = 0; j < V / L::W; ++j) {
-      const F r = L::at(h.r, j), w = L::at(h.w, j);
-      const F n = mul(add(L::get(v, j), L::at(h.mu, j)), r);
-      const F dz = act_grad<ACT>(L::get(d, j), fma(n, w, L::at(h.beta, j)));
-      L::set(o, j, mul(r, fma(n, L::at(D, j), fma(w, dz, L::at(A, j)))));
-    }
-    store_pack<T, V>(dx + (long long)p * a.C, o);
+    for (int u = 0; u < U; ++u)
+      if (p + u * k.ty < q.p1) {
+        v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+        d[u] = load_pack<T, V>(dy + (p + u * k.ty) * a.yp);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u * k.ty < q.p1) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const F n = mul(add(L::get(v[u], j), mu[j]), r[j]);
+          const F dz = act_grad<ACT>(L::get(d[u], j), fma(n, w[j], beta[j]));
+          L::set(v[u], j, mul(r[j], fma(n, mD[j], fma(w[j], dz, mA[j]))));
+        }
+        store_pack<T, V>(dx + (long long)(p + u * k.ty) * a.C, v[u]);
+      }
   }
 }
 
@@ -508,12 +542,6 @@ __device__ __forceinline__ void stay_packed(Pack<T, V> (&d)[NV]) {
   }
 }
 
-__device__ __forceinline__ float warp_total(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  return v;
-}
-
 struct Spot {
   int b, rank, c0, nch, ng, g0, p0, p1, tx, ty, nv;
   bool active;
@@ -553,6 +581,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
   float* wt = sh + width;               // [width] weight, later weight / sigma
   float* bt = wt + width;               // [width] bias, later the whole offset
   float* part = bt + width;             // [2][gb] the block's mean and deviations
+  pdl_trigger();
   pdl_wait();
   const Spot q = spot(a, k, V);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -685,7 +714,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
 // The gradient of a slab: x and dy in registers, the channels' sums exchanged.
 template <typename T, int V, int NV, int ACT>
 __global__ void __launch_bounds__(kSlabThreads, 1)
-    resident_grad(Args a, Slab k, const float* stats, float2* sums, void* dshift) {
+    resident_grad(Args a, Slab k, const float* stats, float* sums, void* dshift) {
   using L = Lanes<T, V>;
   using F = typename L::F;
   constexpr int W = L::W;
@@ -701,6 +730,7 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
   float* all = own + 3 * width;    // [3][width] the sample's sums
   float* ga = all + 3 * width;     // [width] -A
   float* gd = ga + width;          // [width] -D
+  pdl_trigger();
   pdl_wait();
   const Spot q = spot(a, k, V);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -795,7 +825,8 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
       gd[c] = -wd;
       if (q.rank == 0) {
         const long long bc = (long long)q.b * a.C + q.c0 + c;
-        sums[bc] = make_float2(all[c], all[width + c]);
+        sums[bc] = all[c];
+        sums[(long long)a.B * a.C + bc] = all[width + c];
         if (dshift)
           store_param(dshift, a.stype, bc,
                       rs[c] * (wt[c] * all[c] - a.HW * wa - wd * all[2 * width + c]));
@@ -837,17 +868,18 @@ int device_sms() {
   return sms;
 }
 
-Walk make_walk(int B, int HW, int C, int V) {
+Walk make_walk(int B, int HW, int C, int G, int V, bool grad) {
   Walk k;
+  const int cpg = C / G;
   k.cv = C / V;
   k.ncb = (k.cv + kThreads - 1) / kThreads;
   k.tx = (k.cv + k.ncb - 1) / k.ncb;
   k.ty = kThreads / k.tx;
-  // Eight blocks for every SM, but at least four pixels for every thread.
-  const long long blocks = 8ll * device_sms();
-  long long chunks = blocks / ((long long)B * k.ncb);
+  k.cell = k.ncb == 1 || k.tx * V % cpg == 0 ? cpg : 1;
+  // One wave of blocks (by their registers), but at least `kAhead` pixels a thread.
+  long long chunks = (grad ? 2ll : 3ll) * device_sms() / ((long long)B * k.ncb);
   if (chunks < 1) chunks = 1;
-  const long long most = (HW + 4ll * k.ty - 1) / (4ll * k.ty);
+  const long long most = (HW + (long long)kAhead * k.ty - 1) / ((long long)kAhead * k.ty);
   if (chunks > most) chunks = most;
   k.chunk = (int)((HW + chunks - 1) / chunks);
   k.nchunk = (HW + k.chunk - 1) / k.chunk;
@@ -858,17 +890,16 @@ size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
 // Workspace of the larger walk (the vector width depends on the pointers).
 long long workspace_bytes(int B, int HW, int C, int G, bool grad) {
-  long long most = 0;
+  size_t most = 0;
   for (int V : {1, 4, 8}) {
     if (C % V) continue;
-    const Walk k = make_walk(B, HW, C, V);
-    const long long parts = (long long)B * k.nchunk * C;
-    const long long n = grad ? (long long)(align256(parts * 12) + align256((size_t)B * C * 8) +
-                                           align256((size_t)B * G * 8))
-                             : (long long)(align256(parts * 8) + align256((size_t)B * G * 8));
+    const Walk k = make_walk(B, HW, C, G, V, grad);
+    const size_t parts = (size_t)B * k.nchunk * C;
+    const size_t n = grad ? align256(parts * 12) + align256((size_t)B * C * 12)
+                          : align256(parts / k.cell * 8) + align256((size_t)B * G * 8);
     if (n > most) most = n;
   }
-  return most;
+  return (long long)most;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -960,7 +991,7 @@ cudaError_t forward_resident(const Args& a, const Slab& k, float* stats, cudaStr
 }
 
 template <typename T, int V, int ACT>
-cudaError_t grad_resident(const Args& a, const Slab& k, const float* stats, float2* sums,
+cudaError_t grad_resident(const Args& a, const Slab& k, const float* stats, float* sums,
                           void* dshift, cudaStream_t s) {
   const unsigned grid = (unsigned)((long long)a.B * k.nblk * k.cs);
   const size_t smem = slab_smem(k, V, true);
@@ -980,12 +1011,12 @@ cudaError_t forward(const Args& a, int act, float* stats, bool want_stats, unsig
   if (make_slab(a.B, a.HW, a.C, a.G, V, kMostForward, device_sms(), &slab))
     return act == kSilu ? forward_resident<T, V, kSilu>(a, slab, want_stats ? stats : nullptr, s)
                         : forward_resident<T, V, kNone>(a, slab, want_stats ? stats : nullptr, s);
-  const Walk k = make_walk(a.B, a.HW, a.C, V);
+  const Walk k = make_walk(a.B, a.HW, a.C, a.G, V, false);
   float2* part = reinterpret_cast<float2*>(ws);
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
   cudaError_t e = launch_pdl(kPdlInput, partial_stats<T, V>, grid, dim3(kThreads), 0, s, a, k, part);
   if (e == cudaSuccess)
-    e = launch_pdl(kPdlInput, finish_stats, dim3(a.B * a.G), dim3(128), 0, s, a, k,
+    e = launch_pdl(kPdlInput, finish_stats, dim3((a.B * a.G + 3) / 4), dim3(128), 0, s, a, k,
                    (const float2*)part, stats);
   if (e != cudaSuccess) return e;
   return act == kSilu ? launch_pdl(kPdlInput, apply<T, V, kSilu>, grid, dim3(kThreads), 0, s, a, k,
@@ -997,12 +1028,10 @@ cudaError_t forward(const Args& a, int act, float* stats, bool want_stats, unsig
 template <typename T, int V, int ACT>
 cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, void* dshift,
                      unsigned char* ws, cudaStream_t s) {
-  const Walk k = make_walk(a.B, a.HW, a.C, V);
+  const Walk k = make_walk(a.B, a.HW, a.C, a.G, V, true);
   float* part = reinterpret_cast<float*>(ws);
   ws += align256((size_t)a.B * k.nchunk * a.C * 12);
-  float2* sums = reinterpret_cast<float2*>(ws);
-  ws += align256((size_t)a.B * a.C * 8);
-  float2* means = reinterpret_cast<float2*>(ws);
+  float* sums = reinterpret_cast<float*>(ws);  // [3][B][C]
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
   cudaError_t e;
   Slab slab;
@@ -1010,20 +1039,20 @@ cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, v
     e = grad_resident<T, V, ACT>(a, slab, stats, sums, dshift, s);
     if (e == cudaSuccess && (dw || dbeta))
       e = launch_pdl(kPdlInput, param_grad, dim3((a.C + 127) / 128), dim3(128), 0, s, a,
-                     (const float2*)sums, dw, dbeta);
+                     (const float*)sums, dw, dbeta);
     return e;
   }
   e = launch_pdl(kPdlInput, partial_grad<T, V, ACT>, grid, dim3(kThreads), 0, s, a, k,
                              stats, part);
   if (e == cudaSuccess)
-    e = launch_pdl(kPdlInput, finish_grad, dim3(a.B * a.G), dim3(128), a.cpg * sizeof(float), s, a,
-                   k, stats, (const float*)part, sums, means, dshift);
+    e = launch_pdl(kPdlInput, join_grad, dim3(a.B * ((a.C + 31) / 32), 3), dim3(256), 0, s, a, k,
+                   (const float*)part, sums);
   if (e == cudaSuccess)
     e = launch_pdl(kPdlInput, apply_grad<T, V, ACT>, grid, dim3(kThreads), 0, s, a, k, stats,
-                   (const float2*)means);
+                   (const float*)sums, dshift);
   if (e == cudaSuccess && (dw || dbeta))
     e = launch_pdl(kPdlInput, param_grad, dim3((a.C + 127) / 128), dim3(128), 0, s, a,
-                   (const float2*)sums, dw, dbeta);
+                   (const float*)sums, dw, dbeta);
   return e;
 }
 
