@@ -44,19 +44,23 @@ struct Args {
   float eps;
 };
 
-// How the grid walks one tensor: a block takes TX vector columns of `chunk`
-// pixels of one sample, TY pixels at a time.
+// How the grid walks one tensor: a block takes TX vector columns, TY pixels at a time;
+// a tile is U times TY pixels, U vectors that every thread has on their way together,
+// and block `chunk` of a sample has `per` tiles in a row.
 struct Walk {
   int cv;      // vector columns of a pixel
   int ncb;     // column blocks
   int tx, ty;  // threads
-  int chunk;   // pixels per block
-  int nchunk;
+  int tile;    // pixels of a tile
+  int ntile, per, nchunk;
   int cell;    // channels that share a part of the statistics: a group's, or one
 };
 
 constexpr int kThreads = 256;
-constexpr int kAhead = 4;  // pixels that a streaming thread has on their way
+// Vectors that a streaming thread has on their way: with the blocks that fit an SM,
+// the 60 to 90 KB in flight that its share of the bandwidth takes.
+constexpr int kAhead = 8;
+constexpr int kBlocksForward = 3, kBlocksGrad = 2;  // of a streaming kernel on an SM
 
 // Channels are worked on in pairs (the paired 32-bit instructions halve the count),
 // or singly where a thread holds one.
@@ -76,8 +80,6 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float2 ex2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
-__device__ __forceinline__ float2 rcp(float2 x) { return make_float2(rcp(x.x), rcp(x.y)); }
 template <typename F>
 __device__ __forceinline__ F splat(float x);
 template <>
@@ -85,9 +87,16 @@ __device__ __forceinline__ float splat<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ float2 splat<float2>(float x) { return make_float2(x, x); }
 
-template <typename F>
-__device__ __forceinline__ F sigmoid(F z) {
-  return rcp(add(ex2(mul(z, splat<F>(-1.4426950408889634f))), splat<F>(1.f)));
+// 1 / (1 + e^-z).  A pair shares one reciprocal, 1 / (d e) = (1/d) (1/e): the special
+// function unit, at 16 results a clock and SM, is the nearest bound of these passes
+// after memory, and this takes a quarter of its work away.  The exponent stops at 2^63
+// to keep the product finite: below z = -43 the sigmoid is 2^-63 instead of less.
+__device__ __forceinline__ float sigmoid(float z) { return rcp(ex2(z * -1.4426950408889634f) + 1.f); }
+__device__ __forceinline__ float2 sigmoid(float2 z) {
+  const float2 t = mul(z, splat<float2>(-1.4426950408889634f));
+  const float2 d = add(make_float2(ex2(fminf(t.x, 63.f)), ex2(fminf(t.y, 63.f))), splat<float2>(1.f));
+  const float r = rcp(d.x * d.y);
+  return mul(make_float2(r, r), make_float2(d.y, d.x));
 }
 template <int ACT, typename F>
 __device__ __forceinline__ F act(F z) {
@@ -145,7 +154,7 @@ __device__ __forceinline__ void join(float& na, float& ma, float& qa, float nb, 
 }
 
 struct Place {
-  int b, chunk, p0, p1, tx, ty, col;
+  int b, chunk, tx, ty, col;
   bool active;
 };
 __device__ __forceinline__ Place place(const Args& a, const Walk& k) {
@@ -155,18 +164,24 @@ __device__ __forceinline__ Place place(const Args& a, const Walk& k) {
   id /= k.ncb;
   q.chunk = id % k.nchunk;
   q.b = id / k.nchunk;
-  q.p0 = q.chunk * k.chunk;
-  q.p1 = min(a.HW, q.p0 + k.chunk);
   q.tx = threadIdx.x % k.tx;
   q.ty = threadIdx.x / k.tx;
   q.col = cb * k.tx + q.tx;
   q.active = q.ty < k.ty && q.col < k.cv;
   return q;
 }
+// Pixels of a chunk, and of the chunk's thread row `r` (a row takes every TY-th).
+__device__ __forceinline__ int chunk_pixels(const Args& a, const Walk& k, int chunk) {
+  return min(a.HW - chunk * k.per * k.tile, k.per * k.tile);
+}
+__device__ __forceinline__ int row_pixels(const Args& a, const Walk& k, int chunk, int r) {
+  const int left = chunk_pixels(a, k, chunk) - r;
+  return left > 0 ? (left + k.ty - 1) / k.ty : 0;
+}
 
 // Per-channel mean and squared deviations of x over one chunk of pixels.
 template <typename T, int V>
-__global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2* part) {
+__global__ void __launch_bounds__(kThreads, kBlocksForward) partial_stats(Args a, Walk k, float2* part) {
   __shared__ float2 red[kThreads * V];
   pdl_trigger();
   pdl_wait();
@@ -174,23 +189,32 @@ __global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2
   using L = Lanes<T, V>;
   using F = typename L::F;
   float s1[V] = {}, s2[V] = {}, pivot[V] = {};
-  int n = 0;
-  if (q.active && q.p0 + q.ty < q.p1) {
-    n = (q.p1 - q.p0 - q.ty + k.ty - 1) / k.ty;
-    const T* p = static_cast<const T*>(a.x) + q.b * a.xb + (q.p0 + q.ty) * a.xp + q.col * V;
-    const long long step = k.ty * a.xp;
-    const Pack<T, V> first = load_pack<T, V>(p);
+  const int n = q.active ? row_pixels(a, k, q.chunk, q.ty) : 0;
+  if (n) {
+    const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
+    bool fresh = true;
+    const int end = min(k.ntile, (q.chunk + 1) * k.per);
+    for (int i = q.chunk * k.per; i < end; ++i) {
+      const int p = i * k.tile + q.ty;
+      Pack<T, V> v[kAhead];
 #pragma unroll
-    for (int e = 0; e < V; ++e) pivot[e] = to_f32(first.e[e]);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i, p += step) {
-      const Pack<T, V> v = load_pack<T, V>(p);
+      for (int u = 0; u < kAhead; ++u)
+        if (p + u * k.ty < a.HW) v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+      if (fresh) {
 #pragma unroll
-      for (int j = 0; j < V / L::W; ++j) {
-        const F d = fma(L::at(pivot, j), splat<F>(-1.f), L::get(v, j));
-        L::put(s1, j, add(L::at(s1, j), d));
-        L::put(s2, j, fma(d, d, L::at(s2, j)));
+        for (int e = 0; e < V; ++e) pivot[e] = to_f32(v[0].e[e]);
+        fresh = false;
       }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (p + u * k.ty < a.HW) {
+#pragma unroll
+          for (int j = 0; j < V / L::W; ++j) {
+            const F d = fma(L::at(pivot, j), splat<F>(-1.f), L::get(v[u], j));
+            L::put(s1, j, add(L::at(s1, j), d));
+            L::put(s2, j, fma(d, d, L::at(s2, j)));
+          }
+        }
     }
   }
   if (q.ty < k.ty) {
@@ -206,16 +230,14 @@ __global__ void __launch_bounds__(kThreads) partial_stats(Args a, Walk k, float2
   for (int j = threadIdx.x; j < cols; j += kThreads) {
     float cn = 0.f, cm = 0.f, cq = 0.f;
     for (int r = 0; r < k.ty; ++r) {
-      const int rows = q.p1 - q.p0 - r;
-      if (rows <= 0) break;
       const float2 v = red[r * width + j];
-      join(cn, cm, cq, (float)((rows + k.ty - 1) / k.ty), v.x, v.y);
+      join(cn, cm, cq, (float)row_pixels(a, k, q.chunk, r), v.x, v.y);
     }
     if (a.shift) cm += load_param(a.shift, a.stype, (long long)q.b * a.C + c0 + j);
     red[j] = make_float2(cm, cq);  // row 0 of this channel has been read
   }
   __syncthreads();
-  const float pixels = (float)(q.p1 - q.p0);
+  const float pixels = (float)chunk_pixels(a, k, q.chunk);
   float2* out = part + ((long long)q.b * k.nchunk + q.chunk) * (a.C / k.cell) + c0 / k.cell;
   for (int j = threadIdx.x; j < cols / k.cell; j += kThreads) {
     float cn = 0.f, cm = 0.f, cq = 0.f;
@@ -239,7 +261,7 @@ __global__ void __launch_bounds__(128) finish_stats(Args a, Walk k, const float2
   for (int i = lane; i < items; i += 32) {
     const int ch = i / cells;
     const float2 v = part[((long long)b * k.nchunk + ch) * (a.C / k.cell) + g * cells + (i - ch * cells)];
-    join(n, m, s, (float)(min(k.chunk, a.HW - ch * k.chunk) * k.cell), v.x, v.y);
+    join(n, m, s, (float)chunk_pixels(a, k, ch) * k.cell, v.x, v.y);
   }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -276,7 +298,7 @@ __device__ __forceinline__ void channels(Chan<V>& h, const Args& a, const Walk& 
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* stats) {
+__global__ void __launch_bounds__(kThreads, kBlocksForward) apply(Args a, Walk k, const float* stats) {
   using L = Lanes<T, V>;
   using F = typename L::F;
   constexpr int J = V / L::W;
@@ -284,29 +306,32 @@ __global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* s
   pdl_trigger();
   pdl_wait();
   const Place q = place(a, k);
-  channels<V>(h, a, k, q, stats);
-  __syncthreads();
-  if (!q.active) return;
-  F mu[J], w[J], beta[J];
-#pragma unroll
-  for (int j = 0; j < J; ++j) {
-    mu[j] = L::at(h.mu + q.tx * V, j);
-    w[j] = mul(L::at(h.w + q.tx * V, j), L::at(h.r + q.tx * V, j));
-    beta[j] = L::at(h.beta + q.tx * V, j);
-  }
+  const int end = q.active ? min(a.HW, (q.chunk + 1) * k.per * k.tile) : 0;
+  int p = q.chunk * k.per * k.tile + q.ty;
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   T* y = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
-  for (int p = q.p0 + q.ty; p < q.p1; p += kAhead * k.ty) {
-    Pack<T, V> v[kAhead];
+  Pack<T, V> v[kAhead];
+  const auto load = [&] {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (p + u * k.ty < q.p1) v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+      if (p + u * k.ty < end) v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+  };
+  load();  // needs no statistics
+  channels<V>(h, a, k, q, stats);
+  __syncthreads();
+  F w[J], beta[J];  // z = x w + beta
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    w[j] = mul(L::at(h.w + q.tx * V, j), L::at(h.r + q.tx * V, j));
+    beta[j] = fma(L::at(h.mu + q.tx * V, j), w[j], L::at(h.beta + q.tx * V, j));
+  }
+  for (; p < end; p += k.tile, load()) {
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
-      if (p + u * k.ty < q.p1) {
+      if (p + u * k.ty < end) {
 #pragma unroll
         for (int j = 0; j < J; ++j)
-          L::set(v[u], j, act<ACT>(fma(add(L::get(v[u], j), mu[j]), w[j], beta[j])));
+          L::set(v[u], j, act<ACT>(fma(L::get(v[u], j), w[j], beta[j])));
         store_pack<T, V>(y + (long long)(p + u * k.ty) * a.C, v[u]);
       }
   }
@@ -314,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) apply(Args a, Walk k, const float* s
 
 // Gradient, first pass: per channel of one chunk, sums of dz, dz n and n.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const float* stats,
+__global__ void __launch_bounds__(kThreads, kBlocksGrad) partial_grad(Args a, Walk k, const float* stats,
                                                          float* part) {
   using L = Lanes<T, V>;
   using F = typename L::F;
@@ -328,31 +353,44 @@ __global__ void __launch_bounds__(kThreads) partial_grad(Args a, Walk k, const f
   const Place q = place(a, k);
   channels<V>(sm.h, a, k, q, stats);
   __syncthreads();
-  F s1[J], s2[J], s3[J], mu[J], r[J], w[J], beta[J];
+  F s1[J], s2[J], s3[J], mu[J], r[J], w[J], beta[J];  // t = x + mu, n = t r, z = t w + beta
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     s1[j] = s2[j] = s3[j] = splat<F>(0.f);
     mu[j] = L::at(sm.h.mu + q.tx * V, j), r[j] = L::at(sm.h.r + q.tx * V, j);
-    w[j] = L::at(sm.h.w + q.tx * V, j), beta[j] = L::at(sm.h.beta + q.tx * V, j);
+    w[j] = mul(L::at(sm.h.w + q.tx * V, j), r[j]), beta[j] = L::at(sm.h.beta + q.tx * V, j);
   }
   __syncthreads();
   if (q.active) {
     const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
     const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
-#pragma unroll 2
-    for (int p = q.p0 + q.ty; p < q.p1; p += k.ty) {
-      const Pack<T, V> v = load_pack<T, V>(x + p * a.xp);
-      const Pack<T, V> d = load_pack<T, V>(dy + p * a.yp);
+    constexpr int U = kAhead / 2;
+    const int end = min(k.ntile, (q.chunk + 1) * k.per);
+    for (int i = q.chunk * k.per; i < end; ++i) {
+      const int p = i * k.tile + q.ty;
+      Pack<T, V> v[U], d[U];
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const F n = mul(add(L::get(v, j), mu[j]), r[j]);
-        const F dz = act_grad<ACT>(L::get(d, j), fma(n, w[j], beta[j]));
-        s1[j] = add(s1[j], dz);
-        s2[j] = fma(dz, n, s2[j]);
-        s3[j] = add(s3[j], n);
-      }
+      for (int u = 0; u < U; ++u)
+        if (p + u * k.ty < a.HW) {
+          v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+          d[u] = load_pack<T, V>(dy + (p + u * k.ty) * a.yp);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p + u * k.ty < a.HW) {
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const F t = add(L::get(v[u], j), mu[j]);
+            const F dz = act_grad<ACT>(L::get(d[u], j), fma(t, w[j], beta[j]));
+            s1[j] = add(s1[j], dz);
+            s2[j] = fma(dz, t, s2[j]);
+            s3[j] = add(s3[j], t);
+          }
+        }
     }
   }
+#pragma unroll
+  for (int j = 0; j < J; ++j) s2[j] = mul(s2[j], r[j]), s3[j] = mul(s3[j], r[j]);
   const int width = k.tx * V;
   if (q.ty < k.ty) {
     const int i = q.ty * width + q.tx * V;
@@ -418,31 +456,46 @@ __device__ __forceinline__ float warp_total(float v) {
   return v;
 }
 
-// Second pass: dx, and from the first chunk's blocks the shift's gradient.
+// Second pass: dx, and from a sample's first chunk the shift's gradient.
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kThreads) apply_grad(Args a, Walk k, const float* stats,
+__global__ void __launch_bounds__(kThreads, kBlocksGrad) apply_grad(Args a, Walk k, const float* stats,
                                                        const float* sums, void* dshift) {
   using L = Lanes<T, V>;
   using F = typename L::F;
-  constexpr int J = V / L::W;
+  constexpr int J = V / L::W, U = kAhead / 2;
   __shared__ Chan<V> h;
   __shared__ float A[kThreads * V], D[kThreads * V];  // minus the means, by channel
   pdl_trigger();
   pdl_wait();
   const Place q = place(a, k);
-  channels<V>(h, a, k, q, stats);
-  __syncthreads();
   const int c0 = (q.col - q.tx) * V, cols = min(k.tx * V, a.C - c0);
   const long long plane = (long long)a.B * a.C, bc = (long long)q.b * a.C;
+  const int end = q.active ? min(a.HW, (q.chunk + 1) * k.per * k.tile) : 0;
+  int p = q.chunk * k.per * k.tile + q.ty;
+  const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
+  const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
+  T* dx = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
+  Pack<T, V> v[U], d[U];
+  const auto load = [&] {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u * k.ty < end) {
+        v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+        d[u] = load_pack<T, V>(dy + (p + u * k.ty) * a.yp);
+      }
+  };
+  load();  // needs no sums
+  channels<V>(h, a, k, q, stats);
+  __syncthreads();
   const float inv = 1.f / ((float)a.HW * a.cpg);
   for (int g = c0 / a.cpg + (threadIdx.x >> 5); g <= (c0 + cols - 1) / a.cpg; g += kThreads / 32) {
     // The whole group's, also where the block has a part of its channels.
     const int lane = threadIdx.x & 31;
     float wa = 0.f, wd = 0.f;
     for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32) {
-      const float w = a.w ? load_param(a.w, a.wtype, c) : 1.f;
-      wa = fmaf(w, sums[bc + c], wa);
-      wd = fmaf(w, sums[plane + bc + c], wd);
+      const float wc = a.w ? load_param(a.w, a.wtype, c) : 1.f;
+      wa = fmaf(wc, sums[bc + c], wa);
+      wd = fmaf(wc, sums[plane + bc + c], wd);
     }
     wa = warp_total(wa) * inv;
     wd = warp_total(wd) * inv;
@@ -456,34 +509,24 @@ __global__ void __launch_bounds__(kThreads) apply_grad(Args a, Walk k, const flo
     }
   }
   __syncthreads();
-  if (!q.active) return;
-  F mu[J], r[J], w[J], beta[J], mA[J], mD[J];
+  // t = x + mu, z = t w + beta, dx = dz w - r A - t r^2 D (w holds r).
+  F mu[J], w[J], beta[J], ca[J], cd[J];
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    mu[j] = L::at(h.mu + q.tx * V, j), r[j] = L::at(h.r + q.tx * V, j);
-    w[j] = L::at(h.w + q.tx * V, j), beta[j] = L::at(h.beta + q.tx * V, j);
-    mA[j] = L::at(A + q.tx * V, j), mD[j] = L::at(D + q.tx * V, j);
+    const F r = L::at(h.r + q.tx * V, j);
+    mu[j] = L::at(h.mu + q.tx * V, j);
+    w[j] = mul(L::at(h.w + q.tx * V, j), r), beta[j] = L::at(h.beta + q.tx * V, j);
+    ca[j] = mul(L::at(A + q.tx * V, j), r), cd[j] = mul(mul(L::at(D + q.tx * V, j), r), r);
   }
-  const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
-  const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
-  T* dx = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
-  constexpr int U = kAhead / 2;
-  for (int p = q.p0 + q.ty; p < q.p1; p += U * k.ty) {
-    Pack<T, V> v[U], d[U];
+  for (; p < end; p += k.tile, load()) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (p + u * k.ty < q.p1) {
-        v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
-        d[u] = load_pack<T, V>(dy + (p + u * k.ty) * a.yp);
-      }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (p + u * k.ty < q.p1) {
+      if (p + u * k.ty < end) {
 #pragma unroll
         for (int j = 0; j < J; ++j) {
-          const F n = mul(add(L::get(v[u], j), mu[j]), r[j]);
-          const F dz = act_grad<ACT>(L::get(d[u], j), fma(n, w[j], beta[j]));
-          L::set(v[u], j, mul(r[j], fma(n, mD[j], fma(w[j], dz, mA[j]))));
+          const F t = add(L::get(v[u], j), mu[j]);
+          const F dz = act_grad<ACT>(L::get(d[u], j), fma(t, w[j], beta[j]));
+          L::set(v[u], j, fma(t, cd[j], fma(dz, w[j], ca[j])));
         }
         store_pack<T, V>(dx + (long long)(p + u * k.ty) * a.C, v[u]);
       }
@@ -688,8 +731,8 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
       stats[(long long)a.B * a.G + bg] = rstd;
     }
     for (int c = g * a.cpg + lane; c < (g + 1) * a.cpg; c += 32) {
-      mu[c] = sh[c] - m;
       wt[c] *= rstd;
+      bt[c] = fmaf(sh[c] - m, wt[c], bt[c]);
     }
   }
   cluster_arrive();  // this block has read its peers' parts
@@ -697,10 +740,10 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
   pass([&](auto has) {
 #pragma unroll
     for (int j = 0; j < V / W; ++j) {
-      const F m = L::at(mu + q.tx * V, j), w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
+      const F w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
 #pragma unroll
       for (int v = 0; v < NV; ++v)
-        if (has(v)) L::set(d[v], j, act<ACT>(fma(add(L::get(d[v], j), m), w, b)));
+        if (has(v)) L::set(d[v], j, act<ACT>(fma(L::get(d[v], j), w, b)));
     }
     T* y = static_cast<T*>(a.y) + ((long long)q.b * a.HW + q.p0 + q.ty) * a.C + q.c0 + q.tx * V;
     const long long step = (long long)k.ty * a.C;
@@ -765,21 +808,22 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
     float* mine = red + q.ty * width + q.tx * V;
 #pragma unroll
     for (int j = 0; j < V / W; ++j) {
+      // t = x + m, n = t r, z = t w + b
       const F m = L::at(mu + q.tx * V, j), r = L::at(rs + q.tx * V, j);
-      const F w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
+      const F w = mul(L::at(wt + q.tx * V, j), r), b = L::at(bt + q.tx * V, j);
       F s1 = splat<F>(0.f), s2 = s1, s3 = s1;
 #pragma unroll
       for (int v = 0; v < NV; ++v)
         if (has(v)) {
-          const F n = mul(add(L::get(d[v], j), m), r);
-          const F dz = act_grad<ACT>(L::get(e[v], j), fma(n, w, b));
+          const F t = add(L::get(d[v], j), m);
+          const F dz = act_grad<ACT>(L::get(e[v], j), fma(t, w, b));
           s1 = add(s1, dz);
-          s2 = fma(dz, n, s2);
-          s3 = add(s3, n);
+          s2 = fma(dz, t, s2);
+          s3 = add(s3, t);
         }
       L::put(mine, j, s1);
-      L::put(mine + rows, j, s2);
-      L::put(mine + 2 * rows, j, s3);
+      L::put(mine + rows, j, mul(s2, r));
+      L::put(mine + 2 * rows, j, mul(s3, r));
     }
   });
   __syncthreads();
@@ -838,14 +882,14 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
 #pragma unroll
     for (int j = 0; j < V / W; ++j) {
       const F m = L::at(mu + q.tx * V, j), r = L::at(rs + q.tx * V, j);
-      const F w = L::at(wt + q.tx * V, j), b = L::at(bt + q.tx * V, j);
-      const F A = L::at(ga + q.tx * V, j), D = L::at(gd + q.tx * V, j);
+      const F w = mul(L::at(wt + q.tx * V, j), r), b = L::at(bt + q.tx * V, j);
+      const F A = mul(L::at(ga + q.tx * V, j), r), D = mul(mul(L::at(gd + q.tx * V, j), r), r);
 #pragma unroll
       for (int v = 0; v < NV; ++v)
         if (has(v)) {
-          const F n = mul(add(L::get(d[v], j), m), r);
-          const F dz = act_grad<ACT>(L::get(e[v], j), fma(n, w, b));
-          L::set(d[v], j, mul(r, fma(n, D, fma(w, dz, A))));
+          const F t = add(L::get(d[v], j), m);
+          const F dz = act_grad<ACT>(L::get(e[v], j), fma(t, w, b));
+          L::set(d[v], j, fma(t, D, fma(dz, w, A)));
         }
     }
     T* y = static_cast<T*>(a.y) + ((long long)q.b * a.HW + q.p0 + q.ty) * a.C + q.c0 + q.tx * V;
@@ -876,13 +920,15 @@ Walk make_walk(int B, int HW, int C, int G, int V, bool grad) {
   k.tx = (k.cv + k.ncb - 1) / k.ncb;
   k.ty = kThreads / k.tx;
   k.cell = k.ncb == 1 || k.tx * V % cpg == 0 ? cpg : 1;
-  // One wave of blocks (by their registers), but at least `kAhead` pixels a thread.
-  long long chunks = (grad ? 2ll : 3ll) * device_sms() / ((long long)B * k.ncb);
+  const int U = grad ? kAhead / 2 : kAhead;
+  k.tile = U * k.ty;
+  k.ntile = (HW + k.tile - 1) / k.tile;
+  // One wave of blocks, by their registers.
+  long long chunks = (long long)(grad ? kBlocksGrad : kBlocksForward) * device_sms() / ((long long)B * k.ncb);
   if (chunks < 1) chunks = 1;
-  const long long most = (HW + (long long)kAhead * k.ty - 1) / ((long long)kAhead * k.ty);
-  if (chunks > most) chunks = most;
-  k.chunk = (int)((HW + chunks - 1) / chunks);
-  k.nchunk = (HW + k.chunk - 1) / k.chunk;
+  if (chunks > k.ntile) chunks = k.ntile;
+  k.per = (int)((k.ntile + chunks - 1) / chunks);
+  k.nchunk = (k.ntile + k.per - 1) / k.per;
   return k;
 }
 
