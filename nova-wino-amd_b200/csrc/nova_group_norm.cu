@@ -18,6 +18,7 @@
 // a mean far from zero costs no digits, and parts are joined as (count, mean,
 // sum of squared deviations), in 64 bits where whole samples meet.  Every sum
 // has a fixed order: results repeat bit for bit.
+#include <algorithm>
 #include <string>
 
 #include "../../include/nova_winograd.h"
@@ -952,8 +953,11 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
-// The resident form of a call, where its slabs fit.  `most` vectors a thread.
-bool make_slab(int B, int HW, int C, int G, int V, int most, int sms, Slab* best) {
+constexpr int kMostForward = 16, kMostGrad = 8;  // vectors a thread can hold
+
+// The resident form of a call, where it fits and pays.
+bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* best) {
+  const int most = grad ? kMostGrad : kMostForward;
   const int cpg = C / G;
   const int unit = V / gcd(cpg, V);  // groups whose channels fill whole vectors
   bool found = false;
@@ -974,15 +978,19 @@ bool make_slab(int B, int HW, int C, int G, int V, int most, int sms, Slab* best
         k.ty = (k.ppc + nv - 1) / nv;
         k.threads = (tx * k.ty + 31) / 32 * 32;
         if (k.threads > kSlabThreads) continue;
+        // The resident form pays while its blocks fit the SMs at once (twice at most in
+        // the gradient, whose streaming form has four launches): its phases do not
+        // overlap, so further waves cost it more than the second read it saves.
+        // Measured, FP16: 8x640x32x32 forward 12.5 us (streaming 20), 8x320x64x64 in
+        // two waves 27.7 us (streaming 22).
         const long long blocks = (long long)B * k.nblk * cs;
-        const int regs = nv * 4 * (most < 16 ? 2 : 1) + 64;
-        int per_sm = 65536 / (regs * k.threads);
-        if (per_sm > 32) per_sm = 32;
-        const long long waves = (blocks + (long long)sms * per_sm - 1) / ((long long)sms * per_sm);
-        const double row = (double)tx * 16;
-        const double bytes = (double)k.ppc * (row + 16);
-        const double busy = blocks < (long long)sms * per_sm ? (double)blocks / sms : per_sm;
-        const double cost = waves * ((busy < 1 ? 1 : busy) * bytes / 22.0 + 3500.0) + 200.0 * cs;
+        const int per_sm = std::min(32, 65536 / ((nv * 4 * (grad ? 2 : 1) + 64) * k.threads));
+        const long long room = (long long)sms * per_sm;
+        if (blocks > room * (grad ? 2 : 1)) continue;
+        // Bytes of the busiest SM, short rows counted with the sectors they touch, and
+        // the cluster's exchange.
+        const double cost = (double)((blocks + sms - 1) / sms) * k.ppc * (tx * 16 + 16) / 22.0 +
+                            150.0 * cs;
         if (!found || cost < best_cost) {
           found = true;
           best_cost = cost;
@@ -1021,8 +1029,6 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads,
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args2>(args)...);
 }
 
-constexpr int kMostForward = 16, kMostGrad = 8;  // vectors a thread can hold
-
 template <typename T, int V, int ACT>
 cudaError_t forward_resident(const Args& a, const Slab& k, float* stats, cudaStream_t s) {
   const unsigned grid = (unsigned)((long long)a.B * k.nblk * k.cs);
@@ -1054,7 +1060,7 @@ template <typename T, int V>
 cudaError_t forward(const Args& a, int act, float* stats, bool want_stats, unsigned char* ws,
                     cudaStream_t s) {
   Slab slab;
-  if (make_slab(a.B, a.HW, a.C, a.G, V, kMostForward, device_sms(), &slab))
+  if (make_slab(a.B, a.HW, a.C, a.G, V, false, device_sms(), &slab))
     return act == kSilu ? forward_resident<T, V, kSilu>(a, slab, want_stats ? stats : nullptr, s)
                         : forward_resident<T, V, kNone>(a, slab, want_stats ? stats : nullptr, s);
   const Walk k = make_walk(a.B, a.HW, a.C, a.G, V, false);
@@ -1081,7 +1087,7 @@ cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, v
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
   cudaError_t e;
   Slab slab;
-  if (make_slab(a.B, a.HW, a.C, a.G, V, kMostGrad, device_sms(), &slab)) {
+  if (make_slab(a.B, a.HW, a.C, a.G, V, true, device_sms(), &slab)) {
     e = grad_resident<T, V, ACT>(a, slab, stats, sums, dshift, s);
     if (e == cudaSuccess && (dw || dbeta))
       e = launch_pdl(kPdlInput, param_grad, dim3((a.C + 127) / 128), dim3(128), 0, s, a,
