@@ -1247,7 +1247,18 @@ def run_unet_model(args):
     x = x.contiguous(memory_format=torch.channels_last)
     ms_cl, out_cl = timed(model)
     ms_ref_cl, out_ref_cl = timed(ref)
+    # The same, with the layers between the convolutions on the framework's operators.
+    U.use_nova_ops(model)
+    ms_ops, out_ops = timed(model)
+    U.use_nova_ops(model, False)
     channels_last = {
+        "nova_ops": {
+            "latents_s": world * args.batch * args.steps / (ms_ops / 1e3),
+            "ms_per_step": ms_ops / args.steps,
+            "output_finite": bool(torch.isfinite(out_ops).all().item()),
+            "output_rel_diff": float(((out_ops.float() - out_cl.float()).norm() /
+                                      out_cl.float().norm()).item()),
+        },
         "latents_s": world * args.batch * args.steps / (ms_cl / 1e3),
         "ms_per_step": ms_cl / args.steps,
         "cudnn_same_model_latents_s": world * args.batch * args.steps / (ms_ref_cl / 1e3),

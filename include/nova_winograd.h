@@ -203,10 +203,13 @@ enum { NOVA_ACT_NONE = 0, NOVA_ACT_SILU = 1 };
  * each may be NULL (1 and 0).  shift: [batch][C] of type shift_dtype, or NULL.
  * stats: float[2][batch][groups], mean and 1/sqrt(var + eps), for the gradient;
  * NULL where it is not wanted.  The caller passes a 256-byte aligned workspace
- * of nova_group_norm_workspace_bytes() bytes; calls that overlap need one each.
+ * of nova_group_norm_workspace_bytes() bytes (NULL where that is 0); calls that
+ * overlap need one each.  aligned: all tensors and their strides are multiples of
+ * 16 bytes (0 is always safe, and takes the narrow kernels' workspace).
  * Allocates nothing, never synchronizes, runs on `stream`; returns a NOVA_*
  * status. */
-long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups, int grad);
+long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups, int dtype,
+                                          int aligned, int grad);
 int nova_group_norm_v2(const void* d_input, const void* d_weight, const void* d_bias,
                        const void* d_shift, void* d_output, void* d_stats, void* d_workspace,
                        long long workspace_bytes, int batch, int pixels, int C, int groups,
@@ -235,22 +238,28 @@ int nova_group_norm_grad_v2(const void* d_input, const void* d_grad_output, cons
  * k (grad_k, grad_v).  mask: [batch][keys]; a key with false, or with an additive
  * -inf, takes no part whatever k and v hold there, and a query without keys gets
  * zeros.  lse: float[batch][heads][queries], the base-2 logarithm of the softmax's
- * denominator, for the gradient; NULL where it is not wanted.  Workspace, stream
- * and status as above (a workspace of 0 bytes may be NULL). */
+ * denominator, for the gradient; NULL where it is not wanted.  low: like output, what
+ * its rounding left off; the gradient wants it, with output, for more than 128 keys
+ * (80 where head_dim > 128), else both may be NULL there.  Workspace, stream and
+ * status as above (a workspace of 0 bytes may be NULL).
+ * nova_cross_attention_status synchronizes the current device and returns
+ * NOVA_ERR_DEVICE_TIMEOUT if a kernel's bounded wait expired there since the last
+ * call (and clears it): outputs of such a call are not to be used. */
 long long nova_cross_attention_workspace_bytes(int batch, int queries, int keys, int heads,
                                                int head_dim, int grad);
 int nova_cross_attention_v2(const void* d_q, const void* d_k, const void* d_v, const void* d_mask,
-                            void* d_output, void* d_lse, void* d_workspace,
+                            void* d_output, void* d_low, void* d_lse, void* d_workspace,
                             long long workspace_bytes, int batch, int queries, int keys,
                             int heads, int head_dim, const long long* strides, int dtype,
                             int mask_type, float scale, void* stream);
 int nova_cross_attention_grad_v2(const void* d_q, const void* d_k, const void* d_v,
-                                 const void* d_mask, const void* d_output,
+                                 const void* d_mask, const void* d_output, const void* d_low,
                                  const void* d_grad_output, const void* d_lse, void* d_grad_q,
                                  void* d_grad_k, void* d_grad_v, void* d_workspace,
                                  long long workspace_bytes, int batch, int queries, int keys,
                                  int heads, int head_dim, const long long* strides, int dtype,
                                  int mask_type, float scale, void* stream);
+int nova_cross_attention_status(void);
 
 /* Library version string. */
 const char* nova_version(void);

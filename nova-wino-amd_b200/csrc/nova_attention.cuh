@@ -23,6 +23,7 @@ struct Args {
   const void *q, *k, *v, *dout, *mask;
   const float* lse_in;
   void* out;   // o
+  void* low;   // what the rounding of o left off, or null
   float* lse;  // [B][H][Nq], base 2; minus infinity for a query without keys
   void *dq, *dk, *dv;
   const float* delta;  // [B][H][Nq]: sum(p dp)
@@ -65,6 +66,14 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  else
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
 // Bounded wait: false when the phase did not complete within kWaitLimitNs or another
@@ -207,15 +216,16 @@ __device__ __forceinline__ uint32_t sw128(int row, int piece) {
   return (uint32_t)row * 128u + (uint32_t)((piece ^ (row & 7)) << 4);
 }
 
-int device_sms();
-
 // Forward (nova_attention_fwd.cu): workspace and launch.
 long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D);
 cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why);
+cudaError_t forward_status(int* status);  // of the current device; clears it
 
 // Gradient (nova_attention_bwd.cu).
 long long backward_workspace_bytes(int B, int Nq, int Nk, int H, int D);
 cudaError_t launch_backward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why);
+bool backward_reads_output(int Nk, int D);
+cudaError_t backward_status(int* status);
 
 }  // namespace xattn
 }  // namespace nova

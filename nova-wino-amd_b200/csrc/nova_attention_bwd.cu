@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// delta = dO . O: a warp for a query.
+// delta = dO . O, with what the rounding of O left off: O's own rounding would enter every
+// dS of its row (BF16, 333 keys: dQ and dK 1.1 times further off).  A warp for a query.
 template <typename T>
 __global__ void __launch_bounds__(128) row_delta(const __grid_constant__ Args a, float* delta) {
   pdl_trigger();
@@ -509,12 +510,14 @@ __global__ void __launch_bounds__(128) row_delta(const __grid_constant__ Args a,
   const int n = row % a.Nq, h = row / a.Nq % a.H;
   const long long b = row / a.Nq / a.H;
   const T* o = static_cast<const T*>(a.out) + ((b * a.Nq + n) * a.H + h) * a.D;
+  const T* lo = static_cast<const T*>(a.low) + ((b * a.Nq + n) * a.H + h) * a.D;
   const T* g = static_cast<const T*>(a.dout) + b * a.dos.b + n * a.dos.n + h * a.dos.h;
   float t = 0.f;
   for (int i = lane * 8; i < a.D; i += 256) {
-    const Pack<T, 8> x = load_pack<T, 8>(o + i), y = load_pack<T, 8>(g + i);
+    const Pack<T, 8> x = load_pack<T, 8>(o + i), z = load_pack<T, 8>(lo + i),
+                     y = load_pack<T, 8>(g + i);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t = fmaf(to_f32(x.e[e]), to_f32(y.e[e]), t);
+    for (int e = 0; e < 8; ++e) t = fmaf(to_f32(x.e[e]) + to_f32(z.e[e]), to_f32(y.e[e]), t);
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(~0u, t, s);
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(256) join_parts(const float* __restrict__ dk,
 int up(int v, int to) { return (v + to - 1) / to * to; }
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-constexpr size_t kSmemMax = 226 * 1024;
+constexpr size_t kSmemMax = 224 * 1024;  // beside the static part
 
 size_t smem_of(const BwdParams& p, int mode, int stages) {
   const size_t fix = mode == kQueries ? p.q_bytes : p.k_bytes;
@@ -551,12 +554,14 @@ size_t smem_of(const BwdParams& p, int mode, int stages) {
   return 2 * fix + 2 * stages * walk + (mode == kQueries ? 1 : 2) * 2ull * kRows * 128 + 1024;
 }
 
+// Keys of a tile.  Three-block heads: 80 leave shared memory room for P and dS.
+int most_keys(int D) { return D > 128 ? 80 : 128; }
+
 void plan(BwdParams* p, int sms) {
   const Args& a = p->a;
   p->DB = (a.D + 63) / 64;
   p->DP = up(a.D, 16);
-  // Three-block heads: 80 keys a tile leave shared memory room for P and dS.
-  const int most = p->DB > 2 ? 80 : 128;
+  const int most = most_keys(a.D);
   p->nkt = (a.Nk + most - 1) / most;
   p->KT = up((a.Nk + p->nkt - 1) / p->nkt, 16);
   p->nkt = (a.Nk + p->KT - 1) / p->KT;
@@ -597,9 +602,9 @@ size_t arrange(BwdParams* p, int mode) {
 
 template <typename T, bool MASK, int MODE>
 cudaError_t run_mode(BwdParams p, const CUtensorMap* m, cudaStream_t s) {
+  static std::atomic<unsigned long long> allowed{0};
   const size_t smem = arrange(&p, MODE);
-  cudaError_t e = cudaFuncSetAttribute(backward_tc<T, MASK, MODE>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem(backward_tc<T, MASK, MODE>, &allowed, kSmemMax);
   if (e != cudaSuccess) return e;
   const long long heads = (long long)p.a.B * p.a.H;
   const long long grid = MODE == kQueries ? heads * p.qtiles : heads * p.nkt * p.splits;
@@ -639,6 +644,14 @@ long long backward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
   size_t total = p.nkt > 1 ? align256((size_t)B * H * Nq * 4) : 0;
   if (p.splits > 1) total += 2 * align256(n * p.splits);
   return (long long)total;
+}
+
+bool backward_reads_output(int Nk, int D) { return Nk > most_keys(D); }
+
+cudaError_t backward_status(int* status) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_status, sizeof(int));
+  const int zero = 0;
+  return e == cudaSuccess ? cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) : e;
 }
 
 cudaError_t launch_backward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why) {

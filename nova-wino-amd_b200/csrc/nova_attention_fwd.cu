@@ -11,13 +11,16 @@
 //   O += P V       P from tensor memory; V as it lies, its head index contiguous
 //
 // The keys come in `nkt` tiles of `KT` (a multiple of 16, at most 128).  With one
-// tile (77 text tokens) K and V stay in shared memory while the block walks over
-// its share of the head's queries: the next queries land as soon as S has been formed,
-// and the next S is formed while finished rows leave; with more, K and V run through two stages and O keeps its place, its
-// scale renewed only when a row's maximum has risen by more than 2^kLazy.  Few
-// queries against many keys: the keys are split over blocks, which leave partial
-// rows in the workspace for a second kernel to join.
+// tile (77 text tokens) the blocks share all heads' query tiles evenly, in a row; K and
+// V stay in shared memory while the head does, the next queries land as soon as S has
+// been formed, and the next S is formed while finished rows leave.  With more, K and V
+// run through two stages and O keeps its place, its scale renewed only when a row's
+// maximum has risen by more than 2^kLazy.  Too few queries for the SMs against many
+// keys: the keys are split over blocks, which leave partial rows in the workspace for a
+// second kernel to join.
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "nova_attention.cuh"
 
@@ -30,6 +33,7 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kThreads = kRows + 32;  // a thread for a row, and a warp that starts the work
+constexpr int kBlocks = 3;  // on an SM, by their registers
 constexpr float kLazy = 4.f;
 constexpr int kHeld = 80;  // scores that a thread can hold with three blocks on an SM
 
@@ -38,8 +42,10 @@ struct FwdParams {
   Pick qp, kp, vp, op;
   int KT, nkt;       // keys per tile, tiles
   int DB, DP;        // 64-element blocks and padded width of a head
-  int qtiles, chunk; // query tiles of a head, tiles per block
-  int nchunk;
+  int qtiles;        // query tiles of a head
+  long long total;   // query tiles of all heads, which the blocks share evenly
+  int blocks;        // for each key split
+  bool walks;        // a block may have more than one
   int splits, per;   // key splits, tiles per split
   int kstages;           // of K and V
   uint32_t tmem_cols, o_col;
@@ -51,7 +57,7 @@ struct FwdParams {
 __device__ int g_status;
 
 template <typename T, bool MASK, bool ONE>
-__global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant__ CUtensorMap mq,
+__global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_constant__ CUtensorMap mq,
                                                        const __grid_constant__ CUtensorMap mk,
                                                        const __grid_constant__ CUtensorMap mv,
                                                        const __grid_constant__ CUtensorMap mo,
@@ -67,7 +73,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
   const int warp = __shfl_sync(~0u, tid >> 5, 0);  // the same for the warp, and known to be
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   // Q, the finished rows (over Q where a block has one query tile), K, V.
-  const uint32_t sq = base, so = p.chunk > 1 ? sq + p.q_bytes : sq;
+  const uint32_t sq = base, so = p.walks ? sq + p.q_bytes : sq;
   const uint32_t sk = so + p.q_bytes, sv = sk + p.kstages * p.k_bytes;
   const uint32_t bq = smem_u32(&bars[0]), bkv = bq + 8, bs = bq + 24, bo = bq + 32, bm = bq + 40,
                  bp = bq + 48, br = bq + 56;
@@ -93,12 +99,20 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
   unsigned id = blockIdx.x;
   const int split = id % p.splits;
   id /= p.splits;
-  const int ch = id % p.nchunk;
-  id /= p.nchunk;
-  const int h = id % p.a.H, b = id / p.a.H;
-  const int t0 = ch * p.chunk, tiles = min(p.qtiles, t0 + p.chunk) - t0;
+  // Query tiles first, first + 1, ... of all heads in a row, and this split's key tiles.
+  const int first = (int)((long long)id * p.total / p.blocks);
+  const int tiles = (int)((id + 1ll) * p.total / p.blocks) - first;
   const int k0 = split * p.per, nk = min(p.nkt, k0 + p.per) - k0;
-  const bool resident = nk == 1;  // K and V stay
+  const bool resident = nk == 1;  // K and V stay while the head does
+  const int head0 = first / p.qtiles;
+  struct Spot {
+    int b, h, n;  // sample, head, first query
+    int turn;     // heads before this one in the block's walk
+  };
+  const auto spot = [&](int t) {
+    const int g = first + t, head = g / p.qtiles, b = head / p.a.H;
+    return Spot{b, head - b * p.a.H, (g - head * p.qtiles) * kRows, head - head0};
+  };
   const auto wait = [&](uint32_t bar, uint32_t parity, int code) {
     return wait_phase(bar, parity & 1, &abort_flag, &g_status, code);
   };
@@ -108,14 +122,17 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
     const bool one = elect_one();
     const auto load_q = [&](int t) {
       if (!one) return;
+      const Spot at = spot(t);
       mbar_expect_tx(bq, p.q_bytes);
       for (int d = 0; d < p.DB; ++d)
-        tma_load_4d(sq + d * (kRows * 128), &mq, d * 64, (t0 + t) * kRows, h * p.qp.h, b * p.qp.b,
-                    bq);
+        tma_load_4d(sq + d * (kRows * 128), &mq, d * 64, at.n, at.h * p.qp.h, at.b * p.qp.b, bq);
     };
-    const auto load_kv = [&](int j) {
+    // The i-th pair of K and V tiles that the block goes through: its head's key tiles,
+    // or one for each head.
+    const auto load_kv = [&](int i) {
       if (!one) return;
-      const int stage = j % p.kstages;
+      const int head = head0 + (resident ? i : 0), h = head % p.a.H, b = head / p.a.H;
+      const int j = resident ? 0 : i, stage = i % p.kstages;
       const uint32_t bar = bkv + 8u * stage, at = stage * p.k_bytes;
       mbar_expect_tx(bar, 2 * p.k_bytes);
       for (int d = 0; d < p.DB; ++d)
@@ -129,9 +146,9 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
     const uint32_t idesc_o = instr_desc(kBf16, kRows, p.DP, false, true);
     const int nd = p.DP / 16, nc = p.KT / 16;
     const uint64_t qd = smem_desc_sw128(sq);
-    // S of the tile in Q and key tile j.
-    const auto scores = [&](int j) {
-      const uint64_t kd = smem_desc_sw128(sk + (j % p.kstages) * p.k_bytes);
+    // S of the tile in Q and the i-th K.
+    const auto scores = [&](int i) {
+      const uint64_t kd = smem_desc_sw128(sk + (i % p.kstages) * p.k_bytes);
       tc_fence_after();
       if (one) {
 #pragma unroll
@@ -141,8 +158,8 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
         umma_commit(bs);
       }
     };
-    const auto products = [&](int j) {
-      const uint64_t vd = smem_desc_mn(sv + (j % p.kstages) * p.k_bytes, p.KT * 128);
+    const auto products = [&](int i, int j) {
+      const uint64_t vd = smem_desc_mn(sv + (i % p.kstages) * p.k_bytes, p.KT * 128);
       tc_fence_after();
       if (one) {
 #pragma unroll
@@ -152,7 +169,8 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
         umma_commit(bo);
       }
     };
-    int qn = 1, kn = min(nk, p.kstages);  // copies started
+    const int pairs = resident ? spot(tiles - 1).turn + 1 : nk;
+    int qn = 1, kn = min(pairs, p.kstages);  // copies started
     load_q(0);
     for (int j = 0; j < kn; ++j) load_kv(j);
     bool ok = wait(bq, 0, kDevTimeoutProducer) && wait(bkv, 0, kDevTimeoutProducer);
@@ -172,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
         // there, which happens behind this product.
         if (one) bulk_wait_read_all();
         if (!(ok = __all_sync(~0u, ok))) break;
-        products(j);
+        products(resident ? spot(t).turn : j, j);
         if (j + 1 < nk) {
           // Behind the product that reads P, in the same order.
           ok = __all_sync(~0u, wait(bkv + 8u * ((j + 1) % p.kstages), (j + 1) / p.kstages,
@@ -188,14 +206,21 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
       }
       ok = ok && wait(br, t, kDevTimeoutEpilogue);
       if (!(ok = __all_sync(~0u, ok))) break;
+      const Spot at = spot(t);
       if (t + 1 < tiles) {
-        ok = __all_sync(~0u, wait(bq, t + 1, kDevTimeoutProducer));
-        if (!ok) break;
-        scores(0);
+        const int turn = spot(t + 1).turn;
+        ok = wait(bq, t + 1, kDevTimeoutProducer);
+        if (turn != at.turn) {
+          // The next head: the products with the last one's K and V are there.
+          if (kn < pairs && ok) load_kv(kn++);
+          ok = ok && wait(bkv + 8u * (turn % p.kstages), turn / p.kstages, kDevTimeoutProducer);
+        }
+        if (!(ok = __all_sync(~0u, ok))) break;
+        scores(turn);
       }
       if (one && p.splits == 1) {
         for (int d = 0; d < p.DB; ++d)
-          tma_store_4d(&mo, so + d * (kRows * 128), d * 64, (t0 + t) * kRows, h, b);
+          tma_store_4d(&mo, so + d * (kRows * 128), d * 64, at.n, at.h, at.b);
         bulk_commit();
       }
     }
@@ -216,13 +241,15 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const float c = p.a.scale * kLog2e;
     const int chunks = p.KT / 16;
-    int step = 0;
+    int step = 0, turn_seen = -1;
     bool ok = true;
     for (int t = 0; t < tiles && ok; ++t) {
+      const Spot at = spot(t);
+      const int b = at.b, h = at.h;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nk; ++j, ++step) {
         const int key0 = (k0 + j) * p.KT, keys = min(p.KT, p.a.Nk - key0);
-        if (MASK && (t == 0 || !resident)) {
+        if (MASK && (at.turn != turn_seen || !resident)) {
           // The bias of this tile's keys; the rows of V behind a masked key are cleared:
           // P is zero there, and zero times infinity is not.
           float x = -INFINITY;
@@ -230,8 +257,9 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
           // The scores before have been read by everyone who reads the old bias.
           if (j > 0) ok = wait(bo, step - 1, kDevTimeoutMma);
           bias[tid] = in ? x : -INFINITY;
-          const int stage = j % p.kstages;
-          ok = ok && wait(bkv + 8u * stage, j / p.kstages, kDevTimeoutProducer);
+          const int pair = resident ? at.turn : j, stage = pair % p.kstages;
+          turn_seen = at.turn;
+          ok = ok && wait(bkv + 8u * stage, pair / p.kstages, kDevTimeoutProducer);
           if (ok && !in && tid < keys) {
             for (int d = 0; d < p.DB; ++d)
               for (int i = 0; i < 8; ++i)
@@ -240,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(bm);
-          ok = ok && wait(bm, step, kDevTimeoutEpilogue);
+          ok = ok && wait(bm, pair, kDevTimeoutEpilogue);
         }
         ok = ok && wait(bs, step, kDevTimeoutMma);
         __syncwarp();
@@ -379,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
       tc_fence_after();
 
       // O / sum.
-      const int row = (t0 + t) * kRows + tid;
+      const int row = at.n + tid;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const float lse = l == 0.f ? -INFINITY : m + log2f(l);
       const long long lrow = ((long long)b * p.a.H + h) * p.a.Nq + row;
@@ -414,6 +442,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
 #pragma unroll 1
         for (int i = 0; i < p.DP / 16; i += 2) {
           uint32_t o[2][16];
+          __syncwarp();
           tmem_ld16_issue(lanes + p.o_col + 16u * i, o[0]);
           if (i + 1 < p.DP / 16) tmem_ld16_issue(lanes + p.o_col + 16u * (i + 1), o[1]);
           tmem_wait_ld();
@@ -421,6 +450,31 @@ __global__ void __launch_bounds__(kThreads, 3) forward_tc(const __grid_constant_
           if (i + 1 < p.DP / 16) put_rows(o[1], i + 1);
         }
         if (p.a.lse && row < p.a.Nq) p.a.lse[lrow] = lse;
+        if (p.a.low) {
+          T* low = static_cast<T*>(p.a.low) +
+                   (((long long)b * p.a.Nq + row) * p.a.H + h) * (long long)p.a.D;
+#pragma unroll 1
+          for (int i = 0; i < p.DP / 16; ++i) {
+            uint32_t o[16];
+            __syncwarp();
+            tmem_ld16_issue(lanes + p.o_col + 16u * i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              if (row < p.a.Nq && 16 * i + e < p.a.D) {
+                uint32_t w[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  const float x = __uint_as_float(o[e + 2 * u]) * inv,
+                              y = __uint_as_float(o[e + 2 * u + 1]) * inv;
+                  const float2 r = unpack2<T>(pack2<T>(x, y));
+                  w[u] = pack2<T>(x - r.x, y - r.y);
+                }
+                *reinterpret_cast<uint4*>(low + 16 * i + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+          }
+          __syncwarp();
+        }
         fence_async_smem();
       }
       tc_fence_before();
@@ -597,7 +651,9 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
       p.part_o[(long long)split * a.B * a.Nq * a.H * a.D + off] = v;
       if (d == 0) p.part_lse[(long long)split * a.B * a.H * a.Nq + row] = lse;
     } else {
-      static_cast<T*>(a.out)[off] = from_f32<T>(v);
+      const T r = from_f32<T>(v);
+      static_cast<T*>(a.out)[off] = r;
+      if (a.low) static_cast<T*>(a.low)[off] = from_f32<T>(v - to_f32(r));
       if (d == 0 && a.lse) a.lse[row] = lse;
     }
   }
@@ -630,8 +686,12 @@ __global__ void __launch_bounds__(128) join_splits(const __grid_constant__ FwdPa
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int i = 0; i < kMaxD / 32; ++i)
-    if (lane + 32 * i < p.a.D)
-      static_cast<T*>(p.a.out)[off + lane + 32 * i] = from_f32<T>(acc[i] * inv);
+    if (lane + 32 * i < p.a.D) {
+      const float v = acc[i] * inv;
+      const T r = from_f32<T>(v);
+      static_cast<T*>(p.a.out)[off + lane + 32 * i] = r;
+      if (p.a.low) static_cast<T*>(p.a.low)[off + lane + 32 * i] = from_f32<T>(v - to_f32(r));
+    }
   if (p.a.lse && lane == 0) p.a.lse[row] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
@@ -656,13 +716,6 @@ EncodeTiledFn encode_fn() {
 int up(int v, int to) { return (v + to - 1) / to * to; }
 
 }  // namespace
-
-int device_sms() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return sms;
-}
 
 bool encode_tile4(CUtensorMap* map, Pick* pick, const void* ptr, const Strides& s, int B, int N,
                   int H, int D, int rows, bool bf16) {
@@ -741,15 +794,14 @@ void plan(FwdParams* p, int sms) {
   p->nkt = (a.Nk + p->KT - 1) / p->KT;
   p->DP = up(a.D, 16);
   p->qtiles = (a.Nq + kRows - 1) / kRows;
-  const long long heads = (long long)a.B * a.H;
+  p->total = (long long)a.B * a.H * p->qtiles;
   p->splits = 1;
-  if (p->nkt > 1 && heads * p->qtiles < 2 * sms) {
-    long long want = (2ll * sms + heads * p->qtiles - 1) / (heads * p->qtiles);
-    if (want > p->nkt) want = p->nkt;
+  p->per = p->nkt;
+  if (p->nkt > 1 && p->total < sms) {
+    const long long want = std::min((long long)p->nkt, kBlocks * sms / p->total);
     p->per = (int)((p->nkt + want - 1) / want);
     p->splits = (p->nkt + p->per - 1) / p->per;
   }
-  if (p->splits == 1) p->per = p->nkt;
   p->q_bytes = (uint32_t)p->DB * kRows * 128;
   p->k_bytes = (uint32_t)p->DB * p->KT * 128;
   const bool one = p->per == 1;
@@ -757,22 +809,23 @@ void plan(FwdParams* p, int sms) {
   p->o_col = (uint32_t)(one ? up(p->KT / 2, 16) : p->KT);
   const int cols = p->KT > (int)p->o_col + p->DP ? p->KT : (int)p->o_col + p->DP;
   p->tmem_cols = cols <= 32 ? 32 : cols <= 64 ? 64 : cols <= 128 ? 128 : cols <= 256 ? 256 : 512;
-  p->kstages = one ? 1 : 2;
-  // Blocks of the GPU at a time decide how many query tiles a block walks over.
-  const size_t smem = (one ? 2ull : 1ull) * p->q_bytes + 2ull * p->kstages * p->k_bytes + 1024;
-  long long per_sm = (long long)(kSmemMax / smem);
-  if (per_sm > 512 / p->tmem_cols) per_sm = 512 / p->tmem_cols;
-  if (per_sm < 1) per_sm = 1;
-  if (per_sm > 3) per_sm = 3;  // by its registers
-  long long nchunk = one ? (per_sm * sms) / (heads * p->splits) : p->qtiles;
-  if (nchunk < 1) nchunk = 1;
-  if (nchunk > p->qtiles) nchunk = p->qtiles;
-  p->chunk = (int)((p->qtiles + nchunk - 1) / nchunk);
-  p->nchunk = (p->qtiles + p->chunk - 1) / p->chunk;
+  // One tile: the next head's K and V land beside this one's where that costs no block
+  // of an SM.
+  const auto smem = [&](int stages) {
+    return (one ? 2ull : 1ull) * p->q_bytes + 2ull * stages * p->k_bytes + 1024;
+  };
+  const auto per_sm = [&](int stages) {
+    return std::min((long long)(kSmemMax / smem(stages)),
+                    std::min((long long)kBlocks, 512ll / p->tmem_cols));
+  };
+  p->kstages = one && per_sm(2) < per_sm(1) ? 1 : 2;
+  long long blocks = one ? std::max(1ll, per_sm(p->kstages)) * sms / p->splits : p->total;
+  p->blocks = (int)std::max(1ll, std::min(blocks, p->total));
+  p->walks = p->blocks < p->total;
 }
 
 size_t smem_bytes(const FwdParams& p) {
-  size_t n = (p.chunk > 1 ? 2ull : 1ull) * p.q_bytes + 2ull * p.kstages * p.k_bytes + 1024;
+  size_t n = (p.walks ? 2ull : 1ull) * p.q_bytes + 2ull * p.kstages * p.k_bytes + 1024;
   // No more blocks on an SM than its tensor memory holds.
   const size_t least = kSmemMax / (512 / p.tmem_cols + 1) + 1;
   return n > least ? n : least;
@@ -782,11 +835,11 @@ size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
 template <typename T, bool MASK, bool ONE>
 cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
+  static std::atomic<unsigned long long> allowed{0};
   const size_t smem = smem_bytes(p);
-  cudaError_t e = cudaFuncSetAttribute(forward_tc<T, MASK, ONE>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = allow_smem(forward_tc<T, MASK, ONE>, &allowed, kSmemMax);
   if (e != cudaSuccess) return e;
-  const unsigned grid = (unsigned)((long long)p.a.B * p.a.H * p.nchunk * p.splits);
+  const unsigned grid = (unsigned)((long long)p.blocks * p.splits);
   e = launch_pdl(kPdlInput, forward_tc<T, MASK, ONE>, dim3(grid), dim3(kThreads), smem, s, m[0], m[1],
                  m[2], m[3], p);
   if (e == cudaSuccess && p.splits > 1) {
@@ -806,6 +859,12 @@ long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
   if (p.splits == 1) return 0;
   const size_t rows = (size_t)B * H * Nq * p.splits;
   return (long long)(align256(rows * D * 4) + align256(rows * 4));
+}
+
+cudaError_t forward_status(int* status) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_status, sizeof(int));
+  const int zero = 0;
+  return e == cudaSuccess ? cudaMemcpyToSymbol(g_status, &zero, sizeof(int)) : e;
 }
 
 cudaError_t launch_forward(const Args& a, bool bf16, void* ws, cudaStream_t s, const char** why) {

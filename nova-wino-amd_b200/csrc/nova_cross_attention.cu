@@ -42,7 +42,8 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
   if (!fine(a.q, a.qs) || !fine(a.k, a.ks) || !fine(a.v, a.vs) ||
       (grad && !fine(a.dout, a.dos)))
     return bad("rows must start on 16 bytes and no stride may be negative, none of the tokens zero");
-  if (grad ? !aligned16(a.dq) || !aligned16(a.dk) || !aligned16(a.dv) : !aligned16(a.out))
+  if (grad ? !aligned16(a.dq) || !aligned16(a.dk) || !aligned16(a.dv)
+           : !aligned16(a.out) || !aligned16(a.low))
     return bad("outputs must be 16-byte aligned");
   if (a.mb < 0 || a.mn < 0) return bad("negative mask stride");
   const long long rows = (long long)a.B * a.H * (a.Nq > a.Nk ? a.Nq : a.Nk);
@@ -75,7 +76,7 @@ NOVA_EXPORT long long nova_cross_attention_workspace_bytes(int batch, int querie
 }
 
 NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const void* d_v,
-                                        const void* d_mask, void* d_output, void* d_lse,
+                                        const void* d_mask, void* d_output, void* d_low, void* d_lse,
                                         void* d_workspace, long long ws_bytes, int batch,
                                         int queries, int keys, int heads, int head_dim,
                                         const long long* strides, int dtype, int mask_type,
@@ -85,6 +86,7 @@ NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const 
   if (!strides) return record_error(NOVA_ERR_INVALID_ARGUMENT, "cross_attention: null strides");
   Args a{};
   a.q = d_q, a.k = d_k, a.v = d_v, a.mask = d_mask, a.out = d_output;
+  a.low = d_low;
   a.lse = static_cast<float*>(d_lse);
   const long long* t = strides;
   a.qs = {t[0], t[1], t[2]}, a.ks = {t[3], t[4], t[5]}, a.vs = {t[6], t[7], t[8]};
@@ -105,7 +107,7 @@ NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const 
 
 NOVA_EXPORT int nova_cross_attention_grad_v2(
     const void* d_q, const void* d_k, const void* d_v, const void* d_mask, const void* d_output,
-    const void* d_grad_output, const void* d_lse, void* d_grad_q, void* d_grad_k, void* d_grad_v,
+    const void* d_low, const void* d_grad_output, const void* d_lse, void* d_grad_q, void* d_grad_k, void* d_grad_v,
     void* d_workspace, long long ws_bytes, int batch, int queries, int keys, int heads,
     int head_dim, const long long* strides, int dtype, int mask_type, float scale,
     void* stream) try {
@@ -115,6 +117,7 @@ NOVA_EXPORT int nova_cross_attention_grad_v2(
   Args a{};
   a.q = d_q, a.k = d_k, a.v = d_v, a.mask = d_mask, a.dout = d_grad_output;
   a.out = const_cast<void*>(d_output);
+  a.low = const_cast<void*>(d_low);
   a.lse_in = static_cast<const float*>(d_lse);
   a.dq = d_grad_q, a.dk = d_grad_k, a.dv = d_grad_v;
   const long long* t = strides;
@@ -125,8 +128,10 @@ NOVA_EXPORT int nova_cross_attention_grad_v2(
   a.mask_kind = mask_type, a.scale = scale;
   if (const int rc = check("cross_attention_grad", a, dtype, d_workspace, ws_bytes, true))
     return rc;
-  if (!a.out || !aligned16(a.out))
-    return record_error(NOVA_ERR_INVALID_ARGUMENT, "cross_attention_grad: bad output pointer");
+  if (backward_reads_output(keys, head_dim) &&
+      (!a.out || !a.low || !aligned16(a.out) || !aligned16(a.low)))
+    return record_error(NOVA_ERR_INVALID_ARGUMENT,
+                        "cross_attention_grad: these keys want output and low, 16-byte aligned");
   const OnDeviceOf device(d_q);
   if (device.status() != cudaSuccess) return done("cross_attention_grad: q", device.status());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -134,6 +139,22 @@ NOVA_EXPORT int nova_cross_attention_grad_v2(
   const cudaError_t e = launch_backward(a, dtype == kBF16, d_workspace, s, &why);
   if (why) return record_error(NOVA_ERR_CUDA, std::string("cross_attention_grad: ") + why);
   return done("cross_attention_grad", e);
+} catch (...) {
+  return NOVA_ERR_ALLOC;
+}
+
+NOVA_EXPORT int nova_cross_attention_status(void) try {
+  using namespace nova;
+  using namespace nova::xattn;
+  cudaError_t e = cudaDeviceSynchronize();
+  int fwd = 0, bwd = 0;
+  if (e == cudaSuccess) e = forward_status(&fwd);
+  if (e == cudaSuccess) e = backward_status(&bwd);
+  if (e != cudaSuccess) return done("cross_attention_status", e);
+  if (fwd || bwd)
+    return record_error(NOVA_ERR_DEVICE_TIMEOUT, "cross_attention: a kernel's wait expired (code " +
+                                                     std::to_string(fwd ? fwd : bwd) + ")");
+  return NOVA_OK;
 } catch (...) {
   return NOVA_ERR_ALLOC;
 }

@@ -906,13 +906,6 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
 // Host side
 // ---------------------------------------------------------------------------
 
-int device_sms() {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return sms;
-}
-
 Walk make_walk(int B, int HW, int C, int G, int V, bool grad) {
   Walk k;
   const int cpg = C / G;
@@ -935,23 +928,15 @@ Walk make_walk(int B, int HW, int C, int G, int V, bool grad) {
 
 size_t align256(size_t n) { return (n + 255) & ~size_t(255); }
 
-// Workspace of the larger walk (the vector width depends on the pointers).
-long long workspace_bytes(int B, int HW, int C, int G, bool grad) {
-  size_t most = 0;
-  for (int V : {1, 4, 8}) {
-    if (C % V) continue;
-    const Walk k = make_walk(B, HW, C, G, V, grad);
-    const size_t parts = (size_t)B * k.nchunk * C;
-    const size_t n = grad ? align256(parts * 12) + align256((size_t)B * C * 12)
-                          : align256(parts / k.cell * 8) + align256((size_t)B * G * 8);
-    if (n > most) most = n;
-  }
-  return (long long)most;
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+constexpr int kSlabSmem = 220 * 1024;
+size_t slab_smem(const Slab& k, int V, bool grad) {
+  const size_t width = (size_t)k.tx * V;
+  return 4 * (grad ? 3 * k.ty * width + 12 * width : k.ty * width + 4 * width + 2 * k.gb);
+}
 
 constexpr int kMostForward = 16, kMostGrad = 8;  // vectors a thread can hold
 
@@ -977,7 +962,7 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
         k.nv = nv;
         k.ty = (k.ppc + nv - 1) / nv;
         k.threads = (tx * k.ty + 31) / 32 * 32;
-        if (k.threads > kSlabThreads) continue;
+        if (k.threads > kSlabThreads || slab_smem(k, V, grad) > kSlabSmem) continue;
         // The resident form pays while its blocks fit the SMs at once (twice at most in
         // the gradient, whose streaming form has four launches): its phases do not
         // overlap, so further waves cost it more than the second read it saves.
@@ -1002,39 +987,32 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
   return found;
 }
 
-size_t slab_smem(const Slab& k, int V, bool grad) {
-  const size_t width = (size_t)k.tx * V;
-  return 4 * (grad ? 3 * k.ty * width + 12 * width : k.ty * width + 4 * width + 2 * k.gb);
-}
-
-template <typename... KArgs, typename... Args2>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), unsigned grid, int threads, int cs,
-                           size_t smem, cudaStream_t s, Args2&&... args) {
-  cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <auto Kernel, typename... Args2>
+cudaError_t slab_launch(const Slab& k, int B, size_t smem, cudaStream_t s, Args2&&... args) {
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_smem(Kernel, &allowed, kSlabSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
+  cfg.gridDim = dim3((unsigned)((long long)B * k.nblk * k.cs));
+  cfg.blockDim = dim3(k.threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.x = k.cs;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = pdl_enabled(kPdlInput) ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args2>(args)...);
+  return cudaLaunchKernelEx(&cfg, Kernel, std::forward<Args2>(args)...);
 }
 
 template <typename T, int V, int ACT>
 cudaError_t forward_resident(const Args& a, const Slab& k, float* stats, cudaStream_t s) {
-  const unsigned grid = (unsigned)((long long)a.B * k.nblk * k.cs);
   const size_t smem = slab_smem(k, V, false);
 #define NOVA_GN_SLAB(NV) \
-  launch_cluster(resident_forward<T, V, NV, ACT>, grid, k.threads, k.cs, smem, s, a, k, stats)
+  slab_launch<resident_forward<T, V, NV, ACT>>(k, a.B, smem, s, a, k, stats)
   if (k.nv <= 2) return NOVA_GN_SLAB(2);
   if (k.nv <= 4) return NOVA_GN_SLAB(4);
   if (k.nv <= 8) return NOVA_GN_SLAB(8);
@@ -1045,25 +1023,37 @@ cudaError_t forward_resident(const Args& a, const Slab& k, float* stats, cudaStr
 template <typename T, int V, int ACT>
 cudaError_t grad_resident(const Args& a, const Slab& k, const float* stats, float* sums,
                           void* dshift, cudaStream_t s) {
-  const unsigned grid = (unsigned)((long long)a.B * k.nblk * k.cs);
   const size_t smem = slab_smem(k, V, true);
-#define NOVA_GN_SLAB(NV)                                                                     \
-  launch_cluster(resident_grad<T, V, NV, ACT>, grid, k.threads, k.cs, smem, s, a, k, stats, \
-                 sums, dshift)
+#define NOVA_GN_SLAB(NV) \
+  slab_launch<resident_grad<T, V, NV, ACT>>(k, a.B, smem, s, a, k, stats, sums, dshift)
   if (k.nv <= 2) return NOVA_GN_SLAB(2);
   if (k.nv <= 4) return NOVA_GN_SLAB(4);
   return NOVA_GN_SLAB(8);
 #undef NOVA_GN_SLAB
 }
 
+// Workspace of a call with vectors of V elements.
+long long workspace_bytes(int B, int HW, int C, int G, int V, bool grad) {
+  Slab slab;
+  if (make_slab(B, HW, C, G, V, grad, device_sms(), &slab))
+    return grad ? (long long)align256((size_t)B * C * 12) : 0;
+  const Walk k = make_walk(B, HW, C, G, V, grad);
+  const size_t parts = (size_t)B * k.nchunk * C;
+  return (long long)(grad ? align256(parts * 12) + align256((size_t)B * C * 12)
+                          : align256(parts / k.cell * 8) + align256((size_t)B * G * 8));
+}
+
 template <typename T, int V>
-cudaError_t forward(const Args& a, int act, float* stats, bool want_stats, unsigned char* ws,
-                    cudaStream_t s) {
+cudaError_t forward(const Args& a, int act, float* stats, unsigned char* ws, cudaStream_t s) {
   Slab slab;
   if (make_slab(a.B, a.HW, a.C, a.G, V, false, device_sms(), &slab))
-    return act == kSilu ? forward_resident<T, V, kSilu>(a, slab, want_stats ? stats : nullptr, s)
-                        : forward_resident<T, V, kNone>(a, slab, want_stats ? stats : nullptr, s);
+    return act == kSilu ? forward_resident<T, V, kSilu>(a, slab, stats, s)
+                        : forward_resident<T, V, kNone>(a, slab, stats, s);
   const Walk k = make_walk(a.B, a.HW, a.C, a.G, V, false);
+  if (!stats) {
+    stats = reinterpret_cast<float*>(ws);
+    ws += align256((size_t)a.B * a.G * 8);
+  }
   float2* part = reinterpret_cast<float2*>(ws);
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
   cudaError_t e = launch_pdl(kPdlInput, partial_stats<T, V>, grid, dim3(kThreads), 0, s, a, k, part);
@@ -1081,9 +1071,8 @@ template <typename T, int V, int ACT>
 cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, void* dshift,
                      unsigned char* ws, cudaStream_t s) {
   const Walk k = make_walk(a.B, a.HW, a.C, a.G, V, true);
-  float* part = reinterpret_cast<float*>(ws);
-  ws += align256((size_t)a.B * k.nchunk * a.C * 12);
   float* sums = reinterpret_cast<float*>(ws);  // [3][B][C]
+  float* part = reinterpret_cast<float*>(ws + align256((size_t)a.B * a.C * 12));
   const dim3 grid((unsigned)((long long)a.B * k.nchunk * k.ncb));
   cudaError_t e;
   Slab slab;
@@ -1108,6 +1097,13 @@ cudaError_t backward(const Args& a, const float* stats, void* dw, void* dbeta, v
   return e;
 }
 
+// 16-byte accesses where every vector of every operand starts on 16 bytes.
+bool wide(const Args& a, int dtype, bool grad) {
+  const int V = 16 / dtype_bytes(dtype);
+  return a.C % V == 0 && a.xp % V == 0 && a.xb % V == 0 && aligned16(a.x) && aligned16(a.y) &&
+         (!grad || (a.yp % V == 0 && a.yb % V == 0 && aligned16(a.dy)));
+}
+
 int check(const char* what, const Args& a, int dtype, const void* ws, long long ws_bytes,
           bool grad) {
   auto bad = [&](const char* why) {
@@ -1117,25 +1113,19 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
   if (a.C % a.G) return bad("channels must divide into the groups");
   if (a.cpg > 8192) return bad("more than 8192 channels per group");
   if (!dtype_ok(dtype) || !dtype_ok(a.wtype) || !dtype_ok(a.stype)) return bad("bad element type");
-  if (!a.x || !a.y || !ws || (grad && !a.dy)) return bad("null pointer");
+  if (!a.x || !a.y || (grad && !a.dy)) return bad("null pointer");
   if (a.xp < a.C || a.xb < 0 || (grad && (a.yp < a.C || a.yb < 0)))
     return bad("a pixel stride below the channels, or a negative batch stride");
   if (!(a.eps >= 0.f)) return bad("eps must not be negative");
-  if (reinterpret_cast<uintptr_t>(ws) % 256) return bad("workspace not 256-byte aligned");
   if ((long long)a.B * a.HW > (1ll << 31) - 1 - 4096 || (long long)a.B * a.G > (1ll << 31) - 1)
     return bad("more than 2^31 pixels");
-  const long long need = workspace_bytes(a.B, a.HW, a.C, a.G, grad);
+  const long long need = workspace_bytes(a.B, a.HW, a.C, a.G, wide(a, dtype, grad) ? 16 / dtype_bytes(dtype) : 1, grad);
+  if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 256))
+    return bad("workspace missing or not 256-byte aligned");
   if (ws_bytes < need)
     return record_error(NOVA_ERR_WORKSPACE,
                         std::string(what) + ": workspace needs " + std::to_string(need) + " bytes");
   return NOVA_OK;
-}
-
-// 16-byte accesses where every vector of every operand starts on 16 bytes.
-bool wide(const Args& a, int dtype, bool grad) {
-  const int V = 16 / dtype_bytes(dtype);
-  return a.C % V == 0 && a.xp % V == 0 && a.xb % V == 0 && aligned16(a.x) && aligned16(a.y) &&
-         (!grad || (a.yp % V == 0 && a.yb % V == 0 && aligned16(a.dy)));
 }
 
 int done(const char* what, cudaError_t e) {
@@ -1149,9 +1139,12 @@ int done(const char* what, cudaError_t e) {
 #define NOVA_EXPORT extern "C" __attribute__((visibility("default")))
 
 NOVA_EXPORT long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups,
-                                                      int grad) {
-  if (batch < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups) return -1;
-  return nova::gn::workspace_bytes(batch, pixels, C, groups, grad != 0);
+                                                      int dtype, int aligned, int grad) {
+  if (batch < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || !nova::unet::dtype_ok(dtype))
+    return -1;
+  const int V = 16 / nova::unet::dtype_bytes(dtype);
+  return nova::gn::workspace_bytes(batch, pixels, C, groups, aligned && C % V == 0 ? V : 1,
+                                   grad != 0);
 }
 
 NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, const void* d_bias,
@@ -1171,22 +1164,18 @@ NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, co
   if (device.status() != cudaSuccess) return done("group_norm: input", device.status());
   unsigned char* ws = static_cast<unsigned char*>(d_workspace);
   float* stats = static_cast<float*>(d_stats);
-  if (!stats) {
-    stats = reinterpret_cast<float*>(ws);
-    ws += align256((size_t)batch * groups * 8);
-  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool v = wide(a, dtype, false);
   cudaError_t e;
   if (dtype == kF16)
-    e = v ? forward<__half, 8>(a, activation, stats, d_stats != nullptr, ws, s)
-          : forward<__half, 1>(a, activation, stats, d_stats != nullptr, ws, s);
+    e = v ? forward<__half, 8>(a, activation, stats, ws, s)
+          : forward<__half, 1>(a, activation, stats, ws, s);
   else if (dtype == kBF16)
-    e = v ? forward<__nv_bfloat16, 8>(a, activation, stats, d_stats != nullptr, ws, s)
-          : forward<__nv_bfloat16, 1>(a, activation, stats, d_stats != nullptr, ws, s);
+    e = v ? forward<__nv_bfloat16, 8>(a, activation, stats, ws, s)
+          : forward<__nv_bfloat16, 1>(a, activation, stats, ws, s);
   else
-    e = v ? forward<float, 4>(a, activation, stats, d_stats != nullptr, ws, s)
-          : forward<float, 1>(a, activation, stats, d_stats != nullptr, ws, s);
+    e = v ? forward<float, 4>(a, activation, stats, ws, s)
+          : forward<float, 1>(a, activation, stats, ws, s);
   return done("group_norm", e);
 } catch (...) {
   return NOVA_ERR_ALLOC;

@@ -6,6 +6,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "nova_internal.h"
 
 namespace nova {
@@ -15,6 +17,32 @@ namespace unet {
 enum DType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
 inline bool dtype_ok(int t) { return t == kF16 || t == kBF16 || t == kF32; }
 inline int dtype_bytes(int t) { return t == kF32 ? 4 : 2; }
+
+// SMs of the current device, asked once for each device.
+inline int device_sms() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int sms = known[dev].load(std::memory_order_relaxed);
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    known[dev].store(sms, std::memory_order_relaxed);
+  }
+  return sms;
+}
+
+// Lets a kernel have up to `most` bytes of dynamic shared memory, once for each device.
+template <typename Kernel>
+cudaError_t allow_smem(Kernel* kernel, std::atomic<unsigned long long>* done, int most) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (done->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 // Makes the device that `p` lives on, and its context, current for a call: the
 // threads that run a backward pass may come without a context, and a tensor may

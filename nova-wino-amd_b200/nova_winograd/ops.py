@@ -67,16 +67,17 @@ SIGNATURES = {
     "nova_forward_noalloc": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p]),
     "nova_weight_grad_workspace_bytes": (c_longlong, [c_int] * 6),
     "nova_weight_grad_v2": (c_int, [c_void_p] * 4 + [c_longlong] + [c_int] * 6 + [c_void_p]),
-    "nova_group_norm_workspace_bytes": (c_longlong, [c_int] * 5),
+    "nova_group_norm_workspace_bytes": (c_longlong, [c_int] * 7),
     "nova_group_norm_v2": (c_int, [c_void_p] * 7 + [c_longlong] + [c_int] * 4 + [c_longlong] * 2
                            + [c_int] * 4 + [c_float, c_void_p]),
     "nova_group_norm_grad_v2": (c_int, [c_void_p] * 11 + [c_longlong] + [c_int] * 4
                                 + [c_longlong] * 4 + [c_int] * 4 + [c_void_p]),
     "nova_cross_attention_workspace_bytes": (c_longlong, [c_int] * 6),
-    "nova_cross_attention_v2": (c_int, [c_void_p] * 7 + [c_longlong] + [c_int] * 5
+    "nova_cross_attention_v2": (c_int, [c_void_p] * 8 + [c_longlong] + [c_int] * 5
                                 + [c_void_p, c_int, c_int, c_float, c_void_p]),
-    "nova_cross_attention_grad_v2": (c_int, [c_void_p] * 11 + [c_longlong] + [c_int] * 5
+    "nova_cross_attention_grad_v2": (c_int, [c_void_p] * 12 + [c_longlong] + [c_int] * 5
                                      + [c_void_p, c_int, c_int, c_float, c_void_p]),
+    "nova_cross_attention_status": (c_int, []),
     "nova_version": (c_char_p, []),
 }
 

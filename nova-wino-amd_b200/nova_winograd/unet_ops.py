@@ -26,33 +26,38 @@ MASK_NONE, MASK_BOOL = -1, 3
 ACTIVATIONS = {None: 0, "silu": 1}
 MAX_HEAD_DIM = 160
 
-_workspace_sizes = {}
+_fns, _workspace_sizes = {}, {}
+
+
+def _fn(name):
+    """A library function, looked up once."""
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(get_lib(), name)
+    return f
 
 
 def _workspace(name, device, *sizes):
     """Workspace of a call: the library says how much, the caching allocator gives it."""
-    key = (name, device.index) + sizes
+    key = (name, sizes)
     n = _workspace_sizes.get(key)
     if n is None:
-        n = getattr(get_lib(), name)(*sizes)
+        n = _fn(name)(*sizes)
         if n < 0:
             raise ValueError(f"bad sizes for {name[:-len('_workspace_bytes')]}: {sizes}")
         if len(_workspace_sizes) > 4096:
             _workspace_sizes.clear()
         _workspace_sizes[key] = n
     if n == 0:
-        return None, 0
-    return torch.empty(n, dtype=torch.uint8, device=device), n
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), n
 
 
 def _call(name, device, *args):
-    """One library call on ``device`` and its current stream."""
-    fn = getattr(get_lib(), name)
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(device.index))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(device.index))
+    """One library call on ``device`` (the library goes by the operands' device) and
+    its current stream."""
+    status = (_fns.get(name) or _fn(name))(*args, _raw_stream(device.index))
     if status:
         check(status, name)
 
@@ -79,6 +84,12 @@ def _pixel_strides(x):
     return (sb if B > 1 else 0), pitch
 
 
+def _vectors(dtype, t, strides):
+    """Whether the pixels of t start on 16 bytes."""
+    v = 4 if dtype == 2 else 8
+    return int(t.data_ptr() % 16 == 0 and strides[0] % v == 0 and strides[1] % v == 0)
+
+
 def _norm_forward(x, num_groups, weight, bias, eps, act, shift, want_stats):
     B, C, H, W = x.shape
     strides = _pixel_strides(x)
@@ -86,11 +97,13 @@ def _norm_forward(x, num_groups, weight, bias, eps, act, shift, want_stats):
                     memory_format=torch.channels_last)
     stats = torch.empty(2, B, num_groups, device=x.device) if want_stats else None
     if y.numel():
-        ws, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C, num_groups, 0)
+        dtype = DTYPES[x.dtype]
+        ws, at, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C,
+                               num_groups, dtype, _vectors(dtype, x, strides), 0)
         param = weight if weight is not None else bias
         _call("nova_group_norm_v2", x.device, x.data_ptr(), _p(weight), _p(bias), _p(shift),
-              y.data_ptr(), _p(stats), _p(ws), n, B, H * W, C, num_groups, *strides,
-              DTYPES[x.dtype], 2 if param is None else DTYPES[param.dtype],
+              y.data_ptr(), _p(stats), at, n, B, H * W, C, num_groups, *strides, dtype,
+              2 if param is None else DTYPES[param.dtype],
               2 if shift is None else DTYPES[shift.dtype], act, eps)
     return y, stats
 
@@ -105,34 +118,41 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, shift, stats = ctx.saved_tensors
-        B, C, H, W = x.shape
-        need = ctx.needs_input_grad
-        dx = torch.empty((B, C, H, W), dtype=x.dtype, device=x.device,
-                         memory_format=torch.channels_last)
-        dw = torch.empty_like(weight) if need[1] else None
-        db = torch.empty_like(bias) if need[2] else None
-        ds = torch.empty_like(shift) if need[3] else None
-        if not dx.numel():
-            for t in (dw, db, ds):
-                if t is not None:
-                    t.zero_()
-            return dx, dw, db, ds, None, None, None
-        strides = _pixel_strides(dy)
-        if strides is None:
-            dy = dy.contiguous(memory_format=torch.channels_last)
-            strides = _pixel_strides(dy)
-        ws, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C,
-                           ctx.num_groups, 1)
-        param = weight if weight is not None else bias
-        _call("nova_group_norm_grad_v2", x.device, x.data_ptr(), dy.data_ptr(), _p(weight),
-              _p(bias), _p(shift), stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db), _p(ds),
-              _p(ws), n, B, H * W, C, ctx.num_groups, *_pixel_strides(x), *strides,
-              DTYPES[x.dtype], 2 if param is None else DTYPES[param.dtype],
-              2 if shift is None else DTYPES[shift.dtype], ctx.act)
-        return (dx if need[0] else None), dw, db, ds, None, None, None
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, dy)
+
+
+def _norm_backward(ctx, dy):
+    x, weight, bias, shift, stats = ctx.saved_tensors
+    B, C, H, W = x.shape
+    need = ctx.needs_input_grad
+    dx = torch.empty((B, C, H, W), dtype=x.dtype, device=x.device,
+                     memory_format=torch.channels_last)
+    dw = torch.empty_like(weight) if need[1] else None
+    db = torch.empty_like(bias) if need[2] else None
+    ds = torch.empty_like(shift) if need[3] else None
+    if not dx.numel():
+        for t in (dw, db, ds):
+            if t is not None:
+                t.zero_()
+        return dx, dw, db, ds, None, None, None
+    xs, ys = _pixel_strides(x), _pixel_strides(dy)
+    if ys is None:
+        dy = dy.contiguous(memory_format=torch.channels_last)
+        ys = _pixel_strides(dy)
+    dtype = DTYPES[x.dtype]
+    ws, at, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C,
+                           ctx.num_groups, dtype,
+                           _vectors(dtype, x, xs) and _vectors(dtype, dy, ys), 1)
+    param = weight if weight is not None else bias
+    _call("nova_group_norm_grad_v2", x.device, x.data_ptr(), dy.data_ptr(), _p(weight), _p(bias),
+          _p(shift), stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db), _p(ds), at, n, B, H * W, C,
+          ctx.num_groups, *xs, *ys, dtype, 2 if param is None else DTYPES[param.dtype],
+          2 if shift is None else DTYPES[shift.dtype], ctx.act)
+    return (dx if need[0] else None), dw, db, ds, None, None, None
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
 def _check_param(name, t, shape, x):
@@ -187,8 +207,10 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias, shift)):
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)
+                                    or (shift is not None and shift.requires_grad)):
         return _GroupNorm.apply(x, weight, bias, shift, num_groups, eps, act)
     return _norm_forward(x, num_groups, weight, bias, eps, act, shift, False)[0]
 
@@ -232,6 +254,12 @@ class NovaGroupNorm(nn.GroupNorm):
 # Cross attention
 # ---------------------------------------------------------------------------
 
+def _one_tile(D):
+    """Keys that the gradient takes in one tile; with more it reads o, and what the
+    rounding of o left off, for the row sums of do . o."""
+    return 128 if D <= 128 else 80
+
+
 def _rows(t):
     """t [B, N, H, D] with its rows' elements next to each other and every row on 16
     bytes: t itself where it lies so, else a contiguous copy."""
@@ -256,52 +284,64 @@ def _mask_type(mask):
     return MASK_BOOL if mask.dtype == torch.bool else DTYPES[mask.dtype]
 
 
-def _cross_forward(q, k, v, mask, scale, want_lse):
+def _cross_forward(q, k, v, mask, scale, train):
     B, Nq, H, D = q.shape
     Nk = k.shape[1]
     out = torch.empty((B, Nq, H, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device) if want_lse else None
+    low = lse = None
+    if train:
+        lse = torch.empty((B, H, Nq), dtype=torch.float32, device=q.device)
+        if Nk > _one_tile(D):
+            low = torch.empty((B, Nq, H, D), dtype=q.dtype, device=q.device)
     if out.numel() and Nk:
-        ws, n = _workspace("nova_cross_attention_workspace_bytes", q.device, B, Nq, Nk, H, D, 0)
+        ws, at, n = _workspace("nova_cross_attention_workspace_bytes", q.device, B, Nq, Nk, H, D, 0)
         _call("nova_cross_attention_v2", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-              _p(mask), out.data_ptr(), _p(lse), _p(ws), n, B, Nq, Nk, H, D,
+              _p(mask), out.data_ptr(), _p(low), _p(lse), at, n, B, Nq, Nk, H, D,
               _strides(q, k, v, mask), DTYPES[q.dtype], _mask_type(mask), scale)
     else:
         out.zero_()
-    return out, lse
+    return out, low, lse
 
 
 class _CrossAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, mask, scale):
-        out, lse = _cross_forward(q, k, v, mask, scale, True)
-        ctx.save_for_backward(q, k, v, mask, out, lse)
+        out, low, lse = _cross_forward(q, k, v, mask, scale, True)
+        if low is None:
+            ctx.save_for_backward(q, k, v, mask, None, None, lse)
+        else:
+            ctx.save_for_backward(q, k, v, mask, out, low, lse)
         ctx.scale = scale
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, mask, out, lse = ctx.saved_tensors
-        B, Nq, H, D = q.shape
-        Nk = k.shape[1]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        dv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-        if dq.numel() and Nk:
-            do = _rows(do)
-            ws, n = _workspace("nova_cross_attention_workspace_bytes", q.device, B, Nq, Nk, H, D, 1)
-            _call("nova_cross_attention_grad_v2", q.device, q.data_ptr(), k.data_ptr(),
-                  v.data_ptr(), _p(mask), out.data_ptr(), do.data_ptr(), lse.data_ptr(),
-                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(ws), n, B, Nq, Nk, H, D,
-                  _strides(q, k, v, mask, do), DTYPES[q.dtype], _mask_type(mask), ctx.scale)
-        else:
-            for t in (dq, dk, dv):
-                t.zero_()
-        need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None,
-                None)
+        return (_cross_backward_once if torch.is_grad_enabled() else _cross_backward)(ctx, do)
+
+
+def _cross_backward(ctx, do):
+    q, k, v, mask, out, low, lse = ctx.saved_tensors
+    B, Nq, H, D = q.shape
+    Nk = k.shape[1]
+    dq = torch.empty((B, Nq, H, D), dtype=q.dtype, device=q.device)
+    dk = torch.empty((B, Nk, H, D), dtype=q.dtype, device=q.device)
+    dv = torch.empty((B, Nk, H, D), dtype=q.dtype, device=q.device)
+    if dq.numel() and Nk:
+        do = _rows(do)
+        ws, at, n = _workspace("nova_cross_attention_workspace_bytes", q.device, B, Nq, Nk, H, D, 1)
+        _call("nova_cross_attention_grad_v2", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+              _p(mask), _p(out), _p(low), do.data_ptr(), lse.data_ptr(), dq.data_ptr(),
+              dk.data_ptr(), dv.data_ptr(), at, n, B, Nq, Nk, H, D, _strides(q, k, v, mask, do),
+              DTYPES[q.dtype], _mask_type(mask), ctx.scale)
+    else:
+        for t in (dq, dk, dv):
+            t.zero_()
+    need = ctx.needs_input_grad
+    return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, None, None)
+
+
+_cross_backward_once = torch.autograd.function.once_differentiable(_cross_backward)
 
 
 def nova_cross_attention(q, k, v, key_mask=None, scale=None):

@@ -470,3 +470,84 @@ def test_run_of_both_against_the_plain_forms():
     # The attention is held to what the norm gave it.
     o = P.cross_attention(q.double(), k.double(), v.double(), m, 32 ** -0.5, dtype=F16)
     near(both_ops(x, s, w, b, k, v, m), o["o"], o["o_tol"], "attention")
+
+
+@pytest.mark.parametrize("xl", [False, True])
+def test_unet_caller_on_the_operators(xl):
+    """The UNet callers with their norms and cross attentions on the operators: every
+    one of them is called, and the step stays with the 32-bit model as near as the
+    16-bit model does (twice its distance: both round the same intermediate results)."""
+    import unet_callers as U
+    import nova_winograd
+    if xl:
+        spec = U.UNetSpec(channels=(32, 64, 64), attn_depth=(0, 1, 2), mid_depth=2,
+                          context_dim=24, head_dim=16, linear_proj=True, add_embed=True, groups=8,
+                          pooled_dim=20, add_time_dim=8)
+    else:
+        spec = U.UNetSpec(channels=(32, 64), attn_depth=(1, 1), mid_depth=1, context_dim=16,
+                          heads=4, groups=8)
+    torch.manual_seed(0)
+    exact = U.UNet(spec).cuda().eval()
+    model = U.UNet(spec).cuda().eval()
+    model.load_state_dict(exact.state_dict())
+    model = model.half().to(memory_format=torch.channels_last)
+    x, t, ctx, extra = U.make_inputs(spec, 2, 16, "cuda", F32, seed=3)
+    calls = {"nova_group_norm": 0, "nova_cross_attention": 0}
+    saved = {n: getattr(nova_winograd, n) for n in calls}
+
+    def counted(n):
+        def f(*a, **k):
+            calls[n] += 1
+            return saved[n](*a, **k)
+        return f
+
+    with torch.no_grad():
+        want = exact(x, t, ctx, **extra)
+        args = (x.half().contiguous(memory_format=torch.channels_last), t, ctx.half())
+        before = model(*args, **extra)
+        U.use_nova_ops(model)
+        try:
+            for n in calls:
+                setattr(nova_winograd, n, counted(n))
+            got = model(*args, **extra)
+        finally:
+            for n in calls:
+                setattr(nova_winograd, n, saved[n])
+        U.use_nova_ops(model, False)
+        assert torch.equal(model(*args, **extra), before)
+    norms = sum(isinstance(m, torch.nn.GroupNorm) for m in model.modules())
+    layers = sum(isinstance(m, U.TransformerLayer) for m in model.modules())
+    assert calls == {"nova_group_norm": norms, "nova_cross_attention": layers}
+    assert torch.isfinite(got).all()
+    assert (got.float() - want).norm() <= 2 * (before.float() - want).norm()
+
+
+def test_unet_caller_gradients_on_the_operators():
+    """A training step's gradients through the operators against the 32-bit model's."""
+    import unet_callers as U
+    spec = U.UNetSpec(channels=(32, 64), attn_depth=(1, 1), mid_depth=1, context_dim=16, heads=4,
+                      groups=8)
+    torch.manual_seed(1)
+    exact = U.UNet(spec).cuda()
+    model = U.UNet(spec).cuda()
+    model.load_state_dict(exact.state_dict())
+    model = model.half().to(memory_format=torch.channels_last)
+    x, t, ctx, _ = U.make_inputs(spec, 2, 16, "cuda", F32, seed=4)
+    args = (x.half().contiguous(memory_format=torch.channels_last), t, ctx.half())
+
+    def grads(m, *a):
+        m.zero_grad()
+        m(*a).float().square().mean().backward()
+        return torch.cat([p.grad.float().flatten() for p in m.parameters()])
+
+    want = grads(exact, x, t, ctx)
+    before = grads(model, *args)
+    U.use_nova_ops(model)
+    got = grads(model, *args)
+    assert torch.isfinite(got).all()
+    assert (got - want).norm() <= 2 * (before - want).norm()
+
+
+def test_cross_status_is_clear():
+    from nova_winograd import ops
+    assert ops.get_lib().nova_cross_attention_status() == 0

@@ -122,11 +122,15 @@ def norm_args(**kw):
     return [*a.values(), None]
 
 
+# More than the resident form holds: a workspace is needed.
+BIG = {"B": 8, "HW": 1 << 16, "C": 64, "G": 2, "sb": 1 << 22, "sp": 64}
+
+
 @pytest.mark.parametrize("kw,status", [
-    ({"x": None}, 1), ({"y": None}, 1), ({"ws": None}, 1), ({"ws": 128}, 1), ({"B": 0}, 1),
+    ({"x": None}, 1), ({"y": None}, 1), ({"ws": None, **BIG}, 1), ({"ws": 128, **BIG}, 1), ({"B": 0}, 1),
     ({"HW": 0}, 1), ({"C": 0}, 1), ({"G": 0}, 1), ({"G": 3}, 1), ({"sp": 7}, 1), ({"sb": -1}, 1),
     ({"t": 3}, 1), ({"wt": -1}, 1), ({"act": 2}, 1), ({"eps": -1.0}, 1),
-    ({"B": 1 << 20, "HW": 1 << 20}, 1), ({"n": 8}, 3),
+    ({"B": 1 << 20, "HW": 1 << 20}, 1), ({"n": 8, **BIG}, 3),
 ])
 def test_group_norm_entry_validates(lib, kw, status):
     assert lib.nova_group_norm_v2(*norm_args(**kw)) == status
@@ -143,8 +147,10 @@ def test_group_norm_grad_entry_validates(lib):
                {"gb": -8}):
         assert call(**kw) == 1, kw
     assert call(n=0) == 3
-    assert lib.nova_group_norm_workspace_bytes(1, 4, 8, 3, 0) == -1
-    assert lib.nova_group_norm_workspace_bytes(0, 4, 8, 2, 1) == -1
+    assert lib.nova_group_norm_workspace_bytes(1, 4, 8, 3, 0, 1, 0) == -1
+    assert lib.nova_group_norm_workspace_bytes(0, 4, 8, 2, 0, 1, 1) == -1
+    assert lib.nova_group_norm_workspace_bytes(1, 4, 8, 2, 3, 1, 1) == -1
+    assert lib.nova_group_norm_workspace_bytes(1, 4, 8, 2, 0, 1, 0) == 0
 
 
 def cross_strides(B, Nq, Nk, H, D, **kw):
@@ -164,7 +170,7 @@ def cross_strides(B, Nq, Nk, H, D, **kw):
     ({"st": cross_strides(1, 4, 4, 2, 16, i9=-1)}, 1),
 ])
 def test_cross_attention_entry_validates(lib, kw, status):
-    a = dict(q=16, k=16, v=16, m=16, o=16, lse=16, ws=256, n=1 << 40, B=1, Nq=4, Nk=4, H=2, D=16,
+    a = dict(q=16, k=16, v=16, m=16, o=16, low=None, lse=16, ws=256, n=1 << 40, B=1, Nq=4, Nk=4, H=2, D=16,
              st=cross_strides(1, 4, 4, 2, 16), t=0, mt=-1, scale=1.0)
     a.update(kw)
     assert lib.nova_cross_attention_v2(*a.values(), None) == status
@@ -173,16 +179,16 @@ def test_cross_attention_entry_validates(lib, kw, status):
 
 def test_cross_attention_grad_entry_validates(lib):
     def call(**kw):
-        a = dict(q=16, k=16, v=16, m=16, o=16, do=16, lse=16, dq=16, dk=16, dv=16, ws=256,
+        a = dict(q=16, k=16, v=16, m=16, o=16, low=16, do=16, lse=16, dq=16, dk=16, dv=16, ws=256,
                  n=1 << 40, B=1, Nq=4, Nk=4, H=2, D=16, st=cross_strides(1, 4, 4, 2, 16), t=0,
                  mt=-1, scale=1.0)
         a.update(kw)
         return lib.nova_cross_attention_grad_v2(*a.values(), None)
-    for kw in ({"o": None}, {"do": None}, {"lse": None}, {"dq": None}, {"dk": None}, {"dv": None},
+    long = {"Nk": 300, "st": cross_strides(1, 4, 300, 2, 16)}
+    for kw in ({"o": None, **long}, {"low": None, **long}, {"low": 8, **long}, {"do": None}, {"lse": None}, {"dq": None}, {"dk": None}, {"dv": None},
                {"do": 8}, {"dk": 8}, {"st": cross_strides(1, 4, 4, 2, 16, i12=20)}):
         assert call(**kw) == 1, kw
     # More keys than one tile: a workspace is needed.
-    long = {"Nk": 300, "st": cross_strides(1, 4, 300, 2, 16)}
     assert lib.nova_cross_attention_workspace_bytes(1, 4, 300, 2, 16, 1) > 0
     assert call(n=0, **long) == 3
     assert call(ws=None, **long) == 1

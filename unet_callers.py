@@ -18,6 +18,11 @@ shapes:
 Both use GroupNorm(32) + SiLU residual blocks with the time embedding added
 between the two 3x3 convs, stride-2 3x3 downsampling convs (not eligible) and
 nearest-neighbour x2 upsampling followed by a 3x3 stride-1 conv (eligible).
+
+``use_nova_ops(model)`` runs the layers between the convolutions on the
+framework's operators: every group norm of a channels-last activation through
+``nova_group_norm`` (with its SiLU, and the time embedding added before it), every
+cross attention through ``nova_cross_attention``.
 """
 
 import math
@@ -64,7 +69,29 @@ def sinusoid(t, dim):
     return torch.cat([torch.cos(ang), torch.sin(ang)], dim=-1)
 
 
+def use_nova_ops(model, on=True):
+    """Switch the model's group norms and cross attentions to the framework's
+    operators (or back).  Returns the number of modules that have one."""
+    n = 0
+    for m in model.modules():
+        if isinstance(m, (ResBlock, Attention, Transformer2D, UNet)):
+            m.nova_ops = on
+            n += 1
+    return n
+
+
+def norm_act(norm, x, nova, act=None, shift=None):
+    """``act(norm(x + shift[:, :, None, None]))`` of an nn.GroupNorm."""
+    if nova and x.is_cuda and x.is_contiguous(memory_format=torch.channels_last):
+        from nova_winograd import nova_group_norm
+        return nova_group_norm(x, norm.num_groups, norm.weight, norm.bias, norm.eps, act, shift)
+    h = norm(x if shift is None else x + shift[:, :, None, None])
+    return F.silu(h) if act == "silu" else h
+
+
 class ResBlock(nn.Module):
+    nova_ops = False
+
     def __init__(self, cin, cout, temb_dim, groups):
         super().__init__()
         self.norm1 = nn.GroupNorm(groups, cin, eps=1e-5)
@@ -75,13 +102,14 @@ class ResBlock(nn.Module):
         self.skip = nn.Conv2d(cin, cout, 1) if cin != cout else nn.Identity()
 
     def forward(self, x, temb):
-        h = self.conv1(F.silu(self.norm1(x)))
-        h = h + self.temb(F.silu(temb))[:, :, None, None]
-        h = self.conv2(F.silu(self.norm2(h)))
+        h = self.conv1(norm_act(self.norm1, x, self.nova_ops, "silu"))
+        h = self.conv2(norm_act(self.norm2, h, self.nova_ops, "silu", self.temb(F.silu(temb))))
         return self.skip(x) + h
 
 
 class Attention(nn.Module):
+    nova_ops = False
+
     def __init__(self, dim, ctx_dim, heads):
         super().__init__()
         self.heads = heads
@@ -91,9 +119,15 @@ class Attention(nn.Module):
         self.out = nn.Linear(dim, dim)
 
     def forward(self, x, ctx=None):
-        ctx = x if ctx is None else ctx
         B, N, D = x.shape
         h = self.heads
+        if (self.nova_ops and ctx is not None and x.is_cuda and D // h % 8 == 0 and D // h <= 160
+                and x.dtype in (torch.float16, torch.bfloat16)):
+            from nova_winograd import nova_cross_attention
+            o = nova_cross_attention(*(t.view(B, -1, h, D // h)
+                                       for t in (self.q(x), self.k(ctx), self.v(ctx))))
+            return self.out(o.view(B, N, D))
+        ctx = x if ctx is None else ctx
 
         def split(t):
             return t.view(B, -1, h, D // h).transpose(1, 2)
@@ -119,6 +153,8 @@ class TransformerLayer(nn.Module):
 
 
 class Transformer2D(nn.Module):
+    nova_ops = False
+
     def __init__(self, ch, depth, spec):
         super().__init__()
         heads = spec.heads if spec.heads else ch // spec.head_dim
@@ -131,7 +167,7 @@ class Transformer2D(nn.Module):
 
     def forward(self, x, ctx):
         B, C, H, W = x.shape
-        h = self.norm(x)
+        h = norm_act(self.norm, x, self.nova_ops)
         if self.linear:
             h = self.proj_in(h.flatten(2).transpose(1, 2))
         else:
@@ -155,6 +191,8 @@ class Level(nn.Module):
 
 
 class UNet(nn.Module):
+    nova_ops = False
+
     def __init__(self, spec: UNetSpec):
         super().__init__()
         self.spec = spec
@@ -226,7 +264,7 @@ class UNet(nn.Module):
                     h = lvl.attn[j](h, ctx)
             if i < len(self.upsample):
                 h = self.upsample[i](F.interpolate(h, scale_factor=2.0, mode="nearest"))
-        return self.conv_out(F.silu(self.norm_out(h)))
+        return self.conv_out(norm_act(self.norm_out, h, self.nova_ops, "silu"))
 
 
 def make_inputs(spec, batch, latent, device, dtype=torch.float16, seed=0):
