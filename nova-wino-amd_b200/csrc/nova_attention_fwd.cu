@@ -493,13 +493,21 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
 }
 
 // Up to four queries against many keys: nothing to multiply on the tensor cores,
-// K and V are read once.  A warp takes 8 x (32 / LPK) keys at a time; LPK lanes
+// K and V are read once.  A warp takes 4 x (32 / LPK) keys at a time; LPK lanes
 // share a key, 8 elements of its row each, so that a warp's load is whole rows.
-// All K loads of a step are in flight together, then all V loads.  Rows of keys that
-// take no part are not read.  The keys are split over blocks (`per` keys each) and
-// over a block's warps; the warps join in shared memory, the blocks through the
-// workspace.
-constexpr int kTokenWarps = 4, kTokenUnroll = 8, kTokenQueries = 4;
+// K and V of a step are on their way together, and the mask of the next.  Rows of keys
+// that take no part are not read.  The keys are split over blocks (`per` keys each) and
+// over a block's warps; the warps join in shared memory, up to eight blocks as one
+// cluster through distributed shared memory, more through the workspace.
+constexpr int kTokenWarps = 4, kTokenUnroll = 4, kTokenQueries = 4, kTokenCluster = 8;
+
+__device__ __forceinline__ float peer_float(const float* p, int rank) {
+  uint32_t at;
+  float v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
 
 template <typename T, int LPK, int NQ, bool MASK>
 __global__ void __launch_bounds__(kTokenWarps * 32)
@@ -507,6 +515,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
   constexpr int G = 32 / LPK, U = kTokenUnroll;
   __shared__ float po[kTokenWarps][NQ][LPK * 8];
   __shared__ float pm[kTokenWarps][NQ], pl[kTokenWarps][NQ];
+  __shared__ float row[NQ][LPK * 8], top_of[NQ], sum_of[NQ];  // of the block, not divided
   pdl_trigger();
   pdl_wait();
   const Args& a = p.a;
@@ -521,6 +530,18 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
   const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h + sub * 8;
   const float c = a.scale * kLog2e;
 
+  float bias[U];
+  bool on[U];
+  const auto load_mask = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = k0 + u * G + grp;
+      on[u] = key < last;
+      bias[u] = 0.f;
+      if (MASK && on[u]) on[u] = key_bias(a, b, key, &bias[u]);
+    }
+  };
+  load_mask(first + warp * (U * G));
   float2 q[NQ][4], o[NQ][4] = {};
   float m[NQ], l[NQ];
 #pragma unroll
@@ -534,27 +555,27 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
     for (int e = 0; e < 4; ++e) q[i][e] = make_float2(to_f32(r.e[2 * e]), to_f32(r.e[2 * e + 1]));
   }
   for (int k0 = first + warp * (U * G); k0 < last; k0 += kTokenWarps * U * G) {
-    Pack<T, 8> r[U];
-    float bias[U];
-    bool on[U];
+    Pack<T, 8> kr[U], vr[U];
+    float add[U];
+    bool now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int key = k0 + u * G + grp;
-      on[u] = key < last;
-      bias[u] = 0.f;
-      if (MASK && on[u]) on[u] = key_bias(a, b, key, &bias[u]);
+      kr[u] = vr[u] = Pack<T, 8>{};
+      add[u] = bias[u];
+      now[u] = on[u];
+      const long long key = k0 + u * G + grp;
+      if (now[u] && in) {
+        kr[u] = load_pack<T, 8>(kp + key * a.ks.n);
+        vr[u] = load_pack<T, 8>(vp + key * a.vs.n);
+      }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      r[u] = Pack<T, 8>{};
-      if (on[u] && in) r[u] = load_pack<T, 8>(kp + (long long)(k0 + u * G + grp) * a.ks.n);
-    }
+    load_mask(k0 + kTokenWarps * U * G);
     float s[NQ][U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float2 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(r[u].e[2 * e]), to_f32(r[u].e[2 * e + 1]));
+      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(kr[u].e[2 * e]), to_f32(kr[u].e[2 * e + 1]));
 #pragma unroll
       for (int i = 0; i < NQ; ++i) {
         float2 t = __fmul2_rn(x[0], q[i][0]);
@@ -564,18 +585,13 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
       }
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      r[u] = Pack<T, 8>{};
-      if (on[u] && in) r[u] = load_pack<T, 8>(vp + (long long)(k0 + u * G + grp) * a.vs.n);
-    }
-#pragma unroll
     for (int i = 0; i < NQ; ++i) {
       float top = m[i];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int w = LPK / 2; w > 0; w >>= 1) s[i][u] += __shfl_xor_sync(~0u, s[i][u], w);
-        s[i][u] = on[u] ? fmaf(s[i][u], c, bias[u]) : -INFINITY;
+        s[i][u] = now[u] ? fmaf(s[i][u], c, add[u]) : -INFINITY;
         top = fmaxf(top, s[i][u]);
       }
       // One maximum for the warp, so that its lanes can add up their sums at the end.
@@ -591,7 +607,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         // A key that takes no part has zeros for V and minus infinity for its score.
-        s[i][u] = on[u] ? ex2(s[i][u] - base) : 0.f;
+        s[i][u] = now[u] ? ex2(s[i][u] - base) : 0.f;
         l[i] += s[i][u];
       }
     }
@@ -599,7 +615,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
     for (int u = 0; u < U; ++u) {
       float2 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(r[u].e[2 * e]), to_f32(r[u].e[2 * e + 1]));
+      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(vr[u].e[2 * e]), to_f32(vr[u].e[2 * e + 1]));
 #pragma unroll
       for (int i = 0; i < NQ; ++i)
 #pragma unroll
@@ -630,9 +646,9 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
     }
   }
   __syncthreads();
+  // The block's rows: the same sums in the same order in every thread that forms one.
   for (int t = threadIdx.x; t < NQ * LPK * 8; t += kTokenWarps * 32) {
     const int i = t / (LPK * 8), d = t % (LPK * 8);
-    if (i >= a.Nq || d >= a.D) continue;
     float top = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kTokenWarps; ++w) top = fmaxf(top, pm[w][i]);
@@ -643,19 +659,56 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
       sum = fmaf(f, pl[w][i], sum);
       acc = fmaf(f, po[w][i][d], acc);
     }
+    row[i][d] = acc;
+    if (d == 0) {
+      top_of[i] = top;
+      sum_of[i] = sum;
+    }
+  }
+  const bool cluster = p.splits <= kTokenCluster;
+  if (cluster) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+  // The cluster's rows, a share of them by every block; or this block's for the
+  // joining kernel.
+  const int ranks = cluster ? p.splits : 1, rank = cluster ? split : 0;
+  for (int t = threadIdx.x * ranks + rank; t < NQ * LPK * 8; t += kTokenWarps * 32 * ranks) {
+    const int i = t / (LPK * 8), d = t % (LPK * 8);
+    if (i >= a.Nq || d >= a.D) continue;
+    float top = top_of[i], sum = sum_of[i], acc = row[i][d];
+    if (cluster) {
+      top = -INFINITY;
+      for (int r = 0; r < ranks; ++r) top = fmaxf(top, peer_float(&top_of[i], r));
+      const float base = top == -INFINITY ? 0.f : top;
+      sum = acc = 0.f;
+      for (int r = 0; r < ranks; ++r) {
+        const float f = ex2(peer_float(&top_of[i], r) - base);
+        sum = fmaf(f, peer_float(&sum_of[i], r), sum);
+        acc = fmaf(f, peer_float(&row[i][d], r), acc);
+      }
+    }
     const float v = sum == 0.f ? 0.f : acc / sum;
-    const long long row = ((long long)b * a.H + h) * a.Nq + i;
+    const long long at = ((long long)b * a.H + h) * a.Nq + i;
     const long long off = (((long long)b * a.Nq + i) * a.H + h) * a.D + d;
     const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
-    if (p.splits > 1) {
-      p.part_o[(long long)split * a.B * a.Nq * a.H * a.D + off] = v;
-      if (d == 0) p.part_lse[(long long)split * a.B * a.H * a.Nq + row] = lse;
-    } else {
+    if (cluster) {
       const T r = from_f32<T>(v);
       static_cast<T*>(a.out)[off] = r;
       if (a.low) static_cast<T*>(a.low)[off] = from_f32<T>(v - to_f32(r));
-      if (d == 0 && a.lse) a.lse[row] = lse;
+      if (d == 0 && a.lse) a.lse[at] = lse;
+    } else {
+      p.part_o[(long long)split * a.B * a.Nq * a.H * a.D + off] = v;
+      if (d == 0) p.part_lse[(long long)split * a.B * a.H * a.Nq + at] = lse;
     }
+  }
+  if (cluster) {
+    // No block leaves while another reads its rows.
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
 }
 
@@ -743,7 +796,8 @@ constexpr size_t kSmemMax = 227 * 1024 - 1024;  // beside the static part
 // Few queries, more keys than one tile: the form without tensor cores.
 bool is_token(const Args& a) { return a.Nq <= kTokenQueries && a.Nk > 128; }
 
-// Its split: blocks for four times the SMs, of at least one step of every warp.
+// Its split: blocks for four times the SMs, of at least one step of every warp; a
+// power of two up to a cluster's eight.
 void plan_token(FwdParams* p, int sms) {
   const Args& a = p->a;
   const int lanes = a.D <= 64 ? 8 : a.D <= 128 ? 16 : 32;
@@ -753,16 +807,32 @@ void plan_token(FwdParams* p, int sms) {
   const int steps = (a.Nk + step - 1) / step;
   if (want > steps) want = steps;
   if (want > 64) want = 64;  // what the joining pass reads for a row
-  p->per = (int)((steps + want - 1) / want) * step;
-  p->splits = (a.Nk + p->per - 1) / p->per;
+  if (want > 2 * kTokenCluster) {
+    p->per = (int)((steps + want - 1) / want) * step;
+    p->splits = (a.Nk + p->per - 1) / p->per;
+    return;
+  }
+  p->splits = 1;
+  while (p->splits < kTokenCluster && p->splits < want) p->splits *= 2;
+  p->per = (int)((steps + p->splits - 1) / p->splits) * step;
 }
 
 template <typename T, int LPK, int NQ>
 cudaError_t run_token_n(const FwdParams& p, cudaStream_t s) {
-  const dim3 grid((unsigned)((long long)p.a.B * p.a.H * p.splits)), block(kTokenWarps * 32);
-  return p.a.mask_kind == kMaskNone
-             ? launch_pdl(kPdlInput, forward_token<T, LPK, NQ, false>, grid, block, 0, s, p)
-             : launch_pdl(kPdlInput, forward_token<T, LPK, NQ, true>, grid, block, 0, s, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((long long)p.a.B * p.a.H * p.splits));
+  cfg.blockDim = dim3(kTokenWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled(kPdlInput) ? 1 : 0;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.splits <= kTokenCluster ? p.splits : 1;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return p.a.mask_kind == kMaskNone ? cudaLaunchKernelEx(&cfg, forward_token<T, LPK, NQ, false>, p)
+                                    : cudaLaunchKernelEx(&cfg, forward_token<T, LPK, NQ, true>, p);
 }
 template <typename T, int LPK>
 cudaError_t run_token_l(const FwdParams& p, cudaStream_t s) {
@@ -775,7 +845,7 @@ cudaError_t run_token(const FwdParams& p, cudaStream_t s) {
   cudaError_t e = p.a.D <= 64    ? run_token_l<T, 8>(p, s)
                   : p.a.D <= 128 ? run_token_l<T, 16>(p, s)
                                  : run_token_l<T, 32>(p, s);
-  if (e == cudaSuccess && p.splits > 1) {
+  if (e == cudaSuccess && p.splits > kTokenCluster) {
     const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
     e = launch_pdl(kPdlInput, join_splits<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p);
   }
@@ -854,9 +924,10 @@ cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
 long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
   FwdParams p{};
   p.a.B = B, p.a.Nq = Nq, p.a.Nk = Nk, p.a.H = H, p.a.D = D;
-  if (is_token(p.a)) plan_token(&p, device_sms());
+  const bool token = is_token(p.a);
+  if (token) plan_token(&p, device_sms());
   else plan(&p, device_sms());
-  if (p.splits == 1) return 0;
+  if (p.splits == 1 || (token && p.splits <= kTokenCluster)) return 0;
   const size_t rows = (size_t)B * H * Nq * p.splits;
   return (long long)(align256(rows * D * 4) + align256(rows * 4));
 }
