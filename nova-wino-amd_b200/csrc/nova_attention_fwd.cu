@@ -33,7 +33,8 @@ namespace {
 
 constexpr int kRows = 128;
 constexpr int kThreads = kRows + 32;  // a thread for a row, and a warp that starts the work
-constexpr int kBlocks = 3;  // on an SM, by their registers
+constexpr int kBlocks = 3;       // on an SM, by their registers
+constexpr int kMostSplits = 64;  // of the keys: two for every lane of the joining warp
 constexpr float kLazy = 4.f;
 constexpr int kHeld = 80;  // scores that a thread can hold with three blocks on an SM
 
@@ -492,14 +493,27 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
   }
 }
 
-// Up to four queries against many keys: nothing to multiply on the tensor cores,
-// K and V are read once.  A warp takes 4 x (32 / LPK) keys at a time; LPK lanes
-// share a key, 8 elements of its row each, so that a warp's load is whole rows.
-// K and V of a step are on their way together, and the mask of the next.  Rows of keys
-// that take no part are not read.  The keys are split over blocks (`per` keys each) and
-// over a block's warps; the warps join in shared memory, up to eight blocks as one
-// cluster through distributed shared memory, more through the workspace.
-constexpr int kTokenWarps = 4, kTokenUnroll = 4, kTokenQueries = 4, kTokenCluster = 8;
+// Up to eight queries against many keys: K and V are read once, straight into the
+// fragments of mma.m16n8k16, without shared memory; a tile of tcgen05 would be a
+// sixteenth full and its steps would follow one another.  A warp takes 16 keys at a
+// time.  With g = lane / 4 and t = lane % 4:
+//
+//   S: a lane's 16 bytes of K (key g of 8, elements 8 t .. 8 t + 7 of 32) are the B
+//      fragments of two products.  Which elements of a row meet in which product does
+//      not matter to their sum, so Q is taken in the same order.
+//   P: the scores of 16 keys lie as the A fragment wants them.
+//   O: a lane's 16 bytes of V (keys 2t, 2t+1, 2t+8, 2t+9; elements 8 g .. of 64) give
+//      the B fragments of eight products, one for each element, by pairing halves of
+//      two keys; the columns of product j are elements j, 8 + j, 16 + j, ...
+//
+// The loads of a step are on their way together.  Rows of keys that take no part are not read.  The keys are split over blocks (`per` keys
+// each) and over a block's warps; the warps join in shared memory, up to eight blocks
+// as one cluster through distributed shared memory, more through the workspace.
+constexpr int kTokenBiases = 1024;  // keys whose biases are staged together
+constexpr int kTokenWarps = 4, kTokenQueries = 8, kTokenCluster = 8;
+// Steps of 16 keys on their way together, with five blocks' registers on an SM (three for
+// wide heads): 4 x 2041 keys x 20 heads in 15.5 us, with a mask 17.1 (two steps: 19.4).
+__host__ __device__ constexpr int token_steps(int DB, bool mask) { return DB == 1 && !mask ? 2 : 1; }
 
 __device__ __forceinline__ float peer_float(const float* p, int rank) {
   uint32_t at;
@@ -509,13 +523,32 @@ __device__ __forceinline__ float peer_float(const float* p, int rank) {
   return v;
 }
 
-template <typename T, int LPK, int NQ, bool MASK>
-__global__ void __launch_bounds__(kTokenWarps * 32)
+// c += A B, rows 8 .. 15 of A zero.
+template <typename T>
+__device__ __forceinline__ void mma_rows8(float (&c)[2], uint32_t a0, uint32_t a2, uint32_t b0,
+                                          uint32_t b1) {
+  float x, y;  // rows 8 .. 15
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
+        : "+f"(c[0]), "+f"(c[1]), "=f"(x), "=f"(y)
+        : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
+        : "+f"(c[0]), "+f"(c[1]), "=f"(x), "=f"(y)
+        : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// DB: 64-element blocks of a head.
+template <typename T, int DB, bool MASK>
+__global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
     forward_token(const __grid_constant__ FwdParams p) {
-  constexpr int G = 32 / LPK, U = kTokenUnroll;
-  __shared__ float po[kTokenWarps][NQ][LPK * 8];
+  constexpr int S = token_steps(DB, MASK), NQ = kTokenQueries, kKeys = 16 * S;
+  __shared__ float po[kTokenWarps][NQ][DB * 64];
   __shared__ float pm[kTokenWarps][NQ], pl[kTokenWarps][NQ];
-  __shared__ float row[NQ][LPK * 8], top_of[NQ], sum_of[NQ];  // of the block, not divided
+  __shared__ float biases[MASK ? kTokenBiases : 1];
+  __shared__ float row[NQ][DB * 64], top_of[NQ], sum_of[NQ];  // of the block, not divided
   pdl_trigger();
   pdl_wait();
   const Args& a = p.a;
@@ -523,132 +556,139 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
   const int split = id % p.splits;
   id /= p.splits;
   const int h = id % a.H, b = id / a.H;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % LPK, grp = lane / LPK;
-  const bool in = sub * 8 < a.D;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int first = split * p.per, last = min(a.Nk, first + p.per);
-  const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h + sub * 8;
-  const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h + sub * 8;
+  const T* kp = static_cast<const T*>(a.k) + b * a.ks.b + h * a.ks.h + t * 8;
+  const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h + g * 8;
   const float c = a.scale * kLog2e;
+  const uint4 none = make_uint4(0, 0, 0, 0);
 
-  float bias[U];
-  bool on[U];
-  const auto load_mask = [&](int k0) {
+  // Q as K is read: row g, elements 8 t of every 32.
+  uint4 q[2 * DB];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int key = k0 + u * G + grp;
-      on[u] = key < last;
-      bias[u] = 0.f;
-      if (MASK && on[u]) on[u] = key_bias(a, b, key, &bias[u]);
-    }
-  };
-  load_mask(first + warp * (U * G));
-  float2 q[NQ][4], o[NQ][4] = {};
-  float m[NQ], l[NQ];
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-    Pack<T, 8> r{};
-    if (in && i < a.Nq)
-      r = load_pack<T, 8>(static_cast<const T*>(a.q) + b * a.qs.b + i * a.qs.n + h * a.qs.h + sub * 8);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) q[i][e] = make_float2(to_f32(r.e[2 * e]), to_f32(r.e[2 * e + 1]));
+  for (int i = 0; i < 2 * DB; ++i) {
+    q[i] = none;
+    if (g < a.Nq && i * 32 + t * 8 < a.D)
+      q[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.qs.b + g * a.qs.n +
+                                             h * a.qs.h + i * 32 + t * 8);
   }
-  for (int k0 = first + warp * (U * G); k0 < last; k0 += kTokenWarps * U * G) {
-    Pack<T, 8> kr[U], vr[U];
-    float add[U];
-    bool now[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      kr[u] = vr[u] = Pack<T, 8>{};
-      add[u] = bias[u];
-      now[u] = on[u];
-      const long long key = k0 + u * G + grp;
-      if (now[u] && in) {
-        kr[u] = load_pack<T, 8>(kp + key * a.ks.n);
-        vr[u] = load_pack<T, 8>(vp + key * a.vs.n);
+  float o[DB * 8][2] = {};
+  float m = -INFINITY, l = 0.f;  // of row g; l over this lane's keys
+  const int piece = MASK ? kTokenBiases : last - first;
+  for (int c0 = first; c0 < last; c0 += piece) {
+    const int c1 = min(last, c0 + piece);
+    if (MASK) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < kTokenBiases; i += kTokenWarps * 32) {
+        float w = 0.f;
+        const bool in = c0 + i < c1 && key_bias(a, b, c0 + i, &w);
+        biases[i] = in ? w : -INFINITY;
       }
+      __syncthreads();
     }
-    load_mask(k0 + kTokenWarps * U * G);
-    float s[NQ][U];
+    for (int k0 = c0 + warp * kKeys; k0 < c1; k0 += kTokenWarps * kKeys) {
+    // The biases of this lane's keys 2t, 2t+1, 2t+8, 2t+9 of a step, as its scores are;
+    // minus infinity for a key that is out.
+    float add[S][4];
+    uint4 kr[S][2][2 * DB], vr[S][4][DB];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float2 x[4];
+    for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(kr[u].e[2 * e]), to_f32(kr[u].e[2 * e + 1]));
+      for (int u = 0; u < 2; ++u) {
+        const int key = k0 + 16 * s + 8 * u + g;
+        const bool in = MASK ? biases[key - c0] != -INFINITY : key < c1;
+        const T* at = kp + (long long)key * a.ks.n;
 #pragma unroll
-      for (int i = 0; i < NQ; ++i) {
-        float2 t = __fmul2_rn(x[0], q[i][0]);
-#pragma unroll
-        for (int e = 1; e < 4; ++e) t = __ffma2_rn(x[e], q[i][e], t);
-        s[i][u] = t.x + t.y;
+        for (int i = 0; i < 2 * DB; ++i) {
+          kr[s][u][i] = none;
+          if (in && i * 32 + t * 8 < a.D) kr[s][u][i] = *reinterpret_cast<const uint4*>(at + i * 32);
+        }
       }
-    }
-#pragma unroll
-    for (int i = 0; i < NQ; ++i) {
-      float top = m[i];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int w = LPK / 2; w > 0; w >>= 1) s[i][u] += __shfl_xor_sync(~0u, s[i][u], w);
-        s[i][u] = now[u] ? fmaf(s[i][u], c, add[u]) : -INFINITY;
-        top = fmaxf(top, s[i][u]);
-      }
-      // One maximum for the warp, so that its lanes can add up their sums at the end.
-#pragma unroll
-      for (int w = LPK; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
-      const float base = top == -INFINITY ? 0.f : top;
-      const float f = ex2(m[i] - base);
-      m[i] = top;
-      l[i] *= f;
-      const float2 f2 = make_float2(f, f);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[i][e] = __fmul2_rn(o[i][e], f2);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // A key that takes no part has zeros for V and minus infinity for its score.
-        s[i][u] = now[u] ? ex2(s[i][u] - base) : 0.f;
-        l[i] += s[i][u];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float2 x[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = make_float2(to_f32(vr[u].e[2 * e]), to_f32(vr[u].e[2 * e + 1]));
-#pragma unroll
-      for (int i = 0; i < NQ; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = __ffma2_rn(make_float2(s[i][u], s[i][u]), x[e], o[i][e]);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < NQ; ++i) {
-#pragma unroll
-    for (int w = LPK; w < 32; w <<= 1) {
-      l[i] += __shfl_xor_sync(~0u, l[i], w);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        o[i][e].x += __shfl_xor_sync(~0u, o[i][e].x, w);
-        o[i][e].y += __shfl_xor_sync(~0u, o[i][e].y, w);
-      }
-    }
-    if (grp == 0) {
+        const int key = k0 + 16 * s + 2 * t + (e & 1) + (e >> 1) * 8;
+        add[s][e] = MASK ? biases[key - c0] : key < c1 ? 0.f : -INFINITY;
+        const T* at = vp + (long long)key * a.vs.n;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        po[warp][i][sub * 8 + 2 * e] = o[i][e].x;
-        po[warp][i][sub * 8 + 2 * e + 1] = o[i][e].y;
+        for (int i = 0; i < DB; ++i) {
+          vr[s][e][i] = none;
+          if (add[s][e] != -INFINITY && i * 64 + g * 8 < a.D)
+            vr[s][e][i] = *reinterpret_cast<const uint4*>(at + i * 64);
+        }
       }
     }
-    if (lane == 0) {
-      pm[warp][i] = m[i];
-      pl[warp][i] = l[i];
+    float x[S][2][2];
+    float top = m;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        x[s][u][0] = x[s][u][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * DB; ++i) {
+          mma_rows8<T>(x[s][u], q[i].x, q[i].y, kr[s][u][i].x, kr[s][u][i].y);
+          mma_rows8<T>(x[s][u], q[i].z, q[i].w, kr[s][u][i].z, kr[s][u][i].w);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float w = add[s][2 * u + e];
+          x[s][u][e] = w == -INFINITY ? -INFINITY : fmaf(x[s][u][e], c, w);
+          top = fmaxf(top, x[s][u][e]);
+        }
+      }
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float f = ex2(m - base);
+    m = top;
+    l *= f;
+    if (__any_sync(~0u, f != 1.f)) {
+#pragma unroll
+      for (int i = 0; i < DB * 8; ++i) o[i][0] *= f, o[i][1] *= f;
     }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[s][u][e] = add[s][2 * u + e] == -INFINITY ? 0.f : ex2(x[s][u][e] - base);
+          l += x[s][u][e];
+        }
+      const uint32_t a0 = pack2<T>(x[s][0][0], x[s][0][1]), a2 = pack2<T>(x[s][1][0], x[s][1][1]);
+#pragma unroll
+      for (int i = 0; i < DB; ++i) {
+        const auto pair = [&](uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int e) {
+          mma_rows8<T>(o[i * 8 + e], a0, a2, __byte_perm(v0, v1, 0x5410), __byte_perm(v2, v3, 0x5410));
+          mma_rows8<T>(o[i * 8 + e + 1], a0, a2, __byte_perm(v0, v1, 0x7632),
+                       __byte_perm(v2, v3, 0x7632));
+        };
+        pair(vr[s][0][i].x, vr[s][1][i].x, vr[s][2][i].x, vr[s][3][i].x, 0);
+        pair(vr[s][0][i].y, vr[s][1][i].y, vr[s][2][i].y, vr[s][3][i].y, 2);
+        pair(vr[s][0][i].z, vr[s][1][i].z, vr[s][2][i].z, vr[s][3][i].z, 4);
+        pair(vr[s][0][i].w, vr[s][1][i].w, vr[s][2][i].w, vr[s][3][i].w, 6);
+      }
+    }
+  }
+  }
+  l += __shfl_xor_sync(~0u, l, 1);
+  l += __shfl_xor_sync(~0u, l, 2);
+#pragma unroll
+  for (int i = 0; i < DB; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // Columns 2t and 2t+1 of product e: elements e of the 8-element pieces 2t, 2t+1.
+      po[warp][g][i * 64 + 16 * t + e] = o[i * 8 + e][0];
+      po[warp][g][i * 64 + 16 * t + 8 + e] = o[i * 8 + e][1];
+    }
+  if (t == 0) {
+    pm[warp][g] = m;
+    pl[warp][g] = l;
   }
   __syncthreads();
   // The block's rows: the same sums in the same order in every thread that forms one.
-  for (int t = threadIdx.x; t < NQ * LPK * 8; t += kTokenWarps * 32) {
-    const int i = t / (LPK * 8), d = t % (LPK * 8);
+  for (int z = threadIdx.x; z < NQ * DB * 64; z += kTokenWarps * 32) {
+    const int i = z / (DB * 64), d = z % (DB * 64);
     float top = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kTokenWarps; ++w) top = fmaxf(top, pm[w][i]);
@@ -675,19 +715,30 @@ __global__ void __launch_bounds__(kTokenWarps * 32)
   // The cluster's rows, a share of them by every block; or this block's for the
   // joining kernel.
   const int ranks = cluster ? p.splits : 1, rank = cluster ? split : 0;
-  for (int t = threadIdx.x * ranks + rank; t < NQ * LPK * 8; t += kTokenWarps * 32 * ranks) {
-    const int i = t / (LPK * 8), d = t % (LPK * 8);
-    if (i >= a.Nq || d >= a.D) continue;
+  for (int z = threadIdx.x * ranks + rank; z < a.Nq * DB * 64; z += kTokenWarps * 32 * ranks) {
+    const int i = z / (DB * 64), d = z % (DB * 64);
+    if (d >= a.D) continue;
     float top = top_of[i], sum = sum_of[i], acc = row[i][d];
     if (cluster) {
+      // All peers' values are on their way before the first is used.
+      float tops[kTokenCluster], sums[kTokenCluster], accs[kTokenCluster];
+#pragma unroll
+      for (int r = 0; r < kTokenCluster; ++r) {
+        const int peer = min(r, ranks - 1);
+        tops[r] = peer_float(&top_of[i], peer);
+        sums[r] = peer_float(&sum_of[i], peer);
+        accs[r] = peer_float(&row[i][d], peer);
+      }
       top = -INFINITY;
-      for (int r = 0; r < ranks; ++r) top = fmaxf(top, peer_float(&top_of[i], r));
+#pragma unroll
+      for (int r = 0; r < kTokenCluster; ++r) top = fmaxf(top, tops[r]);
       const float base = top == -INFINITY ? 0.f : top;
       sum = acc = 0.f;
-      for (int r = 0; r < ranks; ++r) {
-        const float f = ex2(peer_float(&top_of[i], r) - base);
-        sum = fmaf(f, peer_float(&sum_of[i], r), sum);
-        acc = fmaf(f, peer_float(&row[i][d], r), acc);
+#pragma unroll
+      for (int r = 0; r < kTokenCluster; ++r) {
+        const float f = r < ranks ? ex2(tops[r] - base) : 0.f;
+        sum = fmaf(f, r < ranks ? sums[r] : 0.f, sum);
+        acc = fmaf(f, r < ranks ? accs[r] : 0.f, acc);
       }
     }
     const float v = sum == 0.f ? 0.f : acc / sum;
@@ -723,18 +774,27 @@ __global__ void __launch_bounds__(128) join_splits(const __grid_constant__ FwdPa
   const int lane = threadIdx.x & 31;
   const int n = row % p.a.Nq, h = row / p.a.Nq % p.a.H;
   const long long b = row / p.a.Nq / p.a.H;
-  float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, p.part_lse[s * rows + row]);
+  // A lane for a split's weight (two: there are at most 64).
+  float w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    w[i] = lane + 32 * i < p.splits ? p.part_lse[(lane + 32 * i) * rows + row] : -INFINITY;
+  float top = fmaxf(w[0], w[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
   const float sub = top == -INFINITY ? 0.f : top;
   const long long off = ((b * p.a.Nq + n) * p.a.H + h) * p.a.D, plane = rows * p.a.D;
+  w[0] = ex2(w[0] - sub);
+  w[1] = ex2(w[1] - sub);
   float acc[kMaxD / 32] = {}, sum = 0.f;
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
-    const float w = ex2(p.part_lse[s * rows + row] - sub);
-    sum += w;
+    const float f = __shfl_sync(~0u, s < 32 ? w[0] : w[1], s & 31);
+    sum += f;
 #pragma unroll
     for (int i = 0; i < kMaxD / 32; ++i)
       if (lane + 32 * i < p.a.D)
-        acc[i] = fmaf(w, p.part_o[s * plane + off + lane + 32 * i], acc[i]);
+        acc[i] = fmaf(f, p.part_o[s * plane + off + lane + 32 * i], acc[i]);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
@@ -793,21 +853,23 @@ namespace {
 
 constexpr size_t kSmemMax = 227 * 1024 - 1024;  // beside the static part
 
-// Few queries, more keys than one tile: the form without tensor cores.
+// Few queries, more keys than one tile: the form that reads straight into fragments.
 bool is_token(const Args& a) { return a.Nq <= kTokenQueries && a.Nk > 128; }
 
 // Its split: blocks for four times the SMs, of at least one step of every warp; a
 // power of two up to a cluster's eight.
 void plan_token(FwdParams* p, int sms) {
   const Args& a = p->a;
-  const int lanes = a.D <= 64 ? 8 : a.D <= 128 ? 16 : 32;
-  const int step = kTokenWarps * kTokenUnroll * (32 / lanes);
+  const int step = kTokenWarps * 16 * token_steps((a.D + 63) / 64, a.mask_kind != kMaskNone);
   const long long heads = (long long)a.B * a.H;
   long long want = (4ll * sms + heads - 1) / heads;
   const int steps = (a.Nk + step - 1) / step;
   if (want > steps) want = steps;
-  if (want > 64) want = 64;  // what the joining pass reads for a row
-  if (want > 2 * kTokenCluster) {
+  if (want > kMostSplits) want = kMostSplits;
+  // More blocks than a cluster's where that leaves each of them 512 keys or more: the
+  // second kernel takes 3 us.
+  if (want > 2 * kTokenCluster && a.Nk / kTokenCluster >= 1024) {
+    want = std::min(want, (long long)a.Nk / 512);
     p->per = (int)((steps + want - 1) / want) * step;
     p->splits = (a.Nk + p->per - 1) / p->per;
     return;
@@ -817,8 +879,8 @@ void plan_token(FwdParams* p, int sms) {
   p->per = (int)((steps + p->splits - 1) / p->splits) * step;
 }
 
-template <typename T, int LPK, int NQ>
-cudaError_t run_token_n(const FwdParams& p, cudaStream_t s) {
+template <typename T, int DB>
+cudaError_t run_token_d(const FwdParams& p, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.a.B * p.a.H * p.splits));
   cfg.blockDim = dim3(kTokenWarps * 32);
@@ -831,20 +893,14 @@ cudaError_t run_token_n(const FwdParams& p, cudaStream_t s) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  return p.a.mask_kind == kMaskNone ? cudaLaunchKernelEx(&cfg, forward_token<T, LPK, NQ, false>, p)
-                                    : cudaLaunchKernelEx(&cfg, forward_token<T, LPK, NQ, true>, p);
-}
-template <typename T, int LPK>
-cudaError_t run_token_l(const FwdParams& p, cudaStream_t s) {
-  if (p.a.Nq == 1) return run_token_n<T, LPK, 1>(p, s);
-  if (p.a.Nq == 2) return run_token_n<T, LPK, 2>(p, s);
-  return run_token_n<T, LPK, kTokenQueries>(p, s);
+  return p.a.mask_kind == kMaskNone ? cudaLaunchKernelEx(&cfg, forward_token<T, DB, false>, p)
+                                    : cudaLaunchKernelEx(&cfg, forward_token<T, DB, true>, p);
 }
 template <typename T>
 cudaError_t run_token(const FwdParams& p, cudaStream_t s) {
-  cudaError_t e = p.a.D <= 64    ? run_token_l<T, 8>(p, s)
-                  : p.a.D <= 128 ? run_token_l<T, 16>(p, s)
-                                 : run_token_l<T, 32>(p, s);
+  cudaError_t e = p.a.D <= 64    ? run_token_d<T, 1>(p, s)
+                  : p.a.D <= 128 ? run_token_d<T, 2>(p, s)
+                                 : run_token_d<T, 3>(p, s);
   if (e == cudaSuccess && p.splits > kTokenCluster) {
     const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
     e = launch_pdl(kPdlInput, join_splits<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p);
@@ -868,7 +924,7 @@ void plan(FwdParams* p, int sms) {
   p->splits = 1;
   p->per = p->nkt;
   if (p->nkt > 1 && p->total < sms) {
-    const long long want = std::min((long long)p->nkt, kBlocks * sms / p->total);
+    const long long want = std::min((long long)std::min(p->nkt, kMostSplits), kBlocks * sms / p->total);
     p->per = (int)((p->nkt + want - 1) / want);
     p->splits = (p->nkt + p->per - 1) / p->per;
   }
@@ -922,14 +978,18 @@ cudaError_t run(const FwdParams& p, const CUtensorMap* m, cudaStream_t s) {
 }  // namespace
 
 long long forward_workspace_bytes(int B, int Nq, int Nk, int H, int D) {
-  FwdParams p{};
-  p.a.B = B, p.a.Nq = Nq, p.a.Nk = Nk, p.a.H = H, p.a.D = D;
-  const bool token = is_token(p.a);
-  if (token) plan_token(&p, device_sms());
-  else plan(&p, device_sms());
-  if (p.splits == 1 || (token && p.splits <= kTokenCluster)) return 0;
-  const size_t rows = (size_t)B * H * Nq * p.splits;
-  return (long long)(align256(rows * D * 4) + align256(rows * 4));
+  size_t most = 0;
+  for (int mask : {kMaskNone, kMaskBool}) {  // the larger of the two splits
+    FwdParams p{};
+    p.a.B = B, p.a.Nq = Nq, p.a.Nk = Nk, p.a.H = H, p.a.D = D, p.a.mask_kind = mask;
+    const bool token = is_token(p.a);
+    if (token) plan_token(&p, device_sms());
+    else plan(&p, device_sms());
+    if (p.splits == 1 || (token && p.splits <= kTokenCluster)) continue;
+    const size_t rows = (size_t)B * H * Nq * p.splits;
+    most = std::max(most, align256(rows * D * 4) + align256(rows * 4));
+  }
+  return (long long)most;
 }
 
 cudaError_t forward_status(int* status) {

@@ -240,7 +240,7 @@ def cross_check(q, k, v, m, do, scale=None):
     (1, 127, 128, 1, 128), (1, 128, 129, 1, 96), (2, 200, 333, 2, 64), (1, 77, 1000, 1, 160),
     (1, 40, 16, 2, 152), (1, 33, 17, 2, 24), (1, 513, 64, 2, 48), (70, 3, 3, 2, 8),
     (1, 1000, 256, 1, 72), (1, 600, 300, 2, 136), (4, 16, 700, 1, 120), (2, 3, 1111, 3, 160), (3, 2, 131, 2, 40), (1, 4, 5000, 2, 128),
-    (2, 1, 300, 2, 72), (1, 1, 40000, 1, 64), (1, 2, 9000, 2, 8),
+    (2, 1, 300, 2, 72), (1, 1, 40000, 1, 64), (1, 2, 9000, 2, 8), (1, 40, 12800, 1, 64), (1, 8, 40000, 1, 48), (2, 8, 517, 3, 56), (1, 7, 300, 2, 104), (2, 9, 300, 2, 64),
 ])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_cross_shapes(B, Nq, Nk, H, D, dtype):
@@ -248,7 +248,7 @@ def test_cross_shapes(B, Nq, Nk, H, D, dtype):
 
 
 @pytest.mark.parametrize("mask", ["bool", "f16", "bf16", "f32"])
-@pytest.mark.parametrize("Nq,Nk", [(70, 77), (1, 300), (130, 400)])
+@pytest.mark.parametrize("Nq,Nk", [(70, 77), (1, 300), (130, 400), (3, 9000)])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_cross_masks(mask, Nq, Nk, dtype):
     case = cross_case(3, Nq, Nk, 2, 64, dtype, mask)
