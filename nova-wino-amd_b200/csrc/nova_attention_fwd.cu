@@ -296,20 +296,19 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
           }
           return v;
         };
-        const auto take_top = [&](const uint32_t(&x)[16], int col) {
-          if (MASK || col + 16 <= keys) {
+        // A chunk's largest score; the chunk is left as scores in base 2.
+        const auto take_top = [&](uint32_t(&x)[16], int col) {
+          const bool whole = MASK || col + 16 <= keys;
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float2 v = score2(x, col, e);
-              top = fmaxf(top, fmaxf(v.x, v.y));
+          for (int e = 0; e < 16; e += 2) {
+            float2 v = score2(x, col, e);
+            if (!whole) {
+              if (col + e >= keys) v.x = -INFINITY;
+              if (col + e + 1 >= keys) v.y = -INFINITY;
             }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float2 v = score2(x, col, e);
-              if (col + e < keys) top = fmaxf(top, v.x);
-              if (col + e + 1 < keys) top = fmaxf(top, v.y);
-            }
+            top = fmaxf(top, fmaxf(v.x, v.y));
+            x[e] = __float_as_uint(v.x);
+            x[e + 1] = __float_as_uint(v.y);
           }
         };
         // Chunks of 16 two by two, the next two on their way; `use` once for each.
@@ -373,12 +372,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
 
         // P, packed over the scores that have been read.
         const auto put_p = [&](const uint32_t(&x)[16], int col) {
-          const bool whole = MASK || col + 16 <= keys;
+          const bool whole = ONE || MASK || col + 16 <= keys;
           uint32_t o[8];
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            float2 v = __fadd2_rn(score2(x, col, 2 * e), make_float2(-sub, -sub));
+            float2 v = ONE ? make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]))
+                           : score2(x, col, 2 * e);
+            v = __fadd2_rn(v, make_float2(-sub, -sub));
             v = make_float2(ex2(v.x), ex2(v.y));
             if (!whole) {
               if (col + 2 * e >= keys) v.x = 0.f;
