@@ -96,6 +96,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = __shfl_sync(~0u, tmem_slot, 0);
+  // Warp 0 starts copies and products; one lane of it, always the same, does.
+  bool one = false;
+  if (warp == 0) one = elect_one();
   const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   pdl_trigger();
   pdl_wait();
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t idesc_d = instr_desc(kBf16, kRows, p.DP, true, true);
   const uint32_t idesc_q = instr_desc(kBf16, kRows, p.DP, false, true);
   const int chunks = p.KT / 16;
-  // S and dP of step i; its tiles have landed when this returns true.
+  // S and dP of step i, by warp 0; its tiles have landed when this returns true.
   auto start_scores = [&](int i) {
     const int st = i % p.stages;
     if (!wait_phase(bx + 8u * st, (i / p.stages) & 1, &abort_flag, &g_status, kDevTimeoutProducer))
@@ -152,24 +155,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t x = s_walk + 2 * st * walk_bytes;
     const uint32_t q_at = kWalkQ ? x : s_fix, k_at = kWalkQ ? s_fix : x;
-    for (int u = 0; u < 2; ++u) {
-      const uint64_t ad = smem_desc_sw128(q_at + u * p.q_bytes);
-      const uint64_t kd = smem_desc_sw128(k_at + u * p.k_bytes);
-      for (int s = 0; s < p.DP / 16; ++s)
-        umma_f16(tmem + u * p.KT, ad + (uint32_t)((s >> 2) * (kRows * 8) + (s & 3) * 2),
-                 kd + (uint32_t)((s >> 2) * (p.KT * 8) + (s & 3) * 2), idesc_s, s != 0);
+    if (one) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint64_t ad = smem_desc_sw128(q_at + u * p.q_bytes);
+        const uint64_t kd = smem_desc_sw128(k_at + u * p.k_bytes);
+#pragma unroll
+        for (int s = 0; s < kMaxD / 16; ++s)
+          if (s < p.DP / 16)
+            umma_f16(tmem + u * p.KT, ad + (uint32_t)((s >> 2) * (kRows * 8) + (s & 3) * 2),
+                     kd + (uint32_t)((s >> 2) * (p.KT * 8) + (s & 3) * 2), idesc_s, s != 0);
+      }
+      umma_commit(bs);
     }
-    umma_commit(bs);
     return true;
   };
 
-  int loaded = 0;  // thread 0's count of started walked pairs
+  int loaded = 0;  // started walked pairs
   bool ok = true;
-  if (tid == 0) {
+  if (one) {
     if (kWalkQ) load_k(kt_fix, s_fix, bf);
     else load_q(t_first, s_fix, bf);
-    for (; loaded < p.stages && loaded < steps; ++loaded) load_step(loaded);
+    for (int u = 0; u < p.stages && u < steps; ++u) load_step(u);
   }
+  loaded = min(p.stages, steps);
   // Bias of key tile `t` into bias[slot]; rows of K behind masked keys are cleared
   // for dQ: dS is zero there, and zero times infinity is not.
   auto set_bias = [&](int t, int slot) {
@@ -194,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (MODE == kBoth && ok) clear_masked(s_fix, 0);
   }
   if (!__syncthreads_and(ok)) ok = false;
-  if (tid == 0 && ok) ok = start_scores(0);
+  if (warp == 0 && ok) ok = start_scores(0);
 
   const float c = p.a.scale * kLog2e;
   const int n0 = (chunks + 1) / 2;
@@ -287,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if ((tid & 31) == 0) peak[warp] = most;
     }
     // The rows of dQ staged over P and dS have left before these are written.
-    if (MODE == kBoth && tid == 0) bulk_wait_read_all();
+    if (MODE == kBoth && one) bulk_wait_read_all();
     if (!__syncthreads_and(ok)) {
       ok = false;
       break;
@@ -347,30 +356,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
 
-    if (tid == 0) {
+    if (warp == 0) {
       tc_fence_after();
-      if (MODE != kQueries) {
-        // dV += P^T dO, dK += dS^T Q: the queries are the contraction.
-        const uint64_t pd = smem_desc_mn(s_p, kRows * 128), sd = smem_desc_mn(s_ds, kRows * 128);
-        const uint64_t gd = smem_desc_mn(q_at + p.q_bytes, kRows * 128),
-                       qd = smem_desc_mn(q_at, kRows * 128);
-        for (int u = 0; u < kRows / 16; ++u)
-          umma_f16(tmem + p.c_dv, pd + 128ull * u, gd + 128ull * u, idesc_d, u != 0 || i != 0);
-        for (int u = 0; u < kRows / 16; ++u)
-          umma_f16(tmem + p.c_dk, sd + 128ull * u, qd + 128ull * u, idesc_d, u != 0 || i != 0);
+      if (one) {
+        if (MODE != kQueries) {
+          // dV += P^T dO, dK += dS^T Q: the queries are the contraction.
+          const uint64_t pd = smem_desc_mn(s_p, kRows * 128), sd = smem_desc_mn(s_ds, kRows * 128);
+          const uint64_t gd = smem_desc_mn(q_at + p.q_bytes, kRows * 128),
+                         qd = smem_desc_mn(q_at, kRows * 128);
+#pragma unroll
+          for (int u = 0; u < kRows / 16; ++u)
+            umma_f16(tmem + p.c_dv, pd + 128ull * u, gd + 128ull * u, idesc_d, u != 0 || i != 0);
+#pragma unroll
+          for (int u = 0; u < kRows / 16; ++u)
+            umma_f16(tmem + p.c_dk, sd + 128ull * u, qd + 128ull * u, idesc_d, u != 0 || i != 0);
+        }
+        if (MODE != kKeys) {
+          const uint64_t sd = smem_desc_sw128(s_ds), kd = smem_desc_mn(k_at, p.KT * 128);
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (u < chunks)
+              umma_f16(tmem + p.c_dq, sd + (uint32_t)((u >> 2) * (kRows * 8) + (u & 3) * 2),
+                       kd + 128ull * u, idesc_q, u != 0 || (MODE == kQueries && i != 0));
+        }
+        umma_commit(bd);
       }
-      if (MODE != kKeys) {
-        const uint64_t sd = smem_desc_sw128(s_ds), kd = smem_desc_mn(k_at, p.KT * 128);
-        for (int u = 0; u < chunks; ++u)
-          umma_f16(tmem + p.c_dq, sd + (uint32_t)((u >> 2) * (kRows * 8) + (u & 3) * 2),
-                   kd + 128ull * u, idesc_q, u != 0 || (MODE == kQueries && i != 0));
-      }
-      umma_commit(bd);
       if (p.early && i + 1 < steps) ok = start_scores(i + 1);
     }
     ok = ok && wait_phase(bd, i & 1, &abort_flag, &g_status, kDevTimeoutEpilogue);
-    if (tid == 0 && ok && loaded < steps) {
-      load_step(loaded);
+    if (loaded < steps) {
+      if (one && ok) load_step(loaded);
       ++loaded;
     }
     __syncwarp();
@@ -399,16 +414,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++i;
         break;
       }
-      if (tid == 0) {
+      if (one) {
         for (int d = 0; d < p.DB; ++d)
           tma_store_4d(&mdq, s_p + d * (kRows * 128), d * 64, (t_first + i) * kRows, h, b);
         bulk_commit();
       }
     }
-    if (tid == 0 && ok && !p.early && i + 1 < steps) {
-      tc_fence_after();
-      ok = start_scores(i + 1);
-    }
+    if (warp == 0 && ok && !p.early && i + 1 < steps) ok = start_scores(i + 1);
     if (kWalkQ) {
       lse = lse_next;
       if (MODE == kKeys) delta = delta_next;
@@ -479,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (tid == 0) {
+  } else if (one) {
     // Let the copies and products that were started end before their memory goes.
     mbar_wait_drain(bf, 0);
     for (int u = 0; u < p.stages && loaded - 1 - u >= 0; ++u)
@@ -488,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (globaltimer() - since < kDrainLimitNs) {
     }
   }
-  if (tid == 0) bulk_wait_all();
+  if (one) bulk_wait_all();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
