@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t bars[5];  // fixed pair, walked pair [2], S and dP, the other products
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ float bias[2][kRows];
+  __shared__ alignas(8) float bias[2][kRows];
   __shared__ float red[2][kRows];
   __shared__ uint32_t peak[kThreads / 32];
   const int tid = threadIdx.x, half = tid >> 7, r = tid & (kRows - 1);
@@ -179,8 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int u = 0; u < p.stages && u < steps; ++u) load_step(u);
   }
   loaded = min(p.stages, steps);
-  // Bias of key tile `t` into bias[slot]; rows of K behind masked keys are cleared
-  // for dQ: dS is zero there, and zero times infinity is not.
+  // Bias of key tile `t` into bias[slot], minus infinity for a key that is out.
   auto set_bias = [&](int t, int slot) {
     const int keys = min(p.KT, p.a.Nk - t * p.KT);
     if (tid < p.KT) {
@@ -189,18 +188,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       bias[slot][tid] = in ? x : -INFINITY;
     }
   };
-  auto clear_masked = [&](uint32_t k_at, int slot) {
+  // Clears the rows of K (and of V behind it) of keys that are out: P and dS are zero
+  // there, and zero times infinity is not.
+  auto clear_masked = [&](uint32_t k_at, int slot, bool both) {
     if (tid < p.KT && bias[slot][tid] == -INFINITY) {
-      for (int d = 0; d < p.DB; ++d)
-        for (int i = 0; i < 8; ++i)
-          st_shared_v4(k_at + d * (p.KT * 128) + sw128(tid, i), 0, 0, 0, 0);
+      for (int u = 0; u < (both ? 2 : 1); ++u)
+        for (int d = 0; d < p.DB; ++d)
+          for (int i = 0; i < 8; ++i)
+            st_shared_v4(k_at + u * p.k_bytes + d * (p.KT * 128) + sw128(tid, i), 0, 0, 0, 0);
       fence_async_smem();
     }
   };
   ok = wait_phase(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
   if (MASK && kWalkQ) {
     set_bias(kt_fix, 0);
-    if (MODE == kBoth && ok) clear_masked(s_fix, 0);
+    if (ok) clear_masked(s_fix, 0, true);
   }
   if (!__syncthreads_and(ok)) ok = false;
   if (warp == 0 && ok) ok = start_scores(0);
@@ -255,27 +257,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     tmem_wait_ld();
     tc_fence_before();
-    float sum = 0.f, top = 0.f;
+    float2 sums = make_float2(0.f, 0.f);
+    float top = 0.f;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (u < count) {
         const int col = 16 * (first + u);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float dp = __uint_as_float(g[u][e]);
+        for (int e = 0; e < 16; e += 2) {
+          float2 dp = make_float2(__uint_as_float(g[u][e]), __uint_as_float(g[u][e + 1]));
+          float2 x = make_float2(__uint_as_float(s[u][e]), __uint_as_float(s[u][e + 1]));
           // The product is rounded before lse is taken off, as it was when lse was
           // formed: a single key's probability is then exactly one.
-          float pr;
           if (MASK) {
-            const float add = bias[slot][col + e];
-            const bool in = add != -INFINITY;
-            pr = in ? ex2(fmaf(__uint_as_float(s[u][e]), c, add) - lse + kLift) : 0.f;
-            if (!in) dp = 0.f;
+            const float2 add = *reinterpret_cast<const float2*>(&bias[slot][col + e]);
+            x = __ffma2_rn(x, make_float2(c, c), add);
+            if (MODE == kQueries) {  // K and V of a key that is out hold anything here
+              if (add.x == -INFINITY) x.x = -INFINITY, dp.x = 0.f;
+              if (add.y == -INFINITY) x.y = -INFINITY, dp.y = 0.f;
+            }
           } else {
-            pr = ex2(__fmul_rn(__uint_as_float(s[u][e]), c) - lse + kLift);
+            x = __fmul2_rn(x, make_float2(c, c));
           }
-          s[u][e] = __float_as_uint(pr);
-          g[u][e] = __float_as_uint(dp);
+          x = __fadd2_rn(x, make_float2(-lse, -lse));
+          x = __fadd2_rn(x, make_float2(kLift, kLift));
+          s[u][e] = __float_as_uint(ex2(x.x));
+          s[u][e + 1] = __float_as_uint(ex2(x.y));
+          g[u][e] = __float_as_uint(dp.x);
+          g[u][e + 1] = __float_as_uint(dp.y);
         }
         if (!MASK && col + 16 > keys) {
 #pragma unroll
@@ -283,11 +292,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (col + e >= keys) s[u][e] = 0u;
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (MODE == kBoth) sum = fmaf(__uint_as_float(s[u][e]), __uint_as_float(g[u][e]), sum);
-          if (!kBf16) top = fmaxf(top, fabsf(__uint_as_float(g[u][e])));
+        for (int e = 0; e < 16; e += 2) {
+          const float2 dp = make_float2(__uint_as_float(g[u][e]), __uint_as_float(g[u][e + 1]));
+          if (MODE == kBoth)
+            sums = __ffma2_rn(make_float2(__uint_as_float(s[u][e]), __uint_as_float(s[u][e + 1])), dp,
+                              sums);
+          if (!kBf16) top = fmaxf(top, fmaxf(fabsf(dp.x), fabsf(dp.y)));
         }
       }
+    const float sum = sums.x + sums.y;
     if (MODE == kBoth) red[half][r] = sum;
     if (!kBf16) {
       // A row that is not finite has no say in the scale of the others.
@@ -329,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       lift *= exp2f((float)exp_now);
     }
-    if (MASK && MODE == kQueries) clear_masked(k_at, slot);
+    if (MASK && MODE == kQueries) clear_masked(k_at, slot, false);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (u < count) {
@@ -343,12 +356,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           st_shared_v4(s_p + at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
           st_shared_v4(s_p + at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
         }
-        float d[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          d[e] = __uint_as_float(s[u][e]) * ((__uint_as_float(g[u][e]) - delta) * lift);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = pack2<T>(d[2 * e], d[2 * e + 1]);
+        for (int e = 0; e < 8; ++e) {
+          float2 d = make_float2(__uint_as_float(g[u][2 * e]), __uint_as_float(g[u][2 * e + 1]));
+          d = __fmul2_rn(__fadd2_rn(d, make_float2(-delta, -delta)), make_float2(lift, lift));
+          d = __fmul2_rn(d, make_float2(__uint_as_float(s[u][2 * e]), __uint_as_float(s[u][2 * e + 1])));
+          w[e] = pack2<T>(d.x, d.y);
+        }
         st_shared_v4(s_ds + at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
         st_shared_v4(s_ds + at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
       }
@@ -393,19 +407,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (MODE == kBoth) {
       // dQ of the tile, staged over P and dS.
       const float f = p.a.scale * exp2f((float)-exp_now);
-      for (int u = half; u < p.DP / 16; u += 2) {
-        uint32_t o[16];
-        tmem_ld16_issue(lanes + p.c_dq + 16u * u, o);
-        tmem_wait_ld();
-        float d[16];
+      uint32_t o[kMaxD / 32][16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) d[e] = __uint_as_float(o[e]) * f;
-        const uint32_t at = s_p + (uint32_t)(u >> 2) * (kRows * 128);
+      for (int u = 0; u < kMaxD / 32; ++u)
+        if (half + 2 * u < p.DP / 16) tmem_ld16_issue(lanes + p.c_dq + 16u * (half + 2 * u), o[u]);
+      tmem_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          st_shared_v4(at + sw128(r, (u & 3) * 2 + e), pack2<T>(d[8 * e], d[8 * e + 1]),
-                       pack2<T>(d[8 * e + 2], d[8 * e + 3]), pack2<T>(d[8 * e + 4], d[8 * e + 5]),
-                       pack2<T>(d[8 * e + 6], d[8 * e + 7]));
+      for (int u = 0; u < kMaxD / 32; ++u) {
+        const int ck = half + 2 * u;
+        if (ck < p.DP / 16) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            w[e] = pack2<T>(__uint_as_float(o[u][2 * e]) * f, __uint_as_float(o[u][2 * e + 1]) * f);
+          const uint32_t at = s_p + (uint32_t)(ck >> 2) * (kRows * 128);
+          st_shared_v4(at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
+          st_shared_v4(at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
+        }
       }
       fence_async_smem();
       tc_fence_before();
@@ -511,29 +529,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // delta = dO . O, with what the rounding of O left off: O's own rounding would enter every
-// dS of its row (BF16, 333 keys: dQ and dK 1.1 times further off).  A warp for a query.
+// dS of its row (BF16, 333 keys: dQ and dK 1.1 times further off).
+// `lpr` lanes (a power of two) share a row.
 template <typename T>
-__global__ void __launch_bounds__(128) row_delta(const __grid_constant__ Args a, float* delta) {
+__global__ void __launch_bounds__(128) row_delta(const __grid_constant__ Args a, float* delta,
+                                                 int lpr) {
   pdl_trigger();
   pdl_wait();
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (long long)a.B * a.H * a.Nq) return;
-  const int lane = threadIdx.x & 31;
-  const int n = row % a.Nq, h = row / a.Nq % a.H;
-  const long long b = row / a.Nq / a.H;
-  const T* o = static_cast<const T*>(a.out) + ((b * a.Nq + n) * a.H + h) * a.D;
-  const T* lo = static_cast<const T*>(a.low) + ((b * a.Nq + n) * a.H + h) * a.D;
-  const T* g = static_cast<const T*>(a.dout) + b * a.dos.b + n * a.dos.n + h * a.dos.h;
+  const int lane = threadIdx.x & 31, sub = lane & (lpr - 1);
+  const long long row = ((long long)blockIdx.x * 4 + (threadIdx.x >> 5)) * (32 / lpr) + lane / lpr;
+  const bool in = row < (long long)a.B * a.H * a.Nq && sub * 8 < a.D;
   float t = 0.f;
-  for (int i = lane * 8; i < a.D; i += 256) {
-    const Pack<T, 8> x = load_pack<T, 8>(o + i), z = load_pack<T, 8>(lo + i),
-                     y = load_pack<T, 8>(g + i);
+  if (in) {
+    const int n = row % a.Nq, h = row / a.Nq % a.H;
+    const long long b = row / a.Nq / a.H, off = ((b * a.Nq + n) * a.H + h) * a.D + sub * 8;
+    const Pack<T, 8> x = load_pack<T, 8>(static_cast<const T*>(a.out) + off),
+                     z = load_pack<T, 8>(static_cast<const T*>(a.low) + off),
+                     y = load_pack<T, 8>(static_cast<const T*>(a.dout) + b * a.dos.b + n * a.dos.n +
+                                         h * a.dos.h + sub * 8);
 #pragma unroll
     for (int e = 0; e < 8; ++e) t = fmaf(to_f32(x.e[e]) + to_f32(z.e[e]), to_f32(y.e[e]), t);
   }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) t += __shfl_xor_sync(~0u, t, s);
-  if (lane == 0) delta[row] = t;
+  for (int s = lpr / 2; s > 0; s >>= 1) t += __shfl_xor_sync(~0u, t, s);
+  if (in && sub == 0) delta[row] = t;
 }
 
 // dK and dV from the query splits' parts, in order.
@@ -631,8 +649,9 @@ cudaError_t run(BwdParams p, const CUtensorMap* m, float* delta, cudaStream_t s)
     e = run_mode<T, MASK, kBoth>(p, m, s);
   } else {
     const long long rows = (long long)p.a.B * p.a.H * p.a.Nq;
-    e = launch_pdl(kPdlInput, row_delta<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, s, p.a,
-                   delta);
+    const int lpr = p.a.D <= 64 ? 8 : p.a.D <= 128 ? 16 : 32, per = 4 * (32 / lpr);
+    e = launch_pdl(kPdlInput, row_delta<T>, dim3((unsigned)((rows + per - 1) / per)), dim3(128), 0, s,
+                   p.a, delta, lpr);
     p.a.delta = delta;
     if (e == cudaSuccess) e = run_mode<T, MASK, kKeys>(p, m, s);
     if (e == cudaSuccess) e = run_mode<T, MASK, kQueries>(p, m, s);
