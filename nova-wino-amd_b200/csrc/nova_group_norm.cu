@@ -14,10 +14,21 @@
 // are dense.  No reference counterpart: the reference's UNet callers leave the
 // norm to the host framework (benchmarks/bench_sd_unet.py:38-109).
 //
-// Statistics.  Every thread keeps sums relative to the first value it sees, so
-// a mean far from zero costs no digits, and parts are joined as (count, mean,
-// sum of squared deviations), in 64 bits where whole samples meet.  Every sum
-// has a fixed order: results repeat bit for bit.
+// Two forms.  Resident: one launch, x read once; a cluster of blocks keeps a sample's
+// channel block in registers.  Streaming: a pass that sums, one that joins, one that
+// writes; for what does not fit the SMs at once.  make_slab has the rule.
+//
+// Statistics.  The resident form takes the mean of its registers, then the squared
+// deviations from it; a streaming thread keeps sums relative to the first value it
+// sees.  A mean far from zero thus costs no digits.  Parts are joined as means and
+// squared deviations, sums over samples in 64 bits.  Every sum has a fixed order:
+// results repeat bit for bit.
+//
+// What bounds it.  8 x 960 x 128 x 128 FP16 forward, 504 MB at least: 156 us, 49 % of the
+// measured copy bandwidth (the summing pass 53 us, 4.8 TB/s; the writing pass 101 us,
+// which reads x again); the vector instructions of conversion and activation, 15 for an
+// element, keep the issue slots half busy and do not all hide behind the loads.
+// 1 x 1280 x 8 x 8: 5.2 us, the launch and three exchanges.
 #include <algorithm>
 #include <string>
 
