@@ -47,7 +47,7 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
     return bad("outputs must be 16-byte aligned");
   if (a.mb < 0 || a.mn < 0) return bad("negative mask stride");
   const long long rows = (long long)a.B * a.H * (a.Nq > a.Nk ? a.Nq : a.Nk);
-  if (rows > (1ll << 31) - 1) return bad("more than 2^31 rows");
+  if (rows > (1ll << 31) - 4096) return bad("more than 2^31 - 4096 rows");
   const long long need = workspace_bytes(a.B, a.Nq, a.Nk, a.H, a.D, grad);
   if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 256))
     return bad("workspace missing or not 256-byte aligned");

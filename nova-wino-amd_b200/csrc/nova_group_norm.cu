@@ -1137,8 +1137,8 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
   if (a.xp < a.C || a.xb < 0 || (grad && (a.yp < a.C || a.yb < 0)))
     return bad("a pixel stride below the channels, or a negative batch stride");
   if (!(a.eps >= 0.f)) return bad("eps must not be negative");
-  if ((long long)a.B * a.HW > (1ll << 31) - 1 - 4096 || (long long)a.B * a.G > (1ll << 31) - 1)
-    return bad("more than 2^31 pixels");
+  if ((long long)a.B * a.HW > (1ll << 31) - 4096 || (long long)a.B * a.G > (1ll << 31) - 4096)
+    return bad("more than 2^31 - 4096 pixels");
   const long long need = workspace_bytes(a.B, a.HW, a.C, a.G, wide(a, dtype, grad) ? 16 / dtype_bytes(dtype) : 1, grad);
   if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 256))
     return bad("workspace missing or not 256-byte aligned");

@@ -25,6 +25,7 @@ DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 MASK_NONE, MASK_BOOL = -1, 3
 ACTIVATIONS = {None: 0, "silu": 1}
 MAX_HEAD_DIM = 160
+_MOST = 2 ** 31 - 4096  # pixels or rows that the library counts in 32 bits
 
 _fns, _workspace_sizes = {}, {}
 
@@ -196,6 +197,8 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
         raise ValueError(f"eps must not be negative, got {eps}")
     if _pixel_strides(x) is None:
         raise ValueError("x must be channels-last (torch.channels_last, or channels of one)")
+    if B * x.shape[2] * x.shape[3] > _MOST:
+        raise ValueError("x must have fewer than 2^31 - 4096 pixels")
     if weight is not None:
         weight = _check_param("weight", weight, (C,), x)
     if bias is not None:
@@ -378,6 +381,8 @@ def nova_cross_attention(q, k, v, key_mask=None, scale=None):
                          f"{list(v.shape)}")
     if D % 8 or not 8 <= D <= MAX_HEAD_DIM:
         raise ValueError(f"head width must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
+    if B * H * max(Nq, Nk) > _MOST:
+        raise ValueError("q, k and v must have fewer than 2^31 - 4096 rows")
     if key_mask is not None:
         if key_mask.dtype != torch.bool and key_mask.dtype not in DTYPES:
             raise TypeError(f"key_mask must be bool, float16, bfloat16 or float32, got "

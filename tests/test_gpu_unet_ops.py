@@ -241,6 +241,7 @@ def cross_check(q, k, v, m, do, scale=None):
     (1, 40, 16, 2, 152), (1, 33, 17, 2, 24), (1, 513, 64, 2, 48), (70, 3, 3, 2, 8),
     (1, 1000, 256, 1, 72), (1, 600, 300, 2, 136), (4, 16, 700, 1, 120), (2, 3, 1111, 3, 160), (3, 2, 131, 2, 40), (1, 4, 5000, 2, 128),
     (2, 1, 300, 2, 72), (1, 1, 40000, 1, 64), (1, 2, 9000, 2, 8), (1, 40, 12800, 1, 64), (1, 8, 40000, 1, 48), (2, 8, 517, 3, 56), (1, 7, 300, 2, 104), (2, 9, 300, 2, 64),
+    (14, 10, 200, 10, 160), (3, 640, 77, 3, 40), (40, 130, 20, 8, 64),
 ])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_cross_shapes(B, Nq, Nk, H, D, dtype):
@@ -426,6 +427,47 @@ def test_on_another_stream():
     torch.cuda.synchronize()
     for t in got + again:
         assert torch.equal(t, want)
+
+
+def test_calls_from_two_threads():
+    """Two host threads, a stream each, every result as from one."""
+    import threading
+    sets = [block_inputs(i, B=2 + i, Nk=(77, 300)[i]) for i in range(2)]
+    want = [both_ops(*s[:7]) for s in sets]
+    torch.cuda.synchronize()
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i].append(both_ops(*sets[i][:7]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(2):
+        assert len(got[i]) == 20 and all(torch.equal(t, want[i]) for t in got[i])
+
+
+def test_long_cache_offsets_past_32_bits():
+    """Keys whose bytes lie past 2^32 of the cache's start: the last ones decide."""
+    B, Nk, H, D = 1, 2 ** 21 + 3, 16, 64
+    k = torch.zeros(B, Nk, H, D, device="cuda", dtype=F16)
+    v = torch.zeros(B, Nk, H, D, device="cuda", dtype=F16)
+    k[:, -1] = 8.0
+    v[:, -1] = rand(H, D, seed=1, dtype=F16)
+    for Nq in (1, 20):
+        q = torch.full((B, Nq, H, D), 8.0, device="cuda", dtype=F16)
+        # The last key's score is 8 * 8 * 64 / 8 = 512; e^-512 of the others is nothing.
+        o = nova_cross_attention(q, k, v)
+        assert torch.equal(o, v[:, -1:].expand_as(o))
 
 
 @pytest.mark.parametrize("Nk", [77, 300])

@@ -75,6 +75,19 @@ def test_cross_attention_refuses(args, kw, error):
         nova_cross_attention(*args, **kw)
 
 
+def test_sizes_past_32_bits_are_refused():
+    # The library counts pixels and rows in 32 bits: 2^32 + 65536 must not become 65536.
+    x = torch.empty(1, 1, 65536, 65537, dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="pixels"):
+        nova_group_norm(x, 1)
+    q = torch.empty(1, 1, 1, 8, dtype=torch.float16, device="meta")
+    k = torch.empty(1, 2 ** 32 + 5, 1, 8, dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="rows"):
+        nova_cross_attention(q, k, k)
+    with pytest.raises(ValueError, match="rows"):
+        nova_cross_attention(k, q, q)
+
+
 def test_module_refuses_and_shares_parameters():
     with pytest.raises(ValueError):
         NovaGroupNorm(4, 8, activation="relu")
@@ -168,6 +181,8 @@ def cross_strides(B, Nq, Nk, H, D, **kw):
     ({"st": cross_strides(1, 4, 4, 2, 16, i1=33)}, 1),
     ({"st": cross_strides(1, 4, 4, 2, 16, i4=-32)}, 1),
     ({"st": cross_strides(1, 4, 4, 2, 16, i9=-1)}, 1),
+    ({"st": cross_strides(1, 4, 4, 2, 16, i4=0)}, 1), ({"low": 8}, 1),
+    ({"B": 1 << 20, "Nq": 1 << 10, "H": 2}, 1), ({"Nk": (1 << 30) + 1}, 1),
 ])
 def test_cross_attention_entry_validates(lib, kw, status):
     a = dict(q=16, k=16, v=16, m=16, o=16, low=None, lse=16, ws=256, n=1 << 40, B=1, Nq=4, Nk=4, H=2, D=16,
