@@ -87,22 +87,27 @@ def _pixel_strides(x):
 
 def _vectors(dtype, t, strides):
     """Whether the pixels of t start on 16 bytes."""
-    v = 4 if dtype == 2 else 8
-    return int(t.data_ptr() % 16 == 0 and strides[0] % v == 0 and strides[1] % v == 0)
+    v = 3 if dtype == 2 else 7
+    return 0 if t.data_ptr() & 15 or (strides[0] | strides[1]) & v else 1
 
 
-def _norm_forward(x, num_groups, weight, bias, eps, act, shift, want_stats):
+def _empty_channels_last(x):
     B, C, H, W = x.shape
-    strides = _pixel_strides(x)
-    y = torch.empty((B, C, H, W), dtype=x.dtype, device=x.device,
-                    memory_format=torch.channels_last)
-    stats = torch.empty(2, B, num_groups, device=x.device) if want_stats else None
-    if y.numel():
+    return torch.empty_strided((B, C, H, W), (H * W * C, 1, W * C, C), dtype=x.dtype,
+                               device=x.device)
+
+
+def _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, want_stats):
+    B, C, H, W = x.shape
+    device = x.device
+    y = _empty_channels_last(x)
+    stats = torch.empty(2, B, num_groups, device=device) if want_stats else None
+    if B and H and W:
         dtype = DTYPES[x.dtype]
-        ws, at, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C,
-                               num_groups, dtype, _vectors(dtype, x, strides), 0)
+        ws, at, n = _workspace("nova_group_norm_workspace_bytes", device, B, H * W, C, num_groups,
+                               dtype, _vectors(dtype, x, strides), 0)
         param = weight if weight is not None else bias
-        _call("nova_group_norm_v2", x.device, x.data_ptr(), _p(weight), _p(bias), _p(shift),
+        _call("nova_group_norm_v2", device, x.data_ptr(), _p(weight), _p(bias), _p(shift),
               y.data_ptr(), _p(stats), at, n, B, H * W, C, num_groups, *strides, dtype,
               2 if param is None else DTYPES[param.dtype],
               2 if shift is None else DTYPES[shift.dtype], act, eps)
@@ -112,10 +117,10 @@ def _norm_forward(x, num_groups, weight, bias, eps, act, shift, want_stats):
 class _GroupNorm(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, x, weight, bias, shift, num_groups, eps, act):
-        y, stats = _norm_forward(x, num_groups, weight, bias, eps, act, shift, True)
+    def forward(ctx, x, weight, bias, shift, strides, num_groups, eps, act):
+        y, stats = _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, True)
         ctx.save_for_backward(x, weight, bias, shift, stats)
-        ctx.num_groups, ctx.act = num_groups, act
+        ctx.strides, ctx.num_groups, ctx.act = strides, num_groups, act
         return y
 
     @staticmethod
@@ -127,8 +132,7 @@ def _norm_backward(ctx, dy):
     x, weight, bias, shift, stats = ctx.saved_tensors
     B, C, H, W = x.shape
     need = ctx.needs_input_grad
-    dx = torch.empty((B, C, H, W), dtype=x.dtype, device=x.device,
-                     memory_format=torch.channels_last)
+    dx = _empty_channels_last(x)
     dw = torch.empty_like(weight) if need[1] else None
     db = torch.empty_like(bias) if need[2] else None
     ds = torch.empty_like(shift) if need[3] else None
@@ -136,8 +140,8 @@ def _norm_backward(ctx, dy):
         for t in (dw, db, ds):
             if t is not None:
                 t.zero_()
-        return dx, dw, db, ds, None, None, None
-    xs, ys = _pixel_strides(x), _pixel_strides(dy)
+        return dx, dw, db, ds, None, None, None, None
+    xs, ys = ctx.strides, _pixel_strides(dy)
     if ys is None:
         dy = dy.contiguous(memory_format=torch.channels_last)
         ys = _pixel_strides(dy)
@@ -150,20 +154,20 @@ def _norm_backward(ctx, dy):
           _p(shift), stats.data_ptr(), dx.data_ptr(), _p(dw), _p(db), _p(ds), at, n, B, H * W, C,
           ctx.num_groups, *xs, *ys, dtype, 2 if param is None else DTYPES[param.dtype],
           2 if shift is None else DTYPES[shift.dtype], ctx.act)
-    return (dx if need[0] else None), dw, db, ds, None, None, None
+    return (dx if need[0] else None), dw, db, ds, None, None, None, None
 
 
 _norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
 
 
-def _check_param(name, t, shape, x):
-    if t.device != x.device:
+def _check_param(name, t, shape, device):
+    if t.dtype in DTYPES and t.shape == shape and t.device == device:
+        return t if t.is_contiguous() else t.contiguous()
+    if t.device != device:
         raise ValueError(f"{name} must be on the input's device")
     if t.dtype not in DTYPES:
         raise TypeError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
 
 
 def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None, shift=None):
@@ -181,32 +185,33 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
                     residual block's time embedding), or None.
 
     Returns a channels-last tensor of x's type.  Statistics and arithmetic are in 32
-    bits (the joining of partial sums in 64), with one rounding at the end; results
-    repeat bit for bit.  Gradients for x, weight, bias and shift.
+    bits (sums over samples in 64), with one rounding at the end; results repeat bit
+    for bit.  Gradients for x, weight, bias and shift.
     """
     if x.dim() != 4:
         raise ValueError(f"x must be [B, C, H, W], got {list(x.shape)}")
     if x.dtype not in DTYPES:
         raise TypeError(f"x must be float16, bfloat16 or float32, got {x.dtype}")
-    B, C = x.shape[:2]
+    B, C, H, W = x.shape
     if num_groups < 1 or C < 1 or C % num_groups:
         raise ValueError(f"{C} channels do not divide into {num_groups} groups")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be None or 'silu', got {activation!r}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    if _pixel_strides(x) is None:
+    strides = _pixel_strides(x)
+    if strides is None:
         raise ValueError("x must be channels-last (torch.channels_last, or channels of one)")
-    if B * x.shape[2] * x.shape[3] > _MOST:
+    if B * H * W > _MOST:
         raise ValueError("x must have fewer than 2^31 - 4096 pixels")
     if weight is not None:
-        weight = _check_param("weight", weight, (C,), x)
+        weight = _check_param("weight", weight, (C,), x.device)
     if bias is not None:
-        bias = _check_param("bias", bias, (C,), x)
+        bias = _check_param("bias", bias, (C,), x.device)
         if weight is not None and bias.dtype != weight.dtype:
             raise TypeError("weight and bias must have one type")
     if shift is not None:
-        shift = _check_param("shift", shift, (B, C), x)
+        shift = _check_param("shift", shift, (B, C), x.device)
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
     act = ACTIVATIONS[activation]
@@ -214,8 +219,8 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
                                     or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)
                                     or (shift is not None and shift.requires_grad)):
-        return _GroupNorm.apply(x, weight, bias, shift, num_groups, eps, act)
-    return _norm_forward(x, num_groups, weight, bias, eps, act, shift, False)[0]
+        return _GroupNorm.apply(x, weight, bias, shift, strides, num_groups, eps, act)
+    return _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, False)[0]
 
 
 class NovaGroupNorm(nn.GroupNorm):
@@ -365,18 +370,19 @@ def nova_cross_attention(q, k, v, key_mask=None, scale=None):
     contiguous.  Products are accumulated and the softmax is computed in 32 bits.
     Gradients for q, k and v repeat bit for bit.
     """
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise ValueError(f"{name} must be [B, N, H, D], got {list(t.shape)}")
-        if t.dtype not in (torch.float16, torch.bfloat16):
-            raise TypeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
-        if t.device != q.device:
-            raise ValueError("q, k and v must be on one device")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k and v must be [B, N, H, D], got {list(q.shape)}, {list(k.shape)} "
+                         f"and {list(v.shape)}")
+    dtype, device = q.dtype, q.device
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
+        raise TypeError(f"q must be float16 or bfloat16, got {dtype}")
+    if k.dtype is not dtype or v.dtype is not dtype:
         raise TypeError("q, k and v must have one type")
+    if k.device != device or v.device != device:
+        raise ValueError("q, k and v must be on one device")
     B, Nq, H, D = q.shape
     Nk = k.shape[1]
-    if k.shape != (B, Nk, H, D) or v.shape != (B, Nk, H, D):
+    if k.shape != (B, Nk, H, D) or v.shape != k.shape:
         raise ValueError(f"k and v must both be [{B}, Nk, {H}, {D}], got {list(k.shape)} and "
                          f"{list(v.shape)}")
     if D % 8 or not 8 <= D <= MAX_HEAD_DIM:
