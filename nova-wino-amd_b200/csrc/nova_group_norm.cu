@@ -15,8 +15,9 @@
 // norm to the host framework (benchmarks/bench_sd_unet.py:38-109).
 //
 // Two forms.  Resident: one launch, x read once; a cluster of blocks keeps a sample's
-// channel block in registers.  Streaming: a pass that sums, one that joins, one that
-// writes; for what does not fit the SMs at once.  make_slab has the rule.
+// channel block in registers, of FP32 at least half of it and the rest in L2.
+// Streaming: a pass that sums, one that joins, one that writes; for what does not fit
+// the SMs at once.  make_slab has the rule.
 //
 // Statistics.  The resident form takes the mean of its registers, then the squared
 // deviations from it; a streaming thread keeps sums relative to the first value it
@@ -566,11 +567,13 @@ struct Slab {
   int cs;        // blocks of a cluster
   int ppc;       // pixels per block
   int tx, ty;    // threads: vector columns x pixels
-  int nv;        // vectors per thread
+  int nv;        // vectors that a thread holds; the forward pass reads the rest again
   int threads;
 };
 
 constexpr int kSlabThreads = 512;
+constexpr int kMostForward = 16, kMostGrad = 8;  // vectors a thread can hold
+constexpr int kAgain = 4;  // width of the vectors that the forward pass may read again: FP32's
 
 __device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
@@ -645,7 +648,8 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
   float* part = bt + width;             // [2][gb] the block's mean and deviations
   pdl_trigger();
   pdl_wait();
-  const Spot q = spot(a, k, V);
+  Spot q = spot(a, k, V);
+  q.nv = min(q.nv, NV);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 
   Pack<T, V> d[NV];
@@ -668,6 +672,21 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
     if (q.nv == NV) body([](int) { return true; });
     else body([&](int v) { return v < q.nv; });
   };
+  // The vectors that the registers do not hold, out of L2, four on their way.
+  const auto rest = [&](auto&& use) {
+    if constexpr (NV < kMostForward || V != kAgain) return;
+    if (!q.active) return;
+    const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.c0 + q.tx * V;
+    for (int p = q.p0 + q.ty + NV * k.ty; p < q.p1; p += 4 * k.ty) {
+      Pack<T, V> v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (p + u * k.ty < q.p1) v[u] = load_pack<T, V>(x + (p + u * k.ty) * a.xp);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (p + u * k.ty < q.p1) use(v[u], p + u * k.ty);
+    }
+  };
   pass([&](auto has) {
 #pragma unroll
     for (int j = 0; j < V / W; ++j) {
@@ -677,6 +696,10 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
         if (has(v)) t = add(t, L::get(d[v], j));
       L::put(mine, j, t);
     }
+  });
+  rest([&](const Pack<T, V>& v, int) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) L::put(mine, j, add(L::at(mine, j), L::get(v, j)));
   });
   __syncthreads();
   stay_packed(d);
@@ -720,6 +743,13 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
           t = fma(u, u, t);
         }
       L::put(mine, j, t);
+    }
+  });
+  rest([&](const Pack<T, V>& v, int) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j) {
+      const F u = add(L::get(v, j), L::at(mu + q.tx * V, j));
+      L::put(mine, j, fma(u, u, L::at(mine, j)));
     }
   });
   __syncthreads();
@@ -769,6 +799,12 @@ __global__ void __launch_bounds__(kSlabThreads, 1)
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (has(v)) store_pack<T, V>(y + v * step, d[v]);
+  });
+  rest([&](Pack<T, V> v, int p) {
+#pragma unroll
+    for (int j = 0; j < V / W; ++j)
+      L::set(v, j, act<ACT>(fma(L::get(v, j), L::at(wt + q.tx * V, j), L::at(bt + q.tx * V, j))));
+    store_pack<T, V>(static_cast<T*>(a.y) + ((long long)q.b * a.HW + p) * a.C + q.c0 + q.tx * V, v);
   });
   cluster_wait();
 }
@@ -956,7 +992,6 @@ size_t slab_smem(const Slab& k, int V, bool grad) {
   return 4 * (grad ? 3 * k.ty * width + 12 * width : k.ty * width + 4 * width + 2 * k.gb);
 }
 
-constexpr int kMostForward = 16, kMostGrad = 8;  // vectors a thread can hold
 
 // The resident form of a call, where it fits and pays.
 bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* best) {
@@ -979,6 +1014,20 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
         k.tx = tx;
         k.nv = nv;
         k.ty = (k.ppc + nv - 1) / nv;
+        // The share of the vectors that is read again, three times over.  It pays for
+        // FP32, whose vectors need no conversion, on most of the SMs and with rows of
+        // whole lines: 4x320x61x67 15.0 us, streaming 18.6; 2x640x64x64 15.0, streaming
+        // 21.1.  Not in FP16 (8x320x64x64 25.2 us, streaming 24.3; values one by one
+        // 4x76x64x70 19.1, streaming 14.8), on 32 blocks (1x128x120x120 in 4 groups 16.7,
+        // streaming 14.7) or in rows of 80 bytes (1x320x128x128 29.4, streaming 21.4).
+        double again = 0;
+        if (!grad && nv == most && tx * k.ty > kSlabThreads) {
+          k.ty = kSlabThreads / tx;
+          again = 1.0 - (double)nv * k.ty / k.ppc;
+          if (again > 0.5 || V != kAgain || tx * 16 < 128 ||
+              (long long)B * k.nblk * cs * 4 < 3 * sms)
+            continue;
+        }
         k.threads = (tx * k.ty + 31) / 32 * 32;
         if (k.threads > kSlabThreads || slab_smem(k, V, grad) > kSlabSmem) continue;
         // The resident form pays while its blocks fit the SMs at once (twice at most in
@@ -992,7 +1041,8 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
         if (blocks > room * (grad ? 2 : 1)) continue;
         // Bytes of the busiest SM, short rows counted with the sectors they touch, and
         // the cluster's exchange.
-        const double cost = (double)((blocks + sms - 1) / sms) * k.ppc * (tx * 16 + 16) / 22.0 +
+        const double cost = (double)((blocks + sms - 1) / sms) * k.ppc * (tx * 16 + 16) *
+                                (1 + again) / 22.0 +
                             150.0 * cs;
         if (!found || cost < best_cost) {
           found = true;

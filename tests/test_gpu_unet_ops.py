@@ -101,6 +101,24 @@ def test_norm_mean_far_from_zero(dtype, mean):
     norm_check(x, *norm_case(2, 64, 4, 24, 24, dtype)[1:], 4, None)
 
 
+# Slabs of 32-bit values that the forward pass keeps in part and reads the rest of
+# again; beside them 16-bit ones of the same size, which it does not.
+@pytest.mark.parametrize("B,C,G,H,W,dtype", [(4, 320, 32, 61, 67, F32), (2, 640, 32, 59, 71, F32),
+                                             (7, 128, 4, 53, 97, F32), (4, 320, 32, 61, 67, BF16)])
+@pytest.mark.parametrize("how", ["plain", "far mean", "slice", "one sample for all"])
+def test_norm_slabs_read_again(B, C, G, H, W, dtype, how):
+    x, w, b, s, dy = norm_case(B, C, G, H, W, dtype, shift=dtype)
+    if how == "far mean":
+        x = (x.float() + 64).to(dtype)
+    if how == "slice":
+        wide = torch.zeros(B, H, W, C + 20, device="cuda", dtype=dtype).permute(0, 3, 1, 2)
+        wide[:, 8:8 + C] = x
+        x = wide[:, 8:8 + C]
+    if how == "one sample for all":
+        x = x[:1].expand(B, C, H, W)
+    norm_check(x, w, b, s, dy, G, "silu")
+
+
 def test_norm_first_pixel_far_out():
     x, w, b, s, dy = norm_case(1, 64, 4, 32, 32, F32)
     x[:, :, 0, 0] = 4000.0
