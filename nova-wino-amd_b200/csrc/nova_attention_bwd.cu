@@ -22,10 +22,12 @@
 // FP16's range is short for that: P is held 2^kLift times larger, and dS is scaled
 // by a power of two that follows the largest |dP| of the block's walk.
 //
-// What bounds it.  8 x 1024 queries x 8 heads x 80, 77 keys, FP16: 27 us, of which a
-// 128-query tile takes about 8,000 cycles; one block to an SM, and its steps follow one
-// another: scores and dP 1,700, P 1,500, dS 900, products 1,600, dQ 1,400.  21 products of
-// 16 steps each are too small to keep the tensor cores busy (9 % of their cycles).
+// What bounds it.  8 x 1024 queries x 8 heads x 80, 77 keys, FP16, forward and gradient:
+// 41 us.  One block to an SM, and a tile's steps follow one another; before arithmetic
+// was paired a 128-query tile took about 9,000 cycles: scores and dP waited for 1,700 to
+// 2,400, P 2,100, exchange 490, dS 860, products 1,600, dQ 1,800.  Pairing, with row sums by
+// groups of lanes, took 3 x 1021 queries to 333 keys from 89 us to 76.  The products are too
+// small to keep the tensor cores busy (9 % of their cycles).
 #include <cuda_runtime.h>
 
 #include "nova_attention.cuh"
