@@ -101,7 +101,9 @@ def _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, want_st
     B, C, H, W = x.shape
     device = x.device
     y = _empty_channels_last(x)
-    stats = torch.empty(2, B, num_groups, device=device) if want_stats else None
+    stats = None
+    if want_stats:
+        stats = torch.empty((2, B, num_groups), dtype=torch.float32, device=device)
     if B and H and W:
         dtype = DTYPES[x.dtype]
         ws, at, n = _workspace("nova_group_norm_workspace_bytes", device, B, H * W, C, num_groups,
