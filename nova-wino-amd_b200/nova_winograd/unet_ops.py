@@ -67,6 +67,27 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _save(ctx, *tensors):
+    """Saves a call's tensors for its gradient."""
+    ctx.save_for_backward(*tensors)
+    ctx.kinds = [None if t is None else (t.dtype, t.device, t.shape) for t in tensors]
+
+
+def _saved(ctx):
+    """What _save saved.  A saved-tensor hook (one that keeps them on the CPU
+    meanwhile, say) may hand back other strides, so these are asked anew."""
+    tensors = ctx.saved_tensors
+    for t, kind in zip(tensors, ctx.kinds):
+        if t is not None and (t.dtype, t.device, t.shape) != kind:
+            raise RuntimeError(f"a saved-tensor hook handed back {t.dtype} {list(t.shape)} on "
+                               f"{t.device} for {kind[0]} {list(kind[2])} on {kind[1]}")
+    return tensors
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 # ---------------------------------------------------------------------------
 # Group norm
 # ---------------------------------------------------------------------------
@@ -83,6 +104,15 @@ def _pixel_strides(x):
     if pitch < C or (H > 1 and W > 1 and sh != W * pitch):
         return None
     return (sb if B > 1 else 0), pitch
+
+
+def _even_pixels(x):
+    """x, or a channels-last copy where its pixels are not evenly spaced, and its strides."""
+    strides = _pixel_strides(x)
+    if strides is None:
+        x = x.contiguous(memory_format=torch.channels_last)
+        strides = _pixel_strides(x)
+    return x, strides
 
 
 def _vectors(dtype, t, strides):
@@ -121,8 +151,8 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, shift, strides, num_groups, eps, act):
         y, stats = _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, True)
-        ctx.save_for_backward(x, weight, bias, shift, stats)
-        ctx.strides, ctx.num_groups, ctx.act = strides, num_groups, act
+        _save(ctx, x, weight, bias, shift, stats)
+        ctx.num_groups, ctx.act = num_groups, act
         return y
 
     @staticmethod
@@ -131,7 +161,8 @@ class _GroupNorm(torch.autograd.Function):
 
 
 def _norm_backward(ctx, dy):
-    x, weight, bias, shift, stats = ctx.saved_tensors
+    x, *rest = _saved(ctx)
+    weight, bias, shift, stats = map(_dense, rest)
     B, C, H, W = x.shape
     need = ctx.needs_input_grad
     dx = _empty_channels_last(x)
@@ -143,10 +174,8 @@ def _norm_backward(ctx, dy):
             if t is not None:
                 t.zero_()
         return dx, dw, db, ds, None, None, None, None
-    xs, ys = ctx.strides, _pixel_strides(dy)
-    if ys is None:
-        dy = dy.contiguous(memory_format=torch.channels_last)
-        ys = _pixel_strides(dy)
+    x, xs = _even_pixels(x)
+    dy, ys = _even_pixels(dy)
     dtype = DTYPES[x.dtype]
     ws, at, n = _workspace("nova_group_norm_workspace_bytes", x.device, B, H * W, C,
                            ctx.num_groups, dtype,
@@ -318,10 +347,7 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale):
         out, low, lse = _cross_forward(q, k, v, mask, scale, True)
-        if low is None:
-            ctx.save_for_backward(q, k, v, mask, None, None, lse)
-        else:
-            ctx.save_for_backward(q, k, v, mask, out, low, lse)
+        _save(ctx, q, k, v, mask, None if low is None else out, low, lse)
         ctx.scale = scale
         return out
 
@@ -331,7 +357,9 @@ class _CrossAttention(torch.autograd.Function):
 
 
 def _cross_backward(ctx, do):
-    q, k, v, mask, out, low, lse = ctx.saved_tensors
+    q, k, v, mask, *rest = _saved(ctx)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out, low, lse = map(_dense, rest)
     B, Nq, H, D = q.shape
     Nk = k.shape[1]
     dq = torch.empty((B, Nq, H, D), dtype=q.dtype, device=q.device)

@@ -27,3 +27,50 @@ def test_norm_under_another_default_type(dtype, B, C, G, H, W):
     finally:
         torch.set_default_dtype(before)
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+class FromCpuInThisLayout:
+    """Saved-tensor hooks that keep what is saved on the CPU, with other strides."""
+
+    def __init__(self):
+        self.hooks = torch.autograd.graph.saved_tensors_hooks(self.pack, lambda t: t.cuda())
+
+    @staticmethod
+    def pack(t):
+        last = t.dim() - 1
+        return t.cpu().transpose(0, last).contiguous().transpose(0, last)
+
+
+@pytest.mark.parametrize("hooks", [
+    lambda: torch.autograd.graph.save_on_cpu(),
+    lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+    lambda: FromCpuInThisLayout().hooks,
+], ids=["cpu", "pinned", "transposed"])
+@pytest.mark.parametrize("sliced", [False, True])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_norm_with_saved_tensors_kept_elsewhere(hooks, sliced, dtype):
+    x, w, b, s, dy = norm_case(2, 64, 4, 7, 9, dtype, shift=dtype)
+    if sliced:
+        wide = torch.zeros(2, 7, 9, 100, device="cuda", dtype=dtype).permute(0, 3, 1, 2)
+        wide[:, 8:72] = x
+        x = wide[:, 8:72]
+    want = norm_check(x, w, b, s, dy, 4, "silu")
+    with hooks():
+        got = norm_check(x, w, b, s, dy, 4, "silu")
+    # A slice's copy may be read in wider vectors: other sums, the same bounds.
+    assert sliced or all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("hooks", [
+    lambda: torch.autograd.graph.save_on_cpu(pin_memory=True),
+    lambda: FromCpuInThisLayout().hooks,
+], ids=["pinned", "transposed"])
+@pytest.mark.parametrize("Nk", [77, 300])
+@pytest.mark.parametrize("mask", [None, "bool", "f16"])
+def test_cross_with_saved_tensors_kept_elsewhere(hooks, Nk, mask):
+    q, k, v, m, do = cross_case(3, 150, Nk, 2, 40, F16, mask)
+    kv = torch.stack([k, v], 2)  # k and v as parts of one projection
+    want = cross_check(q, kv[:, :, 0], kv[:, :, 1], m, do)
+    with hooks():
+        got = cross_check(q, kv[:, :, 0], kv[:, :, 1], m, do)
+    assert all(torch.equal(got[n], want[n]) for n in want)

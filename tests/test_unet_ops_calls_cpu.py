@@ -38,3 +38,79 @@ def test_statistics_are_32_bits_whatever_the_default_type(calls, default_dtype, 
     lse = unet_ops._cross_forward(q, q, q, None, 0.25, True)[2]
     assert lse.dtype == torch.float32 and lse.shape == (2, 2, 3)
     assert [c[0] for c in calls] == ["nova_group_norm_v2", "nova_cross_attention_v2"]
+
+
+class Hooks:
+    """Saved-tensor hooks that hand back ``again(tensor)``, and remember what."""
+
+    def __init__(self, again):
+        self.again, self.given = again, []
+
+    def __enter__(self):
+        def unpack(t):
+            self.given.append(self.again(t))
+            return self.given[-1]
+        self.hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack)
+        return self.hooks.__enter__()
+
+    def __exit__(self, *args):
+        return self.hooks.__exit__(*args)
+
+
+@pytest.mark.parametrize("sliced", [False, True])
+def test_norm_gradient_goes_by_the_strides_of_what_hooks_hand_back(calls, sliced):
+    # Channels 8 .. 15 of 32: pixel pitch 32 as it is, 8 in a compact copy.
+    x = cl(2, 32, 4, 5)[:, 8:16] if sliced else cl(2, 8, 4, 5)
+    compact = dict(memory_format=torch.channels_last if sliced else torch.contiguous_format)
+    with Hooks(lambda t: t.clone(**compact) if t.dim() == 4 else t.clone()):
+        y = unet_ops._GroupNorm.apply(x.requires_grad_(), None, None, None,
+                                      unet_ops._pixel_strides(x), 2, 1e-5, 0)
+        y.backward(torch.zeros_like(y))
+    name, args = calls[-1]
+    assert name == "nova_group_norm_grad_v2"
+    assert args[16:18] == (4 * 5 * 8, 8)  # batch and pixel stride of x
+
+
+def test_norm_gradient_copies_what_no_strides_fit(calls):
+    x = cl(2, 8, 4, 5)
+    hooks = Hooks(lambda t: t.clone(memory_format=torch.contiguous_format))
+    with hooks:
+        y = unet_ops._GroupNorm.apply(x.requires_grad_(), None, None, None, (160, 8), 2, 1e-5, 0)
+        y.backward(torch.zeros_like(y))
+    assert calls[-1][1][0] not in [t.data_ptr() for t in hooks.given]  # NCHW memory
+
+
+def test_cross_gradient_takes_rows_as_hooks_hand_them_back(calls):
+    def heads_first(t):  # every 4-D tensor with its heads before its tokens, off 16 bytes
+        if t.dim() != 4:
+            return torch.stack([t, t], -1)[..., 0]
+        B, N, H, D = t.shape
+        return torch.zeros(B, H, N, D + 1, dtype=t.dtype)[..., 1:].transpose(1, 2)
+    q = torch.zeros(2, 3, 2, 16, dtype=torch.float16, requires_grad=True)
+    k = torch.zeros(2, 200, 2, 16, dtype=torch.float16)
+    hooks = Hooks(heads_first)
+    with hooks:
+        o = unet_ops._CrossAttention.apply(q, k, k, None, 0.25)
+        o.backward(torch.zeros_like(o))
+    name, args = calls[-1]
+    assert name == "nova_cross_attention_grad_v2"
+    given = [t.data_ptr() for t in hooks.given]
+    assert len(given) == 6  # q, k, v, o, low, lse
+    assert all(args[i] not in given for i in (0, 1, 2, 4, 5, 7))
+    dense = [200 * 32, 32, 16]
+    assert list(args[18]) == [3 * 32, 32, 16] + dense + dense + [0, 0] + [3 * 32, 32, 16]
+
+
+@pytest.mark.parametrize("again", [lambda t: t.double(), lambda t: t[:1], lambda t: t.to("meta")])
+def test_other_tensors_from_hooks_are_refused(calls, again):
+    x = cl(2, 8, 4, 5)
+    with Hooks(again):
+        y = unet_ops._GroupNorm.apply(x.requires_grad_(), None, None, None, (160, 8), 2, 1e-5, 0)
+        with pytest.raises(RuntimeError, match="hook"):
+            y.backward(torch.zeros_like(y))
+    q = torch.zeros(2, 3, 2, 16, dtype=torch.float16, requires_grad=True)
+    with Hooks(again):
+        o = unet_ops._CrossAttention.apply(q, q, q, None, 0.25)
+        with pytest.raises(RuntimeError, match="hook"):
+            o.backward(torch.zeros_like(o))
+    assert not any("grad" in c[0] for c in calls)
