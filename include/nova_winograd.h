@@ -203,7 +203,8 @@ enum { NOVA_ACT_NONE = 0, NOVA_ACT_SILU = 1 };
  * each may be NULL (1 and 0).  shift: [batch][C] of type shift_dtype, or NULL.
  * stats: float[2][batch][groups], mean and 1/sqrt(var + eps), for the gradient;
  * NULL where it is not wanted.  The caller passes a 256-byte aligned workspace
- * of nova_group_norm_workspace_bytes() bytes (NULL where that is 0); calls that
+ * of nova_group_norm_workspace_bytes() bytes (NULL where that is 0), which answers
+ * for the current device: ask with the operands' device current.  Calls that
  * overlap need one each.  aligned: all tensors and their strides are multiples of
  * 16 bytes (0 is always safe, and takes the narrow kernels' workspace).
  * Allocates nothing, never synchronizes, runs on `stream`; returns a NOVA_*

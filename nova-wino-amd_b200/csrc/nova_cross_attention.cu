@@ -24,8 +24,7 @@ long long workspace_bytes(int B, int Nq, int Nk, int H, int D, bool grad) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-int check(const char* what, const Args& a, int dtype, const void* ws, long long ws_bytes,
-          bool grad) {
+int check(const char* what, const Args& a, int dtype, bool grad) {
   auto bad = [&](const char* why) {
     return record_error(NOVA_ERR_INVALID_ARGUMENT, std::string(what) + ": " + why);
   };
@@ -48,9 +47,16 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
   if (a.mb < 0 || a.mn < 0) return bad("negative mask stride");
   const long long rows = (long long)a.B * a.H * (a.Nq > a.Nk ? a.Nq : a.Nk);
   if (rows > (1ll << 31) - 4096) return bad("more than 2^31 - 4096 rows");
+  return NOVA_OK;
+}
+
+// The workspace of checked arguments, by the current device: the operands' by then,
+// whose SMs the launch plans for.
+int check_workspace(const char* what, const Args& a, const void* ws, long long ws_bytes, bool grad) {
   const long long need = workspace_bytes(a.B, a.Nq, a.Nk, a.H, a.D, grad);
   if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 256))
-    return bad("workspace missing or not 256-byte aligned");
+    return record_error(NOVA_ERR_INVALID_ARGUMENT,
+                        std::string(what) + ": workspace missing or not 256-byte aligned");
   if (ws_bytes < need)
     return record_error(NOVA_ERR_WORKSPACE,
                         std::string(what) + ": workspace needs " + std::to_string(need) + " bytes");
@@ -93,8 +99,9 @@ NOVA_EXPORT int nova_cross_attention_v2(const void* d_q, const void* d_k, const 
   a.mb = t[9], a.mn = t[10];
   a.B = batch, a.Nq = queries, a.Nk = keys, a.H = heads, a.D = head_dim;
   a.mask_kind = mask_type, a.scale = scale;
-  if (const int rc = check("cross_attention", a, dtype, d_workspace, ws_bytes, false)) return rc;
+  if (const int rc = check("cross_attention", a, dtype, false)) return rc;
   const OnDeviceOf device(d_q);
+  if (const int rc = check_workspace("cross_attention", a, d_workspace, ws_bytes, false)) return rc;
   if (device.status() != cudaSuccess) return done("cross_attention: q", device.status());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const char* why = nullptr;
@@ -126,13 +133,14 @@ NOVA_EXPORT int nova_cross_attention_grad_v2(
   a.dos = {t[11], t[12], t[13]};
   a.B = batch, a.Nq = queries, a.Nk = keys, a.H = heads, a.D = head_dim;
   a.mask_kind = mask_type, a.scale = scale;
-  if (const int rc = check("cross_attention_grad", a, dtype, d_workspace, ws_bytes, true))
-    return rc;
+  if (const int rc = check("cross_attention_grad", a, dtype, true)) return rc;
   if (backward_reads_output(keys, head_dim) &&
       (!a.out || !a.low || !aligned16(a.out) || !aligned16(a.low)))
     return record_error(NOVA_ERR_INVALID_ARGUMENT,
                         "cross_attention_grad: these keys want output and low, 16-byte aligned");
   const OnDeviceOf device(d_q);
+  if (const int rc = check_workspace("cross_attention_grad", a, d_workspace, ws_bytes, true))
+    return rc;
   if (device.status() != cudaSuccess) return done("cross_attention_grad: q", device.status());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const char* why = nullptr;

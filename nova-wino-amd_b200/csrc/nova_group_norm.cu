@@ -1174,8 +1174,7 @@ bool wide(const Args& a, int dtype, bool grad) {
          (!grad || (a.yp % V == 0 && a.yb % V == 0 && aligned16(a.dy)));
 }
 
-int check(const char* what, const Args& a, int dtype, const void* ws, long long ws_bytes,
-          bool grad) {
+int check(const char* what, const Args& a, int dtype, bool grad) {
   auto bad = [&](const char* why) {
     return record_error(NOVA_ERR_INVALID_ARGUMENT, std::string(what) + ": " + why);
   };
@@ -1189,9 +1188,18 @@ int check(const char* what, const Args& a, int dtype, const void* ws, long long 
   if (!(a.eps >= 0.f)) return bad("eps must not be negative");
   if ((long long)a.B * a.HW > (1ll << 31) - 4096 || (long long)a.B * a.G > (1ll << 31) - 4096)
     return bad("more than 2^31 - 4096 pixels");
-  const long long need = workspace_bytes(a.B, a.HW, a.C, a.G, wide(a, dtype, grad) ? 16 / dtype_bytes(dtype) : 1, grad);
+  return NOVA_OK;
+}
+
+// The workspace of checked arguments, by the current device: the operands' by then,
+// whose SMs the launch plans for.
+int check_workspace(const char* what, const Args& a, int dtype, const void* ws, long long ws_bytes,
+                    bool grad) {
+  const int V = wide(a, dtype, grad) ? 16 / dtype_bytes(dtype) : 1;
+  const long long need = workspace_bytes(a.B, a.HW, a.C, a.G, V, grad);
   if (need > 0 && (!ws || reinterpret_cast<uintptr_t>(ws) % 256))
-    return bad("workspace missing or not 256-byte aligned");
+    return record_error(NOVA_ERR_INVALID_ARGUMENT,
+                        std::string(what) + ": workspace missing or not 256-byte aligned");
   if (ws_bytes < need)
     return record_error(NOVA_ERR_WORKSPACE,
                         std::string(what) + ": workspace needs " + std::to_string(need) + " bytes");
@@ -1227,10 +1235,11 @@ NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, co
   using namespace nova::gn;
   Args a{d_input, nullptr, d_weight, d_bias, d_shift, d_output, batch_stride, pixel_stride, 0, 0,
          batch, pixels, C, groups, groups > 0 ? C / groups : 0, param_dtype, shift_dtype, eps};
-  if (const int rc = check("group_norm", a, dtype, d_workspace, ws_bytes, false)) return rc;
+  if (const int rc = check("group_norm", a, dtype, false)) return rc;
   if (activation != kNone && activation != kSilu)
     return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm: bad activation");
   const OnDeviceOf device(d_input);
+  if (const int rc = check_workspace("group_norm", a, dtype, d_workspace, ws_bytes, false)) return rc;
   if (device.status() != cudaSuccess) return done("group_norm: input", device.status());
   unsigned char* ws = static_cast<unsigned char*>(d_workspace);
   float* stats = static_cast<float*>(d_stats);
@@ -1274,11 +1283,12 @@ NOVA_EXPORT int nova_group_norm_grad_v2(
   Args a{d_input, d_grad_output, d_weight, d_bias, d_shift, d_grad_input, batch_stride,
          pixel_stride, grad_batch_stride, grad_pixel_stride, batch, pixels, C, groups,
          groups > 0 ? C / groups : 0, param_dtype, shift_dtype, 0.f};
-  if (const int rc = check("group_norm_grad", a, dtype, d_workspace, ws_bytes, true)) return rc;
+  if (const int rc = check("group_norm_grad", a, dtype, true)) return rc;
   if (!d_stats) return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm_grad: null pointer");
   if (activation != kNone && activation != kSilu)
     return record_error(NOVA_ERR_INVALID_ARGUMENT, "group_norm_grad: bad activation");
   const OnDeviceOf device(d_input);
+  if (const int rc = check_workspace("group_norm_grad", a, dtype, d_workspace, ws_bytes, true)) return rc;
   if (device.status() != cudaSuccess) return done("group_norm_grad: input", device.status());
   unsigned char* ws = static_cast<unsigned char*>(d_workspace);
   const float* stats = static_cast<const float*>(d_stats);

@@ -39,11 +39,13 @@ def _fn(name):
 
 
 def _workspace(name, device, *sizes):
-    """Workspace of a call: the library says how much, the caching allocator gives it."""
-    key = (name, sizes)
+    """Workspace of a call: the library says how much, by the SMs of the device, the
+    caching allocator gives it."""
+    key = (name, device.index, sizes)
     n = _workspace_sizes.get(key)
     if n is None:
-        n = _fn(name)(*sizes)
+        with torch.cuda.device(device):
+            n = _fn(name)(*sizes)
         if n < 0:
             raise ValueError(f"bad sizes for {name[:-len('_workspace_bytes')]}: {sizes}")
         if len(_workspace_sizes) > 4096:

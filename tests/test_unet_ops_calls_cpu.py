@@ -114,3 +114,31 @@ def test_other_tensors_from_hooks_are_refused(calls, again):
         with pytest.raises(RuntimeError, match="hook"):
             o.backward(torch.zeros_like(o))
     assert not any("grad" in c[0] for c in calls)
+
+
+def test_workspace_sizes_are_asked_for_each_device(monkeypatch):
+    """Two devices may have another number of SMs, hence other splits: the size is
+    asked with the operands' device current, and kept for that device alone."""
+    current, asked = [0], []
+
+    class On:
+        def __init__(self, device):
+            self.index = device.index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *args):
+            current[0] = self.before
+
+    def size(*sizes):
+        asked.append((current[0], sizes))
+        return 0
+
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(unet_ops, "_fn", lambda name: size)
+    monkeypatch.setattr(unet_ops, "_workspace_sizes", {})
+    for index in (1, 0, 1, 2):
+        assert unet_ops._workspace("x_workspace_bytes", torch.device("cuda", index), 3, 4)[2] == 0
+    assert asked == [(1, (3, 4)), (0, (3, 4)), (2, (3, 4))]
+    assert current == [0]
