@@ -206,7 +206,7 @@ enum { NOVA_ACT_NONE = 0, NOVA_ACT_SILU = 1 };
  * of nova_group_norm_workspace_bytes() bytes (NULL where that is 0), which answers
  * for the current device: ask with the operands' device current.  Calls that
  * overlap need one each.  aligned: all tensors and their strides are multiples of
- * 16 bytes (0 is always safe, and takes the narrow kernels' workspace).
+ * 16 bytes (0: not known, which takes the larger workspace of both cases).
  * Allocates nothing, never synchronizes, runs on `stream`; returns a NOVA_*
  * status. */
 long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups, int dtype,

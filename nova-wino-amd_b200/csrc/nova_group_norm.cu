@@ -1221,8 +1221,11 @@ NOVA_EXPORT long long nova_group_norm_workspace_bytes(int batch, int pixels, int
   if (batch < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || !nova::unet::dtype_ok(dtype))
     return -1;
   const int V = 16 / nova::unet::dtype_bytes(dtype);
-  return nova::gn::workspace_bytes(batch, pixels, C, groups, aligned && C % V == 0 ? V : 1,
-                                   grad != 0);
+  const bool wide = C % V == 0;
+  // Where it is not known whether the operands are aligned: enough for both.
+  return std::max(
+      wide ? nova::gn::workspace_bytes(batch, pixels, C, groups, V, grad != 0) : 0,
+      wide && aligned ? 0 : nova::gn::workspace_bytes(batch, pixels, C, groups, 1, grad != 0));
 }
 
 NOVA_EXPORT int nova_group_norm_v2(const void* d_input, const void* d_weight, const void* d_bias,

@@ -4,7 +4,7 @@ call is recorded in place of being made."""
 import pytest
 import torch
 
-from nova_winograd import unet_ops
+from nova_winograd import ops, unet_ops
 
 
 @pytest.fixture
@@ -142,3 +142,13 @@ def test_workspace_sizes_are_asked_for_each_device(monkeypatch):
         assert unet_ops._workspace("x_workspace_bytes", torch.device("cuda", index), 3, 4)[2] == 0
     assert asked == [(1, (3, 4)), (0, (3, 4)), (2, (3, 4))]
     assert current == [0]
+
+
+@pytest.mark.parametrize("sizes", [(6, 5727, 2640, 8), (1, 9606, 1088, 16), (29, 7956, 1016, 4),
+                                   (8, 4096, 320, 32), (1, 64, 1280, 32)])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("grad", [0, 1])
+def test_workspace_for_unknown_alignment_does_for_both(sizes, dtype, grad):
+    lib = ops.load_library(ops._find_lib())
+    unknown, aligned = (lib.nova_group_norm_workspace_bytes(*sizes, dtype, a, grad) for a in (0, 1))
+    assert unknown >= aligned >= 0
