@@ -20,7 +20,7 @@
 //
 // Rounding.  P and dS are rounded to the element type once, for the products.
 // FP16's range is short for that: P is held 2^kLift times larger, and dS is scaled
-// by a power of two that follows the largest |dP| of the block's walk.
+// by a power of two that follows the largest |dP| and |delta| of the block's walk.
 //
 // What bounds it.  8 x 1024 queries x 8 heads x 80, 77 keys, FP16, forward and gradient:
 // 41 us.  One block to an SM, and a tile's steps follow one another; before arithmetic
@@ -310,6 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float sum = sums.x + sums.y;
     if (MODE == kBoth) red[half][r] = sum;
     if (!kBf16) {
+      // delta comes from all tiles, and may be far above this one's dP.
+      if (MODE != kBoth) top = fmaxf(top, fabsf(delta));
       // A row that is not finite has no say in the scale of the others.
       const uint32_t bits = isfinite(top) && isfinite(sum) ? __float_as_uint(top) : 0u;
       const uint32_t most = __reduce_max_sync(~0u, bits);
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t most = 0;
 #pragma unroll
       for (int w = 0; w < kThreads / 32; ++w) most = max(most, peak[w]);
-      const int ex = (int)(most >> 23) - 127;  // |dP| < 2^(ex + 1), |dS| < 2^(ex + 2)
+      const int ex = (int)(most >> 23) - 127;  // |dP|, |delta| < 2^(ex + 1), |dS| < 2^(ex + 2)
       if (!exp_set || exp_now > 13 - ex) {
         int to = 9 - ex;
         to = to > kMaxExp ? kMaxExp : to < -kMaxExp ? -kMaxExp : to;

@@ -74,3 +74,16 @@ def test_cross_with_saved_tensors_kept_elsewhere(hooks, Nk, mask):
     with hooks():
         got = cross_check(q, kv[:, :, 0], kv[:, :, 1], m, do)
     assert all(torch.equal(got[n], want[n]) for n in want)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D,Nk,tile", [(64, 300, 112), (160, 200, 80)])
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -12, 2.0 ** -6])
+def test_cross_values_small_in_one_tile_of_keys(dtype, D, Nk, tile, which, size):
+    """Padded encoder states through a projection without bias: v is zero, or far
+    smaller, for some keys.  What dP - delta comes to there is delta, from the others.
+    The bound's step of the smallest dS holds: |delta| is at most the largest |dp|."""
+    q, k, v, _, do = cross_case(2, 150, Nk, 2, D, dtype)
+    v[:, which * tile:(which + 1) * tile] *= size
+    cross_check(q, k, v, None, do)
