@@ -239,7 +239,8 @@ int nova_group_norm_grad_v2(const void* d_input, const void* d_grad_output, cons
  * k (grad_k, grad_v).  mask: [batch][keys]; a key with false, or with an additive
  * -inf, takes no part whatever k and v hold there, and a query without keys gets
  * zeros.  lse: float[batch][heads][queries], the base-2 logarithm of the softmax's
- * denominator, for the gradient; NULL where it is not wanted.  low: like output, what
+ * denominator relative to the sample's largest additive bias, for the gradient with
+ * the same mask; NULL where it is not wanted.  low: like output, what
  * its rounding left off; the gradient wants it, with output, for more than 128 keys
  * (80 where head_dim > 128), else both may be NULL there.  Workspace, stream and
  * status as above (a workspace of 0 bytes may be NULL).

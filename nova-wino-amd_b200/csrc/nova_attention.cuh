@@ -24,7 +24,8 @@ struct Args {
   const float* lse_in;
   void* out;   // o
   void* low;   // what the rounding of o left off, or null
-  float* lse;  // [B][H][Nq], base 2; minus infinity for a query without keys
+  float* lse;  // [B][H][Nq], base 2, relative to the sample's largest bias; minus
+               // infinity for a query without keys
   void *dq, *dk, *dv;
   const float* delta;  // [B][H][Nq]: sum(p dp)
   Strides qs, ks, vs, dos;
@@ -34,9 +35,18 @@ struct Args {
   float scale;
 };
 
-// Bias of key n in base 2, and whether the key takes part.  The lowest finite
-// bias stays finite after the change of base, so that a row with nothing else
-// is the uniform row that the definition gives.
+// An additive bias in base 2.  Above 2^126 the change of base gives way to a line that
+// ends at the largest finite value: finite biases stay finite and in their order, so
+// that a row with nothing but lowest values is the uniform row that 32 bits give.
+__device__ __forceinline__ float bias2(float m) {
+  constexpr float kFar = 8.507059173e37f, kMost = 3.402823466e38f;
+  const float far = fabsf(m);
+  if (!(far > kFar && far <= kMost)) return m * kLog2e;
+  const float t = fmaf(far - kFar, (kMost - kFar * kLog2e) / (kMost - kFar), kFar * kLog2e);
+  return copysignf(fminf(t, kMost), m);
+}
+
+// Bias of key n in base 2, and whether the key takes part.
 __device__ __forceinline__ bool key_bias(const Args& a, int b, int n, float* bias) {
   *bias = 0.f;
   if (a.mask_kind == kMaskNone) return true;
@@ -44,9 +54,35 @@ __device__ __forceinline__ bool key_bias(const Args& a, int b, int n, float* bia
   if (a.mask_kind == kMaskBool) return static_cast<const unsigned char*>(a.mask)[i] != 0;
   const float m = load_param(a.mask, a.mask_kind, i);
   if (m == -INFINITY) return false;
-  const float t = m * kLog2e;
-  *bias = t == -INFINITY ? -3.402823466e38f : t;
+  *bias = bias2(m);
   return true;
+}
+
+// The largest additive bias of sample b's keys i, i + step, ..., in base 2; minus
+// infinity for none.  What a row's logarithm is taken relative to: beside a bias that
+// all keys share (the lowest value, -1e9) the logarithm of the sum would be lost.
+__device__ __forceinline__ float largest_bias(const Args& a, int b, int i, int step) {
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int n = i; n < a.Nk; n += 8 * step) {
+    float m[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const long long at = n + (long long)u * step;
+      m[u] = at < a.Nk ? load_param(a.mask, a.mask_kind, b * a.mb + at * a.mn) : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top = fmaxf(top, m[u]);
+  }
+  return bias2(top);
+}
+__device__ __forceinline__ bool is_additive(const Args& a) {
+  return a.mask_kind != kMaskNone && a.mask_kind != kMaskBool;
+}
+__device__ __forceinline__ float warp_most(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  return v;
 }
 
 __device__ __forceinline__ float ex2(float x) {

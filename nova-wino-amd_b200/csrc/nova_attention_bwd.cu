@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ alignas(8) float bias[2][kRows];
   __shared__ float red[2][kRows];
   __shared__ uint32_t peak[kThreads / 32];
+  __shared__ float refs[kThreads / 32];  // largest biases of the sample, a part for each warp
   const int tid = threadIdx.x, half = tid >> 7, r = tid & (kRows - 1);
   const int warp = __shfl_sync(~0u, tid >> 5, 0);
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -206,6 +207,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_async_smem();
     }
   };
+  // lse is relative to the sample's largest bias.
+  float ref = 0.f;
+  if (MASK && is_additive(p.a)) {
+    const float part = warp_most(largest_bias(p.a, b, tid, kThreads));
+    if ((tid & 31) == 0) refs[warp] = part;
+    __syncthreads();
+    ref = refs[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 32; ++w) ref = fmaxf(ref, refs[w]);
+    if (ref == -INFINITY) ref = 0.f;  // no key takes part
+  }
   ok = wait_phase(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
   if (MASK && kWalkQ) {
     set_bias(kt_fix, 0);
@@ -279,6 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (MASK) {
             const float2 add = *reinterpret_cast<const float2*>(&bias[slot][col + e]);
             x = __ffma2_rn(x, make_float2(c, c), add);
+            x = __fadd2_rn(x, make_float2(-ref, -ref));
             if (MODE == kQueries) {  // K and V of a key that is out hold anything here
               if (add.x == -INFINITY) x.x = -INFINITY, dp.x = 0.f;
               if (add.y == -INFINITY) x.y = -INFINITY, dp.y = 0.f;

@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ alignas(8) float bias[kRows];
+  __shared__ float refs[kRows / 32];  // largest bias of the sample, a copy for each warp
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(~0u, tid >> 5, 0);  // the same for the warp, and known to be
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -252,9 +253,28 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
     const int chunks = p.KT / 16;
     int step = 0, turn_seen = -1;
     bool ok = true;
+    // Who reads lse wants the largest bias: the four warps look for the first sample's
+    // together (none of them can have given up yet), for a later one's each by itself.
+    const bool wants_ref = MASK && is_additive(p.a) && (p.a.lse || p.splits > 1);
+    int b_seen = head0 / p.a.H;
+    if (wants_ref) {
+      const float part = warp_most(largest_bias(p.a, b_seen, tid, kRows));
+      if (lane == 0) refs[warp] = part;
+      asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory");
+      float top = refs[0];
+#pragma unroll
+      for (int i = 1; i < kRows / 32; ++i) top = fmaxf(top, refs[i]);
+      asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory");
+      if (lane == 0) refs[warp] = top;
+    }
     for (int t = 0; t < tiles && ok; ++t) {
       const Spot at = spot(t);
       const int b = at.b, h = at.h;
+      if (wants_ref && b != b_seen) {
+        const float top = warp_most(largest_bias(p.a, b, lane, 32));
+        if (lane == 0) refs[warp] = top;
+        b_seen = b;
+      }
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < nk; ++j, ++step) {
         const int key0 = (k0 + j) * p.KT, keys = min(p.KT, p.a.Nk - key0);
@@ -419,7 +439,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
       // O / sum.
       const int row = at.n + tid;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const float lse = l == 0.f ? -INFINITY : m + log2f(l);
+      const float ref = wants_ref ? refs[warp] : 0.f;
+      const float lse = l == 0.f ? -INFINITY : m - ref + log2f(l);
       const long long lrow = ((long long)b * p.a.H + h) * p.a.Nq + row;
       if (p.splits > 1) {
         float* po = p.part_o + ((((long long)split * p.a.B + b) * p.a.Nq + row) * p.a.H + h) * p.a.D;
@@ -557,6 +578,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
   __shared__ float po[kTokenWarps][NQ][DB * 64];
   __shared__ float pm[kTokenWarps][NQ], pl[kTokenWarps][NQ];
   __shared__ float biases[MASK ? kTokenBiases : 1];
+  __shared__ float refs[kTokenWarps];  // largest biases of the sample, a part for each warp
   __shared__ float row[NQ][DB * 64], top_of[NQ], sum_of[NQ];  // of the block, not divided
   pdl_trigger();
   pdl_wait();
@@ -571,6 +593,12 @@ __global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
   const T* vp = static_cast<const T*>(a.v) + b * a.vs.b + h * a.vs.h + g * 8;
   const float c = a.scale * kLog2e;
   const uint4 none = make_uint4(0, 0, 0, 0);
+  const bool cluster = p.splits <= kTokenCluster;
+  const bool wants_ref = MASK && is_additive(a) && (a.lse || !cluster);
+  if (wants_ref) {
+    const float part = warp_most(largest_bias(a, b, threadIdx.x, kTokenWarps * 32));
+    if (lane == 0) refs[warp] = part;  // read behind the barriers below
+  }
 
   // Q as K is read: row g, elements 8 t of every 32.
   uint4 q[2 * DB];
@@ -714,7 +742,6 @@ __global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
       sum_of[i] = sum;
     }
   }
-  const bool cluster = p.splits <= kTokenCluster;
   if (cluster) {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -724,6 +751,10 @@ __global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
   // The cluster's rows, a share of them by every block; or this block's for the
   // joining kernel.
   const int ranks = cluster ? p.splits : 1, rank = cluster ? split : 0;
+  float ref = wants_ref ? refs[0] : 0.f;
+#pragma unroll
+  for (int w = 1; w < kTokenWarps; ++w)
+    if (wants_ref) ref = fmaxf(ref, refs[w]);
   for (int z = threadIdx.x * ranks + rank; z < a.Nq * DB * 64; z += kTokenWarps * 32 * ranks) {
     const int i = z / (DB * 64), d = z % (DB * 64);
     if (d >= a.D) continue;
@@ -753,7 +784,7 @@ __global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
     const float v = sum == 0.f ? 0.f : acc / sum;
     const long long at = ((long long)b * a.H + h) * a.Nq + i;
     const long long off = (((long long)b * a.Nq + i) * a.H + h) * a.D + d;
-    const float lse = sum == 0.f ? -INFINITY : top + log2f(sum);
+    const float lse = sum == 0.f ? -INFINITY : top - ref + log2f(sum);
     if (cluster) {
       const T r = from_f32<T>(v);
       static_cast<T*>(a.out)[off] = r;

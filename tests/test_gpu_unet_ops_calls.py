@@ -87,3 +87,68 @@ def test_cross_values_small_in_one_tile_of_keys(dtype, D, Nk, tile, which, size)
     q, k, v, _, do = cross_case(2, 150, Nk, 2, D, dtype)
     v[:, which * tile:(which + 1) * tile] *= size
     cross_check(q, k, v, None, do)
+
+
+# Biases that every key of a sample has, and beside which a score is less than half a
+# step of 32 bits: the softmax in 32 bits is uniform.
+SHARED = [(BF16, torch.finfo(BF16).min), (F32, torch.finfo(F32).min), (F32, -1e9), (F32, 3e38)]
+
+
+@pytest.mark.parametrize("mtype,low", SHARED)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,Nq,Nk,H,D", [
+    (2, 20, 50, 2, 32), (3, 300, 77, 8, 40),    # one tile of keys; many heads for a block
+    (1, 150, 300, 2, 64), (2, 70, 200, 2, 160),  # keys split, the last part shorter
+    (9, 260, 333, 20, 64),                       # several tiles, not split
+    (2, 1, 300, 3, 64), (1, 3, 9000, 2, 64),     # few queries: a cluster, blocks joined after
+])
+def test_cross_one_bias_for_all_keys(mtype, low, dtype, B, Nq, Nk, H, D):
+    q, k, v, _, do = cross_case(B, Nq, Nk, H, D, dtype, wide=0.5)
+    mask = torch.full((B, Nk), low, device="cuda", dtype=mtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = nova_cross_attention(*leaves, key_mask=mask)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)), o=o.detach())
+    # The uniform row in 64 bits: scores of zero.  dq knows q by them alone, dk knows k.
+    d = [t.double() for t in (q, k, v, do)]
+    flat = P.cross_attention(torch.zeros_like(d[0]), *d[1:3], None, D ** -0.5, d[3], dtype)
+    keys = P.cross_attention(d[0], torch.zeros_like(d[1]), d[2], None, D ** -0.5, d[3], dtype)
+    for name, want in (("o", flat), ("dq", flat), ("dv", flat), ("dk", keys)):
+        near(got[name], want[name], want[name + "_tol"], name)
+
+
+@pytest.mark.parametrize("low", [-1e4, -65504.0, -1e6])
+@pytest.mark.parametrize("Nq,Nk", [(64, 77), (64, 300), (4, 300)])
+def test_cross_probabilities_sum_to_one_beside_a_large_bias(low, Nq, Nk):
+    """do of ones: what dv comes to over the keys is the sum of all probabilities, Nq.
+    Each is rounded once, and dv once: 2 half steps of FP16, and 2^-16 for the sums."""
+    q, k, v, _, _ = cross_case(2, Nq, Nk, 2, 64, F16)
+    mask = torch.full((2, Nk), low, device="cuda", dtype=F32)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = nova_cross_attention(*leaves, key_mask=mask)
+    dv = torch.autograd.grad(o, leaves[2], torch.ones_like(o))[0]
+    # Probabilities of less than FP16's normal 2^-14 / 2^10 keep a step of 2^-34.
+    bound = Nq * (2 * P.half_step(F16) + 2.0 ** -16) + Nq * Nk * 2.0 ** -35
+    # dv below 2^-14 has steps of 2^-24.
+    bound += Nk * 2.0 ** -25
+    assert ((dv.double().sum(1) - Nq).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Nq,Nk", [(70, 77), (150, 300), (1, 300), (3, 9000)])
+def test_cross_far_biases_keep_their_order(dtype, Nq, Nk):
+    """Finite biases of any size count as the sums with them do in 32 bits: the larger
+    one takes all, the smaller nothing."""
+    q, k, v, _, do = cross_case(2, Nq, Nk, 2, 64, dtype, wide=0.5)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    take = torch.rand(2, Nk, generator=g, device="cuda") < 0.5
+    for high, low in ((-3.3e38, torch.finfo(F32).min), (-1e38, -2.5e38), (3.4e38, 2.4e38),
+                      (-8e37, -9e37)):
+        mask = torch.where(take, high, low).float()
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = nova_cross_attention(*leaves, key_mask=mask)
+        got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)), o=o.detach())
+        d = [t.double() for t in (q, k, v, do)]
+        flat = P.cross_attention(torch.zeros_like(d[0]), *d[1:3], take, 0.125, d[3], dtype)
+        keys = P.cross_attention(d[0], torch.zeros_like(d[1]), d[2], take, 0.125, d[3], dtype)
+        for name, want in (("o", flat), ("dq", flat), ("dv", flat), ("dk", keys)):
+            near(got[name], want[name], want[name + "_tol"], name)
