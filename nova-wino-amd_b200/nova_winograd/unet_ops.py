@@ -69,21 +69,12 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _save(ctx, *tensors):
-    """Saves a call's tensors for its gradient."""
-    ctx.save_for_backward(*tensors)
-    ctx.kinds = [None if t is None else (t.dtype, t.device, t.shape) for t in tensors]
-
-
-def _saved(ctx):
-    """What _save saved.  A saved-tensor hook (one that keeps them on the CPU
-    meanwhile, say) may hand back other strides, so these are asked anew."""
-    tensors = ctx.saved_tensors
-    for t, kind in zip(tensors, ctx.kinds):
-        if t is not None and (t.dtype, t.device, t.shape) != kind:
-            raise RuntimeError(f"a saved-tensor hook handed back {t.dtype} {list(t.shape)} on "
-                               f"{t.device} for {kind[0]} {list(kind[2])} on {kind[1]}")
-    return tensors
+def _expect(t, dtype, shape, device):
+    """Refuses a saved tensor that a hook (one that keeps it elsewhere meanwhile, say)
+    handed back as another.  Its strides may differ, and are asked anew."""
+    if t is not None and not (t.dtype is dtype and t.shape == shape and t.device == device):
+        raise RuntimeError(f"a saved-tensor hook handed back {t.dtype} {list(t.shape)} on "
+                           f"{t.device} for {dtype} {list(shape)} on {device}")
 
 
 def _dense(t):
@@ -153,8 +144,10 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, shift, strides, num_groups, eps, act):
         y, stats = _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, True)
-        _save(ctx, x, weight, bias, shift, stats)
+        param_type = weight.dtype if weight is not None else bias.dtype if bias is not None else None
+        ctx.save_for_backward(x, weight, bias, shift, stats)
         ctx.num_groups, ctx.act = num_groups, act
+        ctx.types = param_type, None if shift is None else shift.dtype
         return y
 
     @staticmethod
@@ -163,9 +156,15 @@ class _GroupNorm(torch.autograd.Function):
 
 
 def _norm_backward(ctx, dy):
-    x, *rest = _saved(ctx)
+    x, *rest = ctx.saved_tensors
     weight, bias, shift, stats = map(_dense, rest)
-    B, C, H, W = x.shape
+    B, C, H, W = dy.shape
+    device, (param_type, shift_type) = dy.device, ctx.types
+    _expect(x, dy.dtype, dy.shape, device)
+    _expect(weight, param_type, (C,), device)
+    _expect(bias, param_type, (C,), device)
+    _expect(shift, shift_type, (B, C), device)
+    _expect(stats, torch.float32, (2, B, ctx.num_groups), device)
     need = ctx.needs_input_grad
     dx = _empty_channels_last(x)
     dw = torch.empty_like(weight) if need[1] else None
@@ -349,8 +348,8 @@ class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale):
         out, low, lse = _cross_forward(q, k, v, mask, scale, True)
-        _save(ctx, q, k, v, mask, None if low is None else out, low, lse)
-        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, mask, None if low is None else out, low, lse)
+        ctx.scale, ctx.mask_dtype = scale, None if mask is None else mask.dtype
         return out
 
     @staticmethod
@@ -359,11 +358,17 @@ class _CrossAttention(torch.autograd.Function):
 
 
 def _cross_backward(ctx, do):
-    q, k, v, mask, *rest = _saved(ctx)
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    q, k, v, mask, *rest = ctx.saved_tensors
+    B, Nq, H, D = do.shape
+    Nk, dtype, device = k.shape[1], do.dtype, do.device
     out, low, lse = map(_dense, rest)
-    B, Nq, H, D = q.shape
-    Nk = k.shape[1]
+    for t in (q, out, low):
+        _expect(t, dtype, do.shape, device)
+    for t in (k, v):
+        _expect(t, dtype, (B, Nk, H, D), device)
+    _expect(mask, ctx.mask_dtype, (B, Nk), device)
+    _expect(lse, torch.float32, (B, H, Nq), device)
+    q, k, v = _rows(q), _rows(k), _rows(v)
     dq = torch.empty((B, Nq, H, D), dtype=q.dtype, device=q.device)
     dk = torch.empty((B, Nk, H, D), dtype=q.dtype, device=q.device)
     dv = torch.empty((B, Nk, H, D), dtype=q.dtype, device=q.device)
