@@ -302,12 +302,13 @@ def _one_tile(D):
 
 def _rows(t):
     """t [B, N, H, D] with its rows' elements next to each other and every row on 16
-    bytes: t itself where it lies so, else a contiguous copy."""
+    bytes: t itself where it lies so, else a contiguous copy (contiguous() alone may
+    return t: it looks neither at the start nor at the strides of single indices)."""
     sb, sn, sh, sd = t.stride()
     if (sd == 1 and sb % 8 == 0 and sn % 8 == 0 and sh % 8 == 0 and sn and
             t.data_ptr() % 16 == 0):
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(q, k, v, mask, *more):

@@ -152,3 +152,29 @@ def test_cross_far_biases_keep_their_order(dtype, Nq, Nk):
         keys = P.cross_attention(d[0], torch.zeros_like(d[1]), d[2], take, 0.125, d[3], dtype)
         for name, want in (("o", flat), ("dq", flat), ("dv", flat), ("dk", keys)):
             near(got[name], want[name], want[name + "_tol"], name)
+
+
+@pytest.mark.parametrize("Nq,Nk", [(1, 300), (70, 77), (130, 300)])
+@pytest.mark.parametrize("offset", [1, 4])
+def test_cross_contiguous_tensors_off_16_bytes(Nq, Nk, offset):
+    q, k, v, m, do = cross_case(2, Nq, Nk, 2, 40, F16, "bool")
+    want = cross_check(q, k, v, m, do)
+
+    def moved(t):
+        flat = torch.cat([t.new_zeros(offset), t.flatten()])
+        return flat[offset:].view(t.shape)
+    got = cross_check(*map(moved, (q, k, v)), m, moved(do))
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    # A gradient that comes back through a concatenation, at an odd element.
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = nova_cross_attention(*leaves, key_mask=m)
+    joined = torch.cat([torch.zeros(offset, device="cuda", dtype=F16), o.flatten()])
+    grads = torch.autograd.grad(joined, leaves, torch.cat([joined.new_zeros(offset), do.flatten()]))
+    assert all(torch.equal(g, want[n]) for g, n in zip(grads, ("dq", "dk", "dv")))
+    # One sample, one token, whose strides belong to the tensor that they are a part of.
+    wide = torch.zeros(3, Nk * 2 * 40 + 4, device="cuda", dtype=F16)
+    wide[0, :-4] = k[0].flatten()
+    one = wide[:1, :-4].view(1, Nk, 2, 40)
+    a = cross_check(q[:1], one, v[:1], m[:1], do[:1])
+    b = cross_check(q[:1].contiguous(), k[:1].contiguous(), v[:1], m[:1], do[:1])
+    assert all(torch.equal(a[n], b[n]) for n in a)

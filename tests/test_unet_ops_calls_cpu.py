@@ -152,3 +152,18 @@ def test_workspace_for_unknown_alignment_does_for_both(sizes, dtype, grad):
     lib = ops.load_library(ops._find_lib())
     unknown, aligned = (lib.nova_group_norm_workspace_bytes(*sizes, dtype, a, grad) for a in (0, 1))
     assert unknown >= aligned >= 0
+
+
+def test_rows_off_16_bytes_are_copied_although_contiguous():
+    flat = torch.arange(1 + 2 * 5 * 2 * 16, dtype=torch.float16)
+    t = flat[1:].view(2, 5, 2, 16)
+    assert t.is_contiguous() and t.data_ptr() % 16
+    one = torch.zeros(3, 5 * 2 * 16 + 4, dtype=torch.float16)[:1, :160].view(1, 5, 2, 16)
+    assert one.is_contiguous() and one.stride(0) % 8  # the stride of a single sample
+    token = torch.zeros(2, 1, 2, 16, dtype=torch.float16).as_strided((2, 1, 2, 16), (32, 3, 16, 1))
+    for x in (t, one, token):
+        y = unet_ops._rows(x)
+        assert torch.equal(x, y) and y.data_ptr() % 16 == 0
+        assert all(s % 8 == 0 for s in y.stride()[:3]) and y.stride(1) > 0
+    dense = torch.zeros(2, 5, 2, 16, dtype=torch.float16)
+    assert unet_ops._rows(dense) is dense
