@@ -172,9 +172,9 @@ def test_cross_contiguous_tensors_off_16_bytes(Nq, Nk, offset):
     grads = torch.autograd.grad(joined, leaves, torch.cat([joined.new_zeros(offset), do.flatten()]))
     assert all(torch.equal(g, want[n]) for g, n in zip(grads, ("dq", "dk", "dv")))
     # One sample, one token, whose strides belong to the tensor that they are a part of.
-    wide = torch.zeros(3, Nk * 2 * 40 + 4, device="cuda", dtype=F16)
-    wide[0, :-4] = k[0].flatten()
-    one = wide[:1, :-4].view(1, Nk, 2, 40)
+    wide = torch.zeros(3 * (Nk * 80 + 4), device="cuda", dtype=F16)
+    one = wide.as_strided((3, Nk, 2, 40), (Nk * 80 + 4, 80, 40, 1))[:1]
+    one.copy_(k[:1])
     a = cross_check(q[:1], one, v[:1], m[:1], do[:1])
     b = cross_check(q[:1].contiguous(), k[:1].contiguous(), v[:1], m[:1], do[:1])
     assert all(torch.equal(a[n], b[n]) for n in a)

@@ -158,7 +158,7 @@ def test_rows_off_16_bytes_are_copied_although_contiguous():
     flat = torch.arange(1 + 2 * 5 * 2 * 16, dtype=torch.float16)
     t = flat[1:].view(2, 5, 2, 16)
     assert t.is_contiguous() and t.data_ptr() % 16
-    one = torch.zeros(3, 5 * 2 * 16 + 4, dtype=torch.float16)[:1, :160].view(1, 5, 2, 16)
+    one = torch.zeros(3 * 164, dtype=torch.float16).as_strided((3, 5, 2, 16), (164, 32, 16, 1))[:1]
     assert one.is_contiguous() and one.stride(0) % 8  # the stride of a single sample
     token = torch.zeros(2, 1, 2, 16, dtype=torch.float16).as_strided((2, 1, 2, 16), (32, 3, 16, 1))
     for x in (t, one, token):
