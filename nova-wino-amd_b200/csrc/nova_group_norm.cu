@@ -187,6 +187,10 @@ __device__ __forceinline__ Place place(const Args& a, const Walk& k) {
 __device__ __forceinline__ int chunk_pixels(const Args& a, const Walk& k, int chunk) {
   return min(a.HW - chunk * k.per, k.per);
 }
+// One past its last pixel.  The chunks may reach past 2^31, no pixel does.
+__device__ __forceinline__ int chunk_end(const Args& a, const Walk& k, int chunk) {
+  return chunk * k.per + chunk_pixels(a, k, chunk);
+}
 __device__ __forceinline__ int row_pixels(const Args& a, const Walk& k, int chunk, int r) {
   const int left = chunk_pixels(a, k, chunk) - r;
   return left > 0 ? (left + k.ty - 1) / k.ty : 0;
@@ -206,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksForward) partial_stats(Args a
   if (n) {
     const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
     bool fresh = true;
-    const int end = min(a.HW, (q.chunk + 1) * k.per);
+    const int end = chunk_end(a, k, q.chunk);
     for (int p = q.chunk * k.per + q.ty; p < end; p += k.tile) {
       Pack<T, V> v[kAhead];
 #pragma unroll
@@ -331,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksForward) apply(Args a, Walk k
   __shared__ Chan<V> h;
   pdl_trigger();
   const Place q = place(a, k);
-  const int end = q.active ? min(a.HW, (q.chunk + 1) * k.per) : 0;
+  const int end = q.active ? chunk_end(a, k, q.chunk) : 0;
   int p = q.chunk * k.per + q.ty;
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   T* y = static_cast<T*>(a.y) + (long long)q.b * a.HW * a.C + q.col * V;
@@ -392,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksGrad) partial_grad(Args a, Wa
     const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
     const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
     constexpr int U = kAhead / 2;
-    const int end = min(a.HW, (q.chunk + 1) * k.per);
+    const int end = chunk_end(a, k, q.chunk);
     for (int p = q.chunk * k.per + q.ty; p < end; p += k.tile) {
       Pack<T, V> v[U], d[U];
 #pragma unroll
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksGrad) apply_grad(Args a, Walk
   const Place q = place(a, k);
   const int c0 = (q.col - q.tx) * V, cols = min(k.tx * V, a.C - c0);
   const long long plane = (long long)a.B * a.C, bc = (long long)q.b * a.C;
-  const int end = q.active ? min(a.HW, (q.chunk + 1) * k.per) : 0;
+  const int end = q.active ? chunk_end(a, k, q.chunk) : 0;
   int p = q.chunk * k.per + q.ty;
   const T* x = static_cast<const T*>(a.x) + q.b * a.xb + q.col * V;
   const T* dy = static_cast<const T*>(a.dy) + q.b * a.yb + q.col * V;
@@ -976,7 +980,7 @@ Walk make_walk(int B, int HW, int C, int G, int V, bool grad) {
   if (chunks > (rows + U - 1) / U) chunks = (rows + U - 1) / U;
   if (chunks < 1) chunks = 1;
   k.per = (int)((rows + chunks - 1) / chunks) * k.ty;
-  k.nchunk = (HW + k.per - 1) / k.per;
+  k.nchunk = (int)(((long long)HW + k.per - 1) / k.per);
   return k;
 }
 
@@ -1021,15 +1025,15 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
         // 4x76x64x70 19.1, streaming 14.8), on 32 blocks (1x128x120x120 in 4 groups 16.7,
         // streaming 14.7) or in rows of 80 bytes (1x320x128x128 29.4, streaming 21.4).
         double again = 0;
-        if (!grad && nv == most && tx * k.ty > kSlabThreads) {
+        if (!grad && nv == most && (long long)tx * k.ty > kSlabThreads) {
           k.ty = kSlabThreads / tx;
           again = 1.0 - (double)nv * k.ty / k.ppc;
           if (again > 0.5 || V != kAgain || tx * 16 < 128 ||
               (long long)B * k.nblk * cs * 4 < 3 * sms)
             continue;
         }
+        if ((long long)tx * k.ty > kSlabThreads || slab_smem(k, V, grad) > kSlabSmem) continue;
         k.threads = (tx * k.ty + 31) / 32 * 32;
-        if (k.threads > kSlabThreads || slab_smem(k, V, grad) > kSlabSmem) continue;
         // The resident form pays while its blocks fit the SMs at once (twice at most in
         // the gradient, whose streaming form has four launches): its phases do not
         // overlap, so further waves cost it more than the second read it saves.
@@ -1174,6 +1178,12 @@ bool wide(const Args& a, int dtype, bool grad) {
          (!grad || (a.yp % V == 0 && a.yb % V == 0 && aligned16(a.dy)));
 }
 
+// Pixels, and groups of all samples, are counted in 32 bits.
+bool too_many(int B, int HW, int G) {
+  constexpr long long kMost = (1ll << 31) - 4096;
+  return (long long)B * HW > kMost || (long long)B * G > kMost;
+}
+
 int check(const char* what, const Args& a, int dtype, bool grad) {
   auto bad = [&](const char* why) {
     return record_error(NOVA_ERR_INVALID_ARGUMENT, std::string(what) + ": " + why);
@@ -1186,8 +1196,7 @@ int check(const char* what, const Args& a, int dtype, bool grad) {
   if (a.xp < a.C || a.xb < 0 || (grad && (a.yp < a.C || a.yb < 0)))
     return bad("a pixel stride below the channels, or a negative batch stride");
   if (!(a.eps >= 0.f)) return bad("eps must not be negative");
-  if ((long long)a.B * a.HW > (1ll << 31) - 4096 || (long long)a.B * a.G > (1ll << 31) - 4096)
-    return bad("more than 2^31 - 4096 pixels");
+  if (too_many(a.B, a.HW, a.G)) return bad("more than 2^31 - 4096 pixels or groups");
   return NOVA_OK;
 }
 
@@ -1218,7 +1227,8 @@ int done(const char* what, cudaError_t e) {
 
 NOVA_EXPORT long long nova_group_norm_workspace_bytes(int batch, int pixels, int C, int groups,
                                                       int dtype, int aligned, int grad) {
-  if (batch < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups || !nova::unet::dtype_ok(dtype))
+  if (batch < 1 || pixels < 1 || C < 1 || groups < 1 || C % groups ||
+      !nova::unet::dtype_ok(dtype) || nova::gn::too_many(batch, pixels, groups))
     return -1;
   const int V = 16 / nova::unet::dtype_bytes(dtype);
   const bool wide = C % V == 0;

@@ -178,3 +178,49 @@ def test_cross_contiguous_tensors_off_16_bytes(Nq, Nk, offset):
     a = cross_check(q[:1], one, v[:1], m[:1], do[:1])
     b = cross_check(q[:1].contiguous(), k[:1].contiguous(), v[:1], m[:1], do[:1])
     assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+def test_norm_of_the_most_pixels():
+    """2^31 - 4096 pixels of one channel, the last of them too; piece by piece in 64 bits."""
+    H, W = 524287, 4096
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty(1, 1, H, W, device="cuda", dtype=F16)
+    dy = torch.empty(1, 1, H, W, device="cuda", dtype=F16)
+    pieces = [slice(i, min(i + 16384, H)) for i in range(0, H, 16384)]
+    for p in pieces:
+        for t, at in ((x, 0.5), (dy, 0.25)):
+            t[:, :, p] = torch.randn(1, 1, p.stop - p.start, W, generator=g, device="cuda") + at
+    w = torch.tensor([1.25], device="cuda", requires_grad=True)
+    b = torch.tensor([-0.5], device="cuda", requires_grad=True)
+    x.requires_grad_()
+    y = nova_group_norm(x, 1, w, b, 1e-5, "silu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    x, y = x.detach(), y.detach()
+    n = H * W
+    mean = sum(x[:, :, p].double().sum() for p in pieces) / n
+    r = (sum((x[:, :, p].double() - mean).square().sum() for p in pieces) / n + 1e-5) ** -0.5
+
+    def step(p):
+        m = (x[:, :, p].double() - mean) * r
+        z = m * 1.25 - 0.5
+        s = torch.sigmoid(z)
+        dz = dy[:, :, p].double() * s * (1 + z * (1 - s))
+        return m, z, s, dz
+    A = D = size = sized = 0.0
+    for p in pieces:
+        m, z, s, dz = step(p)
+        A, D = A + dz.sum(), D + (dz * m).sum()
+        size, sized = size + dz.abs().sum(), sized + (dz * m).abs().sum()
+    near(db[0], A, P.half_step(F32) * A.abs() + 2 * P.SUM * P.F32 * size, "db")
+    near(dw[0], D, P.half_step(F32) * D.abs() + 2 * P.SUM * P.F32 * sized, "dw")
+    for p in pieces:
+        m, z, s, dz = step(p)
+        m_off = P.OPS * P.F32 * (m.abs() + mean.abs() * r)
+        z_off = 1.25 * m_off + P.OPS * P.F32 * (z.abs() + 0.5)
+        near(y[:, :, p], z * s, P.rounded(F16, z * s) + 1.1 * z_off + P.OPS * P.F32 * (z * s).abs(), "y")
+        want = r * (1.25 * dz - 1.25 * A / n - m * 1.25 * D / n)
+        off = r * (1.25 * dy[:, :, p].double().abs() * (0.5 * z_off + P.OPS * P.F32)
+                   + 2 * P.SUM * P.F32 * 1.25 * (size + m.abs() * sized) / n
+                   + m_off * (1.25 * D / n).abs()
+                   + P.OPS * P.F32 * 1.25 * (dz.abs() + (A / n).abs() + (m * D / n).abs()))
+        near(dx[:, :, p], want, P.rounded(F16, want) + off + 1e-12, "dx")

@@ -167,3 +167,21 @@ def test_rows_off_16_bytes_are_copied_although_contiguous():
         assert all(s % 8 == 0 for s in y.stride()[:3]) and y.stride(1) > 0
     dense = torch.zeros(2, 5, 2, 16, dtype=torch.float16)
     assert unet_ops._rows(dense) is dense
+
+
+@pytest.mark.parametrize("B,HW,C,G", [(1, 2 ** 31 - 4096, 1, 1), (1, 2 ** 31 - 4096, 24, 3),
+                                      (1, 2 ** 31 - 4096, 4, 2), (3, 715826517, 2, 2),
+                                      (2 ** 31 - 4096, 1, 1, 1), (2 ** 20, 2047, 8, 2)])
+def test_workspace_of_the_most_pixels(B, HW, C, G):
+    """Up to 2^31 - 4096 pixels and groups; a part of 12 bytes at most for a channel of
+    a block, of which a sample has at most 8 for each of 148 SMs, and the samples' sums."""
+    size = ops.load_library(ops._find_lib()).nova_group_norm_workspace_bytes
+    assert B * HW <= 2 ** 31 - 4096
+    for dtype in (0, 1, 2):
+        for aligned in (0, 1):
+            for grad in (0, 1):
+                n = size(B, HW, C, G, dtype, aligned, grad)
+                assert 0 <= n <= 12 * C * (B + max(B, 8 * 148)) + 512
+    assert size(1, 2 ** 31 - 4095, 1, 1, 0, 0, 0) == -1
+    assert size(2 ** 16, 2 ** 16, 1, 1, 0, 0, 0) == -1
+    assert size(2 ** 27, 1, 64, 32, 0, 0, 0) == -1
