@@ -8,7 +8,7 @@
 
 No reference counterpart: the reference's UNet callers leave both to the host
 framework (Jayluci4/nova-wino-amd ``benchmarks/bench_sd_unet.py:38-109``).  Both
-are differentiable once, run on the caller's current CUDA stream, allocate through
+are differentiable once (backwards: a tangent is refused), run on the caller's current CUDA stream, allocate through
 torch's caching allocator only and never synchronize, so both can be captured
 into a CUDA graph.  Like the rest of the package they have no CPU fallback.
 """
@@ -17,6 +17,7 @@ import ctypes
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from nova_winograd.conv2d import _raw_stream
 from nova_winograd.ops import check, get_lib
@@ -75,6 +76,15 @@ def _expect(t, dtype, shape, device):
     if t is not None and not (t.dtype is dtype and t.shape == shape and t.device == device):
         raise RuntimeError(f"a saved-tensor hook handed back {t.dtype} {list(t.shape)} on "
                            f"{t.device} for {dtype} {list(shape)} on {device}")
+
+
+def _differentiated(*tensors):
+    """Whether a call goes through its autograd function: a gradient is wanted, or a
+    dual level is open, in which the function refuses an input that has a tangent
+    (torch counts the open levels from -1)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _dense(t):
@@ -247,10 +257,7 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
     if not x.is_cuda:
         raise ValueError("x must be a CUDA tensor")
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (x.requires_grad
-                                    or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)
-                                    or (shift is not None and shift.requires_grad)):
+    if _differentiated(x, weight, bias, shift):
         return _GroupNorm.apply(x, weight, bias, shift, strides, num_groups, eps, act)
     return _norm_forward(x, strides, num_groups, weight, bias, eps, act, shift, False)[0]
 
@@ -441,6 +448,6 @@ def nova_cross_attention(q, k, v, key_mask=None, scale=None):
         raise ValueError("q, k and v must be CUDA tensors")
     scale = D ** -0.5 if scale is None else float(scale)
     q, k, v = _rows(q), _rows(k), _rows(v)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if _differentiated(q, k, v):
         return _CrossAttention.apply(q, k, v, key_mask, scale)
     return _cross_forward(q, k, v, key_mask, scale, False)[0]

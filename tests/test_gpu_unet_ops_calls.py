@@ -4,6 +4,7 @@ Bounds are unet_ops_plain's."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import unet_ops_plain as P
 from nova_winograd import nova_cross_attention, nova_group_norm
@@ -224,3 +225,24 @@ def test_norm_of_the_most_pixels():
                    + m_off * (1.25 * D / n).abs()
                    + P.OPS * P.F32 * 1.25 * (dz.abs() + (A / n).abs() + (m * D / n).abs()))
         near(dx[:, :, p], want, P.rounded(F16, want) + off + 1e-12, "dx")
+
+
+def test_tangents_are_refused():
+    x, w, b, s, _ = norm_case(2, 32, 4, 6, 6, F16, shift=F16)
+    q, k, v, m, _ = cross_case(2, 9, 20, 2, 16, F16, "f32")
+    want = nova_group_norm(x, 4, w, b, shift=s), nova_cross_attention(q, k, v, key_mask=m)
+    with forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for i in range(4):
+            a = [x, w, b, s]
+            a[i] = dual(a[i])
+            with pytest.raises(NotImplementedError):
+                nova_group_norm(a[0], 4, a[1], a[2], shift=a[3])
+        for i in range(4):
+            a = [q, k, v, m]
+            a[i] = dual(a[i])
+            with pytest.raises(NotImplementedError):
+                nova_cross_attention(*a[:3], key_mask=a[3])
+        got = nova_group_norm(x, 4, w, b, shift=s), nova_cross_attention(q, k, v, key_mask=m)
+    assert all(torch.equal(g, t) for g, t in zip(got, want))

@@ -3,6 +3,7 @@ call is recorded in place of being made."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from nova_winograd import ops, unet_ops
 
@@ -185,3 +186,26 @@ def test_workspace_of_the_most_pixels(B, HW, C, G):
     assert size(1, 2 ** 31 - 4095, 1, 1, 0, 0, 0) == -1
     assert size(2 ** 16, 2 ** 16, 1, 1, 0, 0, 0) == -1
     assert size(2 ** 27, 1, 64, 32, 0, 0, 0) == -1
+
+
+def test_tangents_reach_the_functions_that_refuse_them(calls):
+    x, q = cl(2, 8, 4, 5), torch.zeros(2, 3, 2, 16, dtype=torch.float16)
+    assert not unet_ops._differentiated(x, None)
+    for grad in (False, True):
+        with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+            dual = forward_ad.make_dual(x, torch.ones_like(x))
+            assert unet_ops._differentiated(dual, None)
+            with pytest.raises(NotImplementedError):
+                unet_ops._GroupNorm.apply(dual, None, None, None, (160, 8), 2, 1e-5, 0)
+            dual = forward_ad.make_dual(q, torch.ones_like(q))
+            for at in range(3):
+                qkv = [q, q, q]
+                qkv[at] = dual
+                with pytest.raises(NotImplementedError):
+                    unet_ops._CrossAttention.apply(*qkv, None, 0.25)
+            # Without a tangent the level changes nothing.
+            assert unet_ops._GroupNorm.apply(x, None, None, None, (160, 8), 2, 1e-5, 0).shape == x.shape
+    x.requires_grad_()
+    assert unet_ops._differentiated(None, x)
+    with torch.no_grad():
+        assert not unet_ops._differentiated(None, x)
