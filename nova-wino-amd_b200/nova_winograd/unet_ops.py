@@ -4,7 +4,8 @@
     nova_group_norm        group normalisation with its activation on channels-last
                            activations, a per-sample channel shift added first
     nova_cross_attention   attention of one set of tokens to an encoder's states
-    NovaGroupNorm          module form of the norm, drop-in for ``nn.GroupNorm``
+    NovaGroupNorm          module form of the norm, drop-in for ``nn.GroupNorm`` of
+                           [B, C, H, W]
 
 No reference counterpart: the reference's UNet callers leave both to the host
 framework (Jayluci4/nova-wino-amd ``benchmarks/bench_sd_unet.py:38-109``).  Both
@@ -26,7 +27,8 @@ DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 MASK_NONE, MASK_BOOL = -1, 3
 ACTIVATIONS = {None: 0, "silu": 1}
 MAX_HEAD_DIM = 160
-_MOST = 2 ** 31 - 4096  # pixels or rows that the library counts in 32 bits
+MAX_GROUP_CHANNELS = 8192
+_MOST = 2 ** 31 - 4096  # pixels, groups or rows that the library counts in 32 bits
 
 _fns, _workspace_sizes = {}, {}
 
@@ -219,7 +221,7 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
         x:          [B, C, H, W] float16, bfloat16 or float32 CUDA tensor in
                     channels-last layout, or a channel slice of one (channels next to
                     each other, pixels evenly spaced).
-        num_groups: number of groups; divides C.
+        num_groups: number of groups; divides C, at most 8192 channels each.
         weight, bias: [C] float16, bfloat16 or float32, both of one type, or None.
         eps:        added to the variance.
         activation: None or "silu".
@@ -237,6 +239,8 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
     B, C, H, W = x.shape
     if num_groups < 1 or C < 1 or C % num_groups:
         raise ValueError(f"{C} channels do not divide into {num_groups} groups")
+    if C // num_groups > MAX_GROUP_CHANNELS:
+        raise ValueError(f"more than {MAX_GROUP_CHANNELS} channels per group: {C // num_groups}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be None or 'silu', got {activation!r}")
     if not eps >= 0:
@@ -244,8 +248,8 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
     strides = _pixel_strides(x)
     if strides is None:
         raise ValueError("x must be channels-last (torch.channels_last, or channels of one)")
-    if B * H * W > _MOST:
-        raise ValueError("x must have fewer than 2^31 - 4096 pixels")
+    if B * H * W > _MOST or B * num_groups > _MOST:
+        raise ValueError("x must have at most 2^31 - 4096 pixels, and as many groups in all")
     if weight is not None:
         weight = _check_param("weight", weight, (C,), x.device)
     if bias is not None:
@@ -263,7 +267,7 @@ def nova_group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=
 
 
 class NovaGroupNorm(nn.GroupNorm):
-    """``nn.GroupNorm`` with its activation fused in, on ``nova_group_norm``.
+    """``nn.GroupNorm`` of [B, C, H, W] with its activation fused in, on ``nova_group_norm``.
 
     Channels-last input gives channels-last output.  Contiguous NCHW input goes
     through an on-device copy to channels-last and back.
@@ -433,7 +437,7 @@ def nova_cross_attention(q, k, v, key_mask=None, scale=None):
     if D % 8 or not 8 <= D <= MAX_HEAD_DIM:
         raise ValueError(f"head width must be a multiple of 8 up to {MAX_HEAD_DIM}, got {D}")
     if B * H * max(Nq, Nk) > _MOST:
-        raise ValueError("q, k and v must have fewer than 2^31 - 4096 rows")
+        raise ValueError("q, k and v must have at most 2^31 - 4096 rows")
     if key_mask is not None:
         if key_mask.dtype != torch.bool and key_mask.dtype not in DTYPES:
             raise TypeError(f"key_mask must be bool, float16, bfloat16 or float32, got "

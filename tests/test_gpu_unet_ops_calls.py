@@ -246,3 +246,8 @@ def test_tangents_are_refused():
                 nova_cross_attention(*a[:3], key_mask=a[3])
         got = nova_group_norm(x, 4, w, b, shift=s), nova_cross_attention(q, k, v, key_mask=m)
     assert all(torch.equal(g, t) for g, t in zip(got, want))
+
+
+def test_norm_of_the_most_channels_in_a_group():
+    norm_check(*norm_case(2, 2 * 8192, 2, 3, 3, F16, shift=F16), 2, "silu")
+    norm_check(*norm_case(1, 8192, 1, 5, 1, F32), 1, None)

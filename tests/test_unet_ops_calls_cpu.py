@@ -209,3 +209,14 @@ def test_tangents_reach_the_functions_that_refuse_them(calls):
     assert unet_ops._differentiated(None, x)
     with torch.no_grad():
         assert not unet_ops._differentiated(None, x)
+
+
+def test_norm_refuses_what_the_library_would():
+    x = torch.empty(1, 2 * 8193, 1, 1, dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="8192 channels"):
+        unet_ops.nova_group_norm(x, 2)
+    many = torch.empty(2 ** 26, 64, 1, 1, dtype=torch.float16, device="meta")
+    with pytest.raises(ValueError, match="groups"):
+        unet_ops.nova_group_norm(many, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        unet_ops.nova_group_norm(torch.empty(1, 2 * 8192, 1, 1, dtype=torch.float16, device="meta"), 2)
