@@ -239,12 +239,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float v = p.a.lse_in[row0 + row];
     return v == -INFINITY ? INFINITY : v;
   };
-  auto row_delta = [&](int t) {
-    const int row = t * kRows + r;
-    return row < p.a.Nq ? p.a.delta[row0 + row] : 0.f;
+  auto row_delta = [&](int t, float row_lse) {
+    return row_lse == INFINITY ? 0.f : p.a.delta[row0 + t * kRows + r];
   };
   float lse = row_lse(t_first);
-  float delta = MODE == kBoth ? 0.f : row_delta(t_first);
+  float delta = MODE == kBoth ? 0.f : row_delta(t_first, lse);
 
   int i = 0;
   for (; i < steps; ++i) {  // leaves early only where all threads do
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float lse_next = 0.f, delta_next = 0.f;
     if (kWalkQ && i + 1 < steps) {
       lse_next = row_lse(t_first + i + 1);
-      if (MODE == kKeys) delta_next = row_delta(t_first + i + 1);
+      if (MODE == kKeys) delta_next = row_delta(t_first + i + 1, lse_next);
     }
     ok = wait_phase(bs, i & 1, &abort_flag, &g_status, kDevTimeoutMma);
     __syncwarp();
@@ -276,6 +275,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     tmem_wait_ld();
     tc_fence_before();
+    // A row without keys passes nothing on, whatever q and do hold there.
+    if (MASK && __any_sync(~0u, lse == INFINITY)) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (u < count && lse == INFINITY) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[u][e] = g[u][e] = 0u;
+        }
+    }
     float2 sums = make_float2(0.f, 0.f);
     float top = 0.f;
 #pragma unroll

@@ -251,3 +251,23 @@ def test_tangents_are_refused():
 def test_norm_of_the_most_channels_in_a_group():
     norm_check(*norm_case(2, 2 * 8192, 2, 3, 3, F16, shift=F16), 2, "silu")
     norm_check(*norm_case(1, 8192, 1, 5, 1, F32), 1, None)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("mask", ["bool", "f32"])
+@pytest.mark.parametrize("Nk", [77, 300])
+@pytest.mark.parametrize("poison", [float("nan"), INF])
+def test_cross_sample_without_keys_passes_nothing_on(dtype, mask, Nk, poison):
+    """A padded sample: its queries and what comes back for them may hold anything."""
+    q, k, v, m, do = cross_case(3, 150, Nk, 2, 64, dtype, mask)
+    want = cross_check(q, k, v, m, do)
+    for bad in ((q,), (do,), (q, k, v, do)):
+        held = [t[1].clone() for t in bad]
+        for t in bad:
+            t[1] = poison
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = nova_cross_attention(*leaves, key_mask=m)
+        got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)), o=o.detach())
+        assert all(torch.equal(got[n], want[n]) and (got[n][1] == 0).all() for n in want)
+        for t, h in zip(bad, held):
+            t[1] = h
