@@ -253,6 +253,13 @@ def test_norm_of_the_most_channels_in_a_group():
     norm_check(*norm_case(1, 8192, 1, 5, 1, F32), 1, None)
 
 
+@pytest.mark.parametrize("B,C,G,H,W", [(2, 12000, 2, 3, 3), (2, 16384, 2, 30, 30), (1, 5000, 1, 4, 4),
+                                       (4, 1024, 1, 40, 41), (2, 2048, 1, 64, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_norm_of_many_channels_in_a_group(B, C, G, H, W, dtype):
+    norm_check(*norm_case(B, C, G, H, W, dtype, shift=dtype), G, "silu")
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("mask", ["bool", "f32"])
 @pytest.mark.parametrize("Nk", [77, 300])
