@@ -7,8 +7,9 @@ import ctypes
 import pytest
 import torch
 
+import unet_ops_plain as P
 from nova_winograd import nova_cross_attention, nova_group_norm, ops, unet_ops
-from test_gpu_unet_ops import cross_case, norm_case
+from test_gpu_unet_ops import cross_case, near, norm_case
 
 pytestmark = pytest.mark.gpu
 
@@ -120,3 +121,44 @@ def test_cross_writes_within_its_buffers(B, Nq, Nk, H, D, mask, dtype):
     g.intact()
     for got, t in zip((dq, dk, dv), want):
         assert torch.equal(got, t)
+
+
+def test_norm_offsets_past_32_bits():
+    """4.4 billion elements: the first and the last group, each against its plain form."""
+    C, G, H, W, c = 520, 130, 2048, 4096, 4
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, dy = (torch.empty(1, H, W, C, device="cuda", dtype=F16).normal_(generator=g).permute(0, 3, 1, 2)
+             for _ in range(2))
+    w, b = (torch.randn(C, generator=g, device="cuda") for _ in range(2))
+    s = torch.randn(1, C, generator=g, device="cuda")
+    leaves = [t.requires_grad_() for t in (x, w, b, s)]
+    y = nova_group_norm(*leaves[:1], G, w, b, 1e-5, "silu", s)
+    dx, dw, db, ds = torch.autograd.grad(y, leaves, dy)
+    for part in (slice(0, c), slice(C - c, C)):
+        d = [t.detach().double() for t in (x[:, part], w[part], b[part], s[:, part], dy[:, part])]
+        want = P.group_norm(d[0], 1, d[1], d[2], 1e-5, "silu", d[3], d[4], (F16, F32, F32))
+        for name, t in (("y", y.detach()[:, part]), ("dx", dx[:, part]), ("dw", dw[part]),
+                        ("db", db[part]), ("ds", ds[:, part])):
+            near(t, want[name], want[name + "_tol"], name)
+
+
+def test_cross_offsets_past_32_bits():
+    """4.8 billion elements of q; the last queries are those that have a gradient."""
+    Nq, Nk, H, D, n = 2 ** 22 + 128, 9, 16, 72, 256
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.empty(1, Nq, H, D, device="cuda", dtype=BF16).normal_(generator=g)
+    k, v = (torch.empty(1, Nk, H, D, device="cuda", dtype=BF16).normal_(generator=g) for _ in range(2))
+    do = torch.zeros_like(q)
+    do[:, -n:] = torch.randn(1, n, H, D, generator=g, device="cuda")
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = nova_cross_attention(*leaves)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    last = [t.detach()[:, -n:] for t in (q, do)]
+    part = [t.detach().clone().requires_grad_() for t in (last[0], k, v)]
+    alone = nova_cross_attention(*part)
+    assert torch.equal(o.detach()[:, -n:], alone.detach())
+    assert torch.equal(dq[:, -n:], torch.autograd.grad(alone, part[0], last[1])[0])
+    assert not dq[:, :-n].any()
+    want = P.cross_attention(*(t.detach().double() for t in part), None, D ** -0.5, last[1].double(), BF16)
+    near(dk, want["dk"], want["dk_tol"], "dk")
+    near(dv, want["dv"], want["dv_tol"], "dv")
