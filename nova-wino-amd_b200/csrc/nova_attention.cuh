@@ -61,20 +61,34 @@ __device__ __forceinline__ bool key_bias(const Args& a, int b, int n, float* bia
 // The largest additive bias of sample b's keys i, i + step, ..., in base 2; minus
 // infinity for none.  What a row's logarithm is taken relative to: beside a bias that
 // all keys share (the lowest value, -1e9) the logarithm of the sum would be lost.
-__device__ __forceinline__ float largest_bias(const Args& a, int b, int i, int step) {
+// Not inlined: few calls need it, and its code would keep the others' from the
+// instruction cache (8 x 1024 queries to 77 keys, forward and gradient: 43.5 us for 41.5).
+template <typename T>
+__device__ __forceinline__ float most_of(const T* m, long long mn, int keys, int i, int step) {
   float top = -INFINITY;
 #pragma unroll 1
-  for (int n = i; n < a.Nk; n += 8 * step) {
-    float m[8];
+  for (int n = i; n < keys; n += 8 * step) {
+    T v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const long long at = n + (long long)u * step;
-      m[u] = at < a.Nk ? load_param(a.mask, a.mask_kind, b * a.mb + at * a.mn) : -INFINITY;
+      v[u] = m[(at < keys ? at : n) * mn];
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) top = fmaxf(top, m[u]);
+    for (int u = 0; u < 8; ++u) top = fmaxf(top, to_f32(v[u]));
   }
+  return top;
+}
+static __device__ __noinline__ float largest_bias(const void* mask, int kind, long long from,
+                                                  long long mn, int keys, int i, int step) {
+  const float top =
+      kind == kF32   ? most_of(static_cast<const float*>(mask) + from, mn, keys, i, step)
+      : kind == kF16 ? most_of(static_cast<const __half*>(mask) + from, mn, keys, i, step)
+                     : most_of(static_cast<const __nv_bfloat16*>(mask) + from, mn, keys, i, step);
   return bias2(top);
+}
+__device__ __forceinline__ float largest_bias(const Args& a, int b, int i, int step) {
+  return largest_bias(a.mask, a.mask_kind, b * a.mb, a.mn, a.Nk, i, step);
 }
 __device__ __forceinline__ bool is_additive(const Args& a) {
   return a.mask_kind != kMaskNone && a.mask_kind != kMaskBool;

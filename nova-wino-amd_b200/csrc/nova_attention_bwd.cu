@@ -208,23 +208,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   };
   // lse is relative to the sample's largest bias.
-  float ref = 0.f;
+  if (MASK && kWalkQ) set_bias(kt_fix, 0);
   if (MASK && is_additive(p.a)) {
     const float part = warp_most(largest_bias(p.a, b, tid, kThreads));
     if ((tid & 31) == 0) refs[warp] = part;
-    __syncthreads();
+  }
+  ok = wait_phase(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
+  if (MASK && kWalkQ && ok) clear_masked(s_fix, 0, true);
+  if (!__syncthreads_and(ok)) ok = false;
+  if (warp == 0 && ok) ok = start_scores(0);
+  float ref = 0.f;
+  if (MASK && is_additive(p.a)) {
     ref = refs[0];
 #pragma unroll
     for (int w = 1; w < kThreads / 32; ++w) ref = fmaxf(ref, refs[w]);
     if (ref == -INFINITY) ref = 0.f;  // no key takes part
   }
-  ok = wait_phase(bf, 0, &abort_flag, &g_status, kDevTimeoutProducer);
-  if (MASK && kWalkQ) {
-    set_bias(kt_fix, 0);
-    if (ok) clear_masked(s_fix, 0, true);
-  }
-  if (!__syncthreads_and(ok)) ok = false;
-  if (warp == 0 && ok) ok = start_scores(0);
 
   const float c = p.a.scale * kLog2e;
   const int n0 = (chunks + 1) / 2;
@@ -239,11 +238,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float v = p.a.lse_in[row0 + row];
     return v == -INFINITY ? INFINITY : v;
   };
-  auto row_delta = [&](int t, float row_lse) {
-    return row_lse == INFINITY ? 0.f : p.a.delta[row0 + t * kRows + r];
+  auto row_delta = [&](int t) {
+    const int row = t * kRows + r;
+    return row < p.a.Nq ? p.a.delta[row0 + row] : 0.f;
   };
+  // A sample without keys (all its rows are) passes nothing on, whatever its q and do hold.
+  const uint32_t keep = MASK && p.a.lse_in[row0] == -INFINITY ? 0u : ~0u;
   float lse = row_lse(t_first);
-  float delta = MODE == kBoth ? 0.f : row_delta(t_first, lse);
+  float delta = MODE == kBoth ? 0.f : row_delta(t_first);
 
   int i = 0;
   for (; i < steps; ++i) {  // leaves early only where all threads do
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float lse_next = 0.f, delta_next = 0.f;
     if (kWalkQ && i + 1 < steps) {
       lse_next = row_lse(t_first + i + 1);
-      if (MODE == kKeys) delta_next = row_delta(t_first + i + 1, lse_next);
+      if (MODE == kKeys) delta_next = row_delta(t_first + i + 1);
     }
     ok = wait_phase(bs, i & 1, &abort_flag, &g_status, kDevTimeoutMma);
     __syncwarp();
@@ -275,15 +277,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     tmem_wait_ld();
     tc_fence_before();
-    // A row without keys passes nothing on, whatever q and do hold there.
-    if (MASK && __any_sync(~0u, lse == INFINITY)) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (u < count && lse == INFINITY) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[u][e] = g[u][e] = 0u;
-        }
-    }
     float2 sums = make_float2(0.f, 0.f);
     float top = 0.f;
 #pragma unroll
@@ -449,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            w[e] = pack2<T>(__uint_as_float(o[u][2 * e]) * f, __uint_as_float(o[u][2 * e + 1]) * f);
+            w[e] = keep & pack2<T>(__uint_as_float(o[u][2 * e]) * f, __uint_as_float(o[u][2 * e + 1]) * f);
           const uint32_t at = s_p + (uint32_t)(ck >> 2) * (kRows * 128);
           st_shared_v4(at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
           st_shared_v4(at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);
@@ -528,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_ld();
         float d[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) d[e] = __uint_as_float(o[e]) * f;
+        for (int e = 0; e < 16; ++e) d[e] = keep ? __uint_as_float(o[e]) * f : 0.f;
         if (row < p.a.Nq) {
 #pragma unroll
           for (int e = 0; e < 16; e += 8)

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ alignas(8) float bias[kRows];
-  __shared__ float refs[kRows / 32];  // largest bias of the sample, a copy for each warp
+  __shared__ float refs[4];  // largest bias of the sample, a copy for each warp
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(~0u, tid >> 5, 0);  // the same for the warp, and known to be
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -256,22 +256,18 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
     // Who reads lse wants the largest bias: the four warps look for the first sample's
     // together (none of them can have given up yet), for a later one's each by itself.
     const bool wants_ref = MASK && is_additive(p.a) && (p.a.lse || p.splits > 1);
-    int b_seen = head0 / p.a.H;
-    if (wants_ref) {
-      const float part = warp_most(largest_bias(p.a, b_seen, tid, kRows));
-      if (lane == 0) refs[warp] = part;
-      asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory");
-      float top = refs[0];
-#pragma unroll
-      for (int i = 1; i < kRows / 32; ++i) top = fmaxf(top, refs[i]);
-      asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory");
-      if (lane == 0) refs[warp] = top;
-    }
+    int b_seen = -1;
     for (int t = 0; t < tiles && ok; ++t) {
       const Spot at = spot(t);
       const int b = at.b, h = at.h;
       if (wants_ref && b != b_seen) {
-        const float top = warp_most(largest_bias(p.a, b, lane, 32));
+        float top = warp_most(largest_bias(p.a, b, t ? lane : tid, t ? 32 : kRows));
+        if (t == 0) {
+          if (lane == 0) refs[warp] = top;
+          asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory");
+          top = fmaxf(fmaxf(refs[0], refs[1]), fmaxf(refs[2], refs[3]));
+          asm volatile("bar.sync 1, %0;" ::"n"(kRows) : "memory");
+        }
         if (lane == 0) refs[warp] = top;
         b_seen = b;
       }

@@ -278,3 +278,19 @@ def test_cross_sample_without_keys_passes_nothing_on(dtype, mask, Nk, poison):
         assert all(torch.equal(got[n], want[n]) and (got[n][1] == 0).all() for n in want)
         for t, h in zip(bad, held):
             t[1] = h
+
+
+@pytest.mark.parametrize("B,Nq,Nk,H,D", [(300, 20, 50, 2, 32), (49, 20, 288, 3, 160), (200, 3, 300, 2, 64)])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_cross_one_bias_for_all_keys_of_each_sample(dtype, B, Nq, Nk, H, D):
+    """Blocks that go from one sample to the next, whose biases differ."""
+    q, k, v, _, do = cross_case(B, Nq, Nk, H, D, dtype, wide=0.5)
+    mask = (-1e9 * (1 + torch.arange(B, device="cuda") % 5)).float()[:, None].expand(B, Nk)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    o = nova_cross_attention(*leaves, key_mask=mask)
+    got = dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)), o=o.detach())
+    d = [t.double() for t in (q, k, v, do)]
+    flat = P.cross_attention(torch.zeros_like(d[0]), *d[1:3], None, D ** -0.5, d[3], dtype)
+    keys = P.cross_attention(d[0], torch.zeros_like(d[1]), d[2], None, D ** -0.5, d[3], dtype)
+    for name, want in (("o", flat), ("dq", flat), ("dv", flat), ("dk", keys)):
+        near(got[name], want[name], want[name + "_tol"], name)
