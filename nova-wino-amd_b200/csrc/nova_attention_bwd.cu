@@ -23,11 +23,12 @@
 // by a power of two that follows the largest |dP| and |delta| of the block's walk.
 //
 // What bounds it.  8 x 1024 queries x 8 heads x 80, 77 keys, FP16, forward and gradient:
-// 41 us.  One block to an SM, and a tile's steps follow one another; before arithmetic
+// 41.5 us.  One block to an SM, and a tile's steps follow one another; before arithmetic
 // was paired a 128-query tile took about 9,000 cycles: scores and dP waited for 1,700 to
 // 2,400, P 2,100, exchange 490, dS 860, products 1,600, dQ 1,800.  Pairing, with row sums by
-// groups of lanes, took 3 x 1021 queries to 333 keys from 89 us to 76.  The products are too
-// small to keep the tensor cores busy (9 % of their cycles).
+// groups of lanes, took 3 x 1021 queries to 333 keys from 89 us to 76; their additive
+// biases' largest, and what it is taken off, cost 3 again (80).  The products are too small
+// to keep the tensor cores busy (9 % of their cycles).
 #include <cuda_runtime.h>
 
 #include "nova_attention.cuh"
@@ -442,7 +443,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t w[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            w[e] = keep & pack2<T>(__uint_as_float(o[u][2 * e]) * f, __uint_as_float(o[u][2 * e + 1]) * f);
+            w[e] = keep &
+                   pack2<T>(__uint_as_float(o[u][2 * e]) * f, __uint_as_float(o[u][2 * e + 1]) * f);
           const uint32_t at = s_p + (uint32_t)(ck >> 2) * (kRows * 128);
           st_shared_v4(at + sw128(r, (ck & 3) * 2), w[0], w[1], w[2], w[3]);
           st_shared_v4(at + sw128(r, (ck & 3) * 2 + 1), w[4], w[5], w[6], w[7]);

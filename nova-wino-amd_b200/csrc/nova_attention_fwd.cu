@@ -532,13 +532,14 @@ __global__ void __launch_bounds__(kThreads, kBlocks) forward_tc(const __grid_con
 //      the B fragments of eight products, one for each element, by pairing halves of
 //      two keys; the columns of product j are elements j, 8 + j, 16 + j, ...
 //
-// The loads of a step are on their way together.  Rows of keys that take no part are not read.  The keys are split over blocks (`per` keys
-// each) and over a block's warps; the warps join in shared memory, up to eight blocks
-// as one cluster through distributed shared memory, more through the workspace.
+// The loads of a step are on their way together.  Rows of keys that take no part are not
+// read.  The keys are split over blocks (`per` keys each) and over a block's warps; the
+// warps join in shared memory, up to eight blocks as one cluster through distributed
+// shared memory, more through the workspace.
 constexpr int kTokenBiases = 1024;  // keys whose biases are staged together
 constexpr int kTokenWarps = 4, kTokenQueries = 8, kTokenCluster = 8;
 // Steps of 16 keys on their way together, with five blocks' registers on an SM (three for
-// wide heads): 4 x 2041 keys x 20 heads in 15.5 us, with a mask 17.1 (two steps: 19.4).
+// wide heads): 4 x 2041 keys x 20 heads in 15.3 us, with a mask 16.6 (two steps: 19.4).
 __host__ __device__ constexpr int token_steps(int DB, bool mask) { return DB == 1 && !mask ? 2 : 1; }
 
 __device__ __forceinline__ float peer_float(const float* p, int rank) {
@@ -620,89 +621,89 @@ __global__ void __launch_bounds__(kTokenWarps * 32, DB == 1 ? 5 : 3)
       __syncthreads();
     }
     for (int k0 = c0 + warp * kKeys; k0 < c1; k0 += kTokenWarps * kKeys) {
-    // The biases of this lane's keys 2t, 2t+1, 2t+8, 2t+9 of a step, as its scores are;
-    // minus infinity for a key that is out.
-    float add[S][4];
-    uint4 kr[S][2][2 * DB], vr[S][4][DB];
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int key = k0 + 16 * s + 8 * u + g;
-        const bool in = MASK ? biases[key - c0] != -INFINITY : key < c1;
-        const T* at = kp + (long long)key * a.ks.n;
-#pragma unroll
-        for (int i = 0; i < 2 * DB; ++i) {
-          kr[s][u][i] = none;
-          if (in && i * 32 + t * 8 < a.D) kr[s][u][i] = *reinterpret_cast<const uint4*>(at + i * 32);
+      // The biases of this lane's keys 2t, 2t+1, 2t+8, 2t+9 of a step, as its scores are;
+      // minus infinity for a key that is out.
+      float add[S][4];
+      uint4 kr[S][2][2 * DB], vr[S][4][DB];
+  #pragma unroll
+      for (int s = 0; s < S; ++s) {
+  #pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int key = k0 + 16 * s + 8 * u + g;
+          const bool in = MASK ? biases[key - c0] != -INFINITY : key < c1;
+          const T* at = kp + (long long)key * a.ks.n;
+  #pragma unroll
+          for (int i = 0; i < 2 * DB; ++i) {
+            kr[s][u][i] = none;
+            if (in && i * 32 + t * 8 < a.D) kr[s][u][i] = *reinterpret_cast<const uint4*>(at + i * 32);
+          }
+        }
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + 16 * s + 2 * t + (e & 1) + (e >> 1) * 8;
+          add[s][e] = MASK ? biases[key - c0] : key < c1 ? 0.f : -INFINITY;
+          const T* at = vp + (long long)key * a.vs.n;
+  #pragma unroll
+          for (int i = 0; i < DB; ++i) {
+            vr[s][e][i] = none;
+            if (add[s][e] != -INFINITY && i * 64 + g * 8 < a.D)
+              vr[s][e][i] = *reinterpret_cast<const uint4*>(at + i * 64);
+          }
         }
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + 16 * s + 2 * t + (e & 1) + (e >> 1) * 8;
-        add[s][e] = MASK ? biases[key - c0] : key < c1 ? 0.f : -INFINITY;
-        const T* at = vp + (long long)key * a.vs.n;
-#pragma unroll
+      float x[S][2][2];
+      float top = m;
+  #pragma unroll
+      for (int s = 0; s < S; ++s)
+  #pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          x[s][u][0] = x[s][u][1] = 0.f;
+  #pragma unroll
+          for (int i = 0; i < 2 * DB; ++i) {
+            mma_rows8<T>(x[s][u], q[i].x, q[i].y, kr[s][u][i].x, kr[s][u][i].y);
+            mma_rows8<T>(x[s][u], q[i].z, q[i].w, kr[s][u][i].z, kr[s][u][i].w);
+          }
+  #pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float w = add[s][2 * u + e];
+            x[s][u][e] = w == -INFINITY ? -INFINITY : fmaf(x[s][u][e], c, w);
+            top = fmaxf(top, x[s][u][e]);
+          }
+        }
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+      const float base = top == -INFINITY ? 0.f : top;
+      const float f = ex2(m - base);
+      m = top;
+      l *= f;
+      if (__any_sync(~0u, f != 1.f)) {
+  #pragma unroll
+        for (int i = 0; i < DB * 8; ++i) o[i][0] *= f, o[i][1] *= f;
+      }
+  #pragma unroll
+      for (int s = 0; s < S; ++s) {
+  #pragma unroll
+        for (int u = 0; u < 2; ++u)
+  #pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            x[s][u][e] = add[s][2 * u + e] == -INFINITY ? 0.f : ex2(x[s][u][e] - base);
+            l += x[s][u][e];
+          }
+        const uint32_t a0 = pack2<T>(x[s][0][0], x[s][0][1]), a2 = pack2<T>(x[s][1][0], x[s][1][1]);
+  #pragma unroll
         for (int i = 0; i < DB; ++i) {
-          vr[s][e][i] = none;
-          if (add[s][e] != -INFINITY && i * 64 + g * 8 < a.D)
-            vr[s][e][i] = *reinterpret_cast<const uint4*>(at + i * 64);
+          const auto pair = [&](uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int e) {
+            mma_rows8<T>(o[i * 8 + e], a0, a2, __byte_perm(v0, v1, 0x5410), __byte_perm(v2, v3, 0x5410));
+            mma_rows8<T>(o[i * 8 + e + 1], a0, a2, __byte_perm(v0, v1, 0x7632),
+                         __byte_perm(v2, v3, 0x7632));
+          };
+          pair(vr[s][0][i].x, vr[s][1][i].x, vr[s][2][i].x, vr[s][3][i].x, 0);
+          pair(vr[s][0][i].y, vr[s][1][i].y, vr[s][2][i].y, vr[s][3][i].y, 2);
+          pair(vr[s][0][i].z, vr[s][1][i].z, vr[s][2][i].z, vr[s][3][i].z, 4);
+          pair(vr[s][0][i].w, vr[s][1][i].w, vr[s][2][i].w, vr[s][3][i].w, 6);
         }
       }
     }
-    float x[S][2][2];
-    float top = m;
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        x[s][u][0] = x[s][u][1] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * DB; ++i) {
-          mma_rows8<T>(x[s][u], q[i].x, q[i].y, kr[s][u][i].x, kr[s][u][i].y);
-          mma_rows8<T>(x[s][u], q[i].z, q[i].w, kr[s][u][i].z, kr[s][u][i].w);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float w = add[s][2 * u + e];
-          x[s][u][e] = w == -INFINITY ? -INFINITY : fmaf(x[s][u][e], c, w);
-          top = fmaxf(top, x[s][u][e]);
-        }
-      }
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float f = ex2(m - base);
-    m = top;
-    l *= f;
-    if (__any_sync(~0u, f != 1.f)) {
-#pragma unroll
-      for (int i = 0; i < DB * 8; ++i) o[i][0] *= f, o[i][1] *= f;
-    }
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[s][u][e] = add[s][2 * u + e] == -INFINITY ? 0.f : ex2(x[s][u][e] - base);
-          l += x[s][u][e];
-        }
-      const uint32_t a0 = pack2<T>(x[s][0][0], x[s][0][1]), a2 = pack2<T>(x[s][1][0], x[s][1][1]);
-#pragma unroll
-      for (int i = 0; i < DB; ++i) {
-        const auto pair = [&](uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3, int e) {
-          mma_rows8<T>(o[i * 8 + e], a0, a2, __byte_perm(v0, v1, 0x5410), __byte_perm(v2, v3, 0x5410));
-          mma_rows8<T>(o[i * 8 + e + 1], a0, a2, __byte_perm(v0, v1, 0x7632),
-                       __byte_perm(v2, v3, 0x7632));
-        };
-        pair(vr[s][0][i].x, vr[s][1][i].x, vr[s][2][i].x, vr[s][3][i].x, 0);
-        pair(vr[s][0][i].y, vr[s][1][i].y, vr[s][2][i].y, vr[s][3][i].y, 2);
-        pair(vr[s][0][i].z, vr[s][1][i].z, vr[s][2][i].z, vr[s][3][i].z, 4);
-        pair(vr[s][0][i].w, vr[s][1][i].w, vr[s][2][i].w, vr[s][3][i].w, 6);
-      }
-    }
-  }
   }
   l += __shfl_xor_sync(~0u, l, 1);
   l += __shfl_xor_sync(~0u, l, 2);

@@ -21,9 +21,10 @@
 //
 // Statistics.  The resident form takes the mean of its registers, then the squared
 // deviations from it; a streaming thread keeps sums relative to the first value it
-// sees.  A mean far from zero thus costs no digits.  Parts are joined as means and
-// squared deviations, sums over samples in 64 bits.  Every sum has a fixed order:
-// results repeat bit for bit.
+// sees: a mean far from zero costs the statistics no digits.  (The passes fold it into an
+// offset, rounded once at its own size: as a subtraction of the rounded mean would be.)
+// Parts are joined as means and squared deviations, a group's and the samples' in 64
+// bits.  Every sum has a fixed order: results repeat bit for bit.
 //
 // What bounds it.  8 x 960 x 128 x 128 FP16 forward, 504 MB at least: 156 us, 49 % of the
 // measured copy bandwidth (the summing pass 53 us, 4.8 TB/s; the writing pass 101 us,
@@ -1028,8 +1029,8 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
         k.ty = (k.ppc + nv - 1) / nv;
         // The share of the vectors that is read again, three times over.  It pays for
         // FP32, whose vectors need no conversion, on most of the SMs and with rows of
-        // whole lines: 4x320x61x67 15.0 us, streaming 18.6; 2x640x64x64 15.0, streaming
-        // 21.1.  Not in FP16 (8x320x64x64 25.2 us, streaming 24.3; values one by one
+        // whole lines: 4x320x61x67 15.0 us, streaming 18.6; 2x640x64x64 15.4, streaming
+        // 21.1.  Not in FP16 (8x320x64x64 25.2 us, streaming 24.7; values one by one
         // 4x76x64x70 19.1, streaming 14.8), on 32 blocks (1x128x120x120 in 4 groups 16.7,
         // streaming 14.7) or in rows of 80 bytes (1x320x128x128 29.4, streaming 21.4).
         double again = 0;
@@ -1046,7 +1047,7 @@ bool make_slab(int B, int HW, int C, int G, int V, bool grad, int sms, Slab* bes
         // the gradient, whose streaming form has four launches): its phases do not
         // overlap, so further waves cost it more than the second read it saves.
         // Measured, FP16: 8x640x32x32 forward 12.5 us (streaming 20), 8x320x64x64 in
-        // two waves 27.7 us (streaming 22).
+        // two waves 27.7 us (streaming 24.7).
         const long long blocks = (long long)B * k.nblk * cs;
         const int per_sm = std::min(32, 65536 / ((nv * 4 * (grad ? 2 : 1) + 64) * k.threads));
         const long long room = (long long)sms * per_sm;

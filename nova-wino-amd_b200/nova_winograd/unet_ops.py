@@ -415,9 +415,20 @@ def nova_cross_attention(q, k, v, key_mask=None, scale=None):
         scale:    default 1 / sqrt(D).
 
     A key that takes no part is never multiplied, whatever k and v hold there.  A
-    query without keys gets zeros and passes no gradient on.  Returns [B, Nq, H, D],
-    contiguous.  Products are accumulated and the softmax is computed in 32 bits.
-    Gradients for q, k and v repeat bit for bit.
+    query without keys gets zeros and passes no gradient on, whatever it and its
+    gradient hold.  Finite biases count as 32-bit sums with them do: with the lowest
+    value, or -1e9, for every key of a sample its rows are uniform.  Returns
+    [B, Nq, H, D], contiguous.
+
+    Products are accumulated and the softmax is computed in 32 bits.  Probabilities,
+    and in the gradient their derivatives too, are rounded to q's type once, as
+    operands of the products with v, k, q and the incoming gradient; what the rounding
+    of the output left off goes to the gradient in q's type as well.  Gradients for q,
+    k and v repeat bit for bit.
+
+    The kernels' waits are bounded.  One that expires leaves an output that is not to
+    be used, and ``nova_cross_attention_status()`` of the library (``ops.get_lib()``)
+    reports it.
     """
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"q, k and v must be [B, N, H, D], got {list(q.shape)}, {list(k.shape)} "
