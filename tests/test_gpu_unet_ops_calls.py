@@ -294,3 +294,22 @@ def test_cross_one_bias_for_all_keys_of_each_sample(dtype, B, Nq, Nk, H, D):
     keys = P.cross_attention(d[0], torch.zeros_like(d[1]), d[2], None, D ** -0.5, d[3], dtype)
     for name, want in (("o", flat), ("dq", flat), ("dv", flat), ("dk", keys)):
         near(got[name], want[name], want[name + "_tol"], name)
+
+
+def test_unet_caller_in_64_bits_keeps_torchs_layers():
+    """What the operators do not take stays with torch's layers, switched on or not."""
+    import unet_callers as U
+    spec = U.UNetSpec(channels=(32, 64), attn_depth=(1, 1), mid_depth=1, context_dim=16, heads=4,
+                      groups=8)
+    torch.manual_seed(0)
+    model = U.UNet(spec).cuda().double().to(memory_format=torch.channels_last).eval()
+    norm, x = model.norm_out, rand(2, 32, 9, 9, seed=1).double()
+    x = x.contiguous(memory_format=torch.channels_last)
+    U.use_nova_ops(model)
+    assert torch.equal(U.norm_act(norm, x, True, "silu"), U.norm_act(norm, x, False, "silu"))
+    layer = model.mid_attn
+    ctx = rand(2, 5, 16, seed=2).double()
+    h = rand(2, 64, 6, 6, seed=3).double().contiguous(memory_format=torch.channels_last)
+    on = layer(h, ctx)
+    U.use_nova_ops(model, False)
+    assert torch.equal(layer(h, ctx), on)

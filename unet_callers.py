@@ -82,7 +82,8 @@ def use_nova_ops(model, on=True):
 
 def norm_act(norm, x, nova, act=None, shift=None):
     """``act(norm(x + shift[:, :, None, None]))`` of an nn.GroupNorm."""
-    if nova and x.is_cuda and x.is_contiguous(memory_format=torch.channels_last):
+    if (nova and x.is_cuda and x.dtype in (torch.float16, torch.bfloat16, torch.float32)
+            and x.is_contiguous(memory_format=torch.channels_last)):
         from nova_winograd import nova_group_norm
         return nova_group_norm(x, norm.num_groups, norm.weight, norm.bias, norm.eps, act, shift)
     h = norm(x if shift is None else x + shift[:, :, None, None])
